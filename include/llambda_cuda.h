@@ -385,6 +385,140 @@ LLAMBDA_CUDA_API int llambda_cuda_moe_forward_static_scratch(const llambda_cuda_
                                                              void* cuda_stream);
 
 /* ------------------------------------------------------------------------
+ * Choice of experts from router logits, and the routed experts' products in
+ * 8-bit floating point.  These entry points have no counterpart in the
+ * reference, whose router rules are those of its two architectures and whose
+ * weights are GGML blocks; they serve checkpoints with other routing rules
+ * and with e4m3 weights.
+ *
+ * Device forms take device memory of the current device (sessions: of the
+ * session's device), enqueue on `cuda_stream` and return without waiting.
+ * They allocate nothing, use no memory but what they are given, and may be
+ * captured into a CUDA graph; two calls may overlap when their outputs and
+ * workspaces are apart.  Element types are tags: LLAMBDA_CUDA_TYPE_F32 or
+ * LLAMBDA_CUDA_TYPE_BF16.  Row strides are in elements. */
+#define LLAMBDA_CUDA_TYPE_BF16 30
+
+#define LLAMBDA_CUDA_SCORE_SOFTMAX 0
+#define LLAMBDA_CUDA_SCORE_SIGMOID 1
+
+typedef struct {
+  int experts;        /* 1..1024 */
+  int top_k;          /* 1..32, at most the experts of top_groups groups */
+  int score;          /* LLAMBDA_CUDA_SCORE_* over a token's logits */
+  int groups;         /* the experts form this many equal groups (1..32) ... */
+  int top_groups;     /* ... of which a token chooses among its best (1..groups) */
+  int group_top;      /* a group's rank: its largest choice (1) or the sum of its
+                         two largest (2; needs two experts a group) */
+  int renormalise;    /* 1: weights divided by their sum */
+  float weight_scale; /* and multiplied by this */
+} llambda_cuda_route_desc;
+
+/* For each of `tokens` rows of logits [tokens][experts] (row stride ld): the
+ * score s of every expert, the choice c = s + bias (bias [experts] F32 or
+ * NULL), and the top_k experts of largest c within the kept groups, in
+ * decreasing order, equal ones by index; selected [tokens][top_k], weights
+ * [tokens][top_k] = s of the chosen (renormalised, scaled).  The order is that
+ * of exact scores.  An expert with a logit of -inf has score 0 and is chosen
+ * last, one with NaN after it; weights whose sum is 0 stay 0. */
+LLAMBDA_CUDA_API int llambda_cuda_route_device(const llambda_cuda_route_desc* desc,
+                                               int logits_type, const void* device_logits,
+                                               int64_t ld, const float* device_bias, size_t tokens,
+                                               int32_t* device_selected, float* device_weights,
+                                               void* cuda_stream);
+
+/* The same on host buffers: logits [tokens][experts] F32. */
+LLAMBDA_CUDA_API int llambda_cuda_route(const llambda_cuda_route_desc* desc, const float* logits,
+                                        const float* bias, size_t tokens, int32_t* selected,
+                                        float* weights);
+
+/* Rows x [tokens][cols] (stride ldx, F32 or BF16) to e4m3 with one scale per
+ * row and 128 columns: scale = max(max|x| / 448, 2^-126), q = e4m3(x / scale),
+ * both divisions and the rounding to nearest.  q [tokens][round_up(cols, 16)]
+ * (zeros past cols), scales F32 [ceil(cols / 128)][round_up(tokens, 4)] (zeros
+ * past tokens), both 16-byte aligned.  A NaN or an infinity makes its block NaN
+ * (an infinite block's finite values become 0). */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_quantize_device(int type, const void* device_x, int64_t ldx,
+                                                      size_t tokens, uint64_t cols, void* device_q,
+                                                      float* device_scales, void* cuda_stream);
+
+/* E4M3 matrices with one F32 scale per 128 x 128 block: data [ne2][ne1][ne0]
+ * bytes (ne0 = columns, ne1 = rows, ne2 = experts), scales
+ * [ne2][ceil(ne1 / 128)][ceil(ne0 / 128)], finite. */
+typedef struct {
+  uint64_t ne0, ne1, ne2;
+  const void* data;
+  const float* scales;
+} llambda_cuda_fp8_tensor;
+
+typedef struct llambda_cuda_fp8_session llambda_cuda_fp8_session;
+
+/* One matrix (ne2 1) as a projection.  on_device 0: host memory, copied; 1:
+ * device memory of the current device, borrowed until the session is
+ * destroyed (data 16-byte aligned, ne0 a multiple of 16). */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor,
+                                                     int on_device,
+                                                     llambda_cuda_fp8_session** result);
+LLAMBDA_CUDA_API void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session* session);
+
+/* Host buffers: out [tokens][ne1] = W . x[t], x [tokens][ne0] quantised as by
+ * llambda_cuda_fp8_quantize_device; products of a block summed exactly enough
+ * for fp32, blocks added in fp32. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* session, const float* x,
+                                                  size_t tokens, float* out);
+
+/* Bytes of device workspace that a device call over `tokens` rows needs. */
+LLAMBDA_CUDA_API size_t llambda_cuda_fp8_session_workspace(const llambda_cuda_fp8_session* session,
+                                                           size_t tokens);
+
+/* Device form: x [tokens][ne0] of x_type and stride ldx, out [tokens][ne1] of
+ * out_type and stride ldo; workspace 256-byte aligned. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run_device(
+    llambda_cuda_fp8_session* session, int x_type, const void* device_x, int64_t ldx, size_t tokens,
+    int out_type, void* device_out, int64_t ldo, void* workspace, size_t workspace_bytes,
+    void* cuda_stream);
+
+/* As above over rows that are quantised already (several projections of one
+ * input): q and scales as llambda_cuda_fp8_quantize_device writes them. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run_quantized(
+    llambda_cuda_fp8_session* session, const void* device_q, const float* device_scales,
+    size_t tokens, int out_type, void* device_out, int64_t ldo, void* cuda_stream);
+
+/* Status word of the session's device-side checks, cleared by reading (0 = ok;
+ * 2 = a wait inside a kernel timed out); -1 on a CUDA error. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_session_status(llambda_cuda_fp8_session* session);
+
+typedef struct llambda_cuda_fp8_moe_session llambda_cuda_fp8_moe_session;
+
+/* The routed experts of one layer: up and (or data NULL) gate [E][I][H], down
+ * [E][O][I].  Expert e of an input x gives down_e . q(h), h = silu(gate_e . x)
+ * * (up_e . x), or relu(up_e . x)^2 without gate, q the quantisation above
+ * (x is quantised too).  E at most 1024.  on_device as for a projection. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_moe_session_create(const llambda_cuda_fp8_tensor* gate,
+                                                         const llambda_cuda_fp8_tensor* up,
+                                                         const llambda_cuda_fp8_tensor* down,
+                                                         int on_device,
+                                                         llambda_cuda_fp8_moe_session** result);
+LLAMBDA_CUDA_API void llambda_cuda_fp8_moe_session_destroy(llambda_cuda_fp8_moe_session* session);
+
+/* Host buffers: out [tokens][O] = sum over j < top_k, in order, of
+ * weights[t][j] * expert selected[t][j] of x[t].  An entry whose expert is
+ * outside 0..E-1 (one that another process owns, a padded row) adds nothing;
+ * a token without any entry gives zeros. */
+LLAMBDA_CUDA_API int llambda_cuda_fp8_moe_session_run(llambda_cuda_fp8_moe_session* session,
+                                                      const float* x, size_t tokens, int top_k,
+                                                      const int32_t* selected,
+                                                      const float* weights, float* out);
+LLAMBDA_CUDA_API size_t llambda_cuda_fp8_moe_session_workspace(
+    const llambda_cuda_fp8_moe_session* session, size_t tokens, int top_k);
+LLAMBDA_CUDA_API int llambda_cuda_fp8_moe_session_run_device(
+    llambda_cuda_fp8_moe_session* session, int x_type, const void* device_x, int64_t ldx,
+    size_t tokens, int top_k, const int32_t* device_selected, const float* device_weights,
+    int out_type, void* device_out, int64_t ldo, void* workspace, size_t workspace_bytes,
+    void* cuda_stream);
+LLAMBDA_CUDA_API int llambda_cuda_fp8_moe_session_status(llambda_cuda_fp8_moe_session* session);
+
+/* ------------------------------------------------------------------------
  * Synthetic GGUF data for benchmarks and tests (seeded, counter-based; the
  * same generator runs on the host in the test oracle, byte for byte).
  * type: Q4_K / Q6_K write `count` super-blocks starting at block `first`;

@@ -11,9 +11,12 @@ from ._native import (ARCH_NEMOTRON_H_MOE, ARCH_QWEN3NEXT, TYPE_F32, TYPE_Q4_K, 
                       GgufFile, ProjectionSession, bridge_version, device_free,
                       lib, prefill_min_tokens, probe, row_bytes, runtime_version,
                       set_prefill_min_tokens, sha256, synth_fill_device)
+from .experts import (Fp8MoeSession, Fp8ProjectionSession, fp8_quantize,  # noqa: F401
+                      route_experts)
 
 __all__ = ["ARCH_NEMOTRON_H_MOE", "ARCH_QWEN3NEXT", "TYPE_F32", "TYPE_Q4_K", "TYPE_Q5_0",
            "TYPE_Q5_K", "TYPE_Q6_K", "TYPE_Q8_0",
+           "Fp8MoeSession", "Fp8ProjectionSession", "fp8_quantize", "route_experts",
            "GgufFile", "LlambdaCudaError", "MoeSession", "ProjectionSession", "bridge_version",
            "device_free", "lib",
            "prefill_min_tokens", "set_prefill_min_tokens",

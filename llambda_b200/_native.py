@@ -19,6 +19,8 @@ LIB_PATH = os.path.join(HERE, "libllambda_cuda.so")
 
 TYPE_F32, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K = 0, 12, 13, 14
 TYPE_Q5_0, TYPE_Q8_0 = 6, 8  # 32-value blocks: projection sessions only
+TYPE_BF16 = 30  # element type of device operands (with TYPE_F32)
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ARCH_QWEN3NEXT, ARCH_NEMOTRON_H_MOE = 0, 1
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q5_K: 176, TYPE_Q6_K: 210}
 BLOCK32_BYTES = {TYPE_Q5_0: 22, TYPE_Q8_0: 34}
@@ -60,6 +62,17 @@ class MoeDesc(C.Structure):
                 ("input_norm", C.c_void_p), ("norm_epsilon", C.c_float),
                 ("add_residual", C.c_int),
                 ("latent_down", Tensor), ("latent_up", Tensor)]
+
+
+class RouteDesc(C.Structure):
+    _fields_ = [("experts", C.c_int), ("top_k", C.c_int), ("score", C.c_int),
+                ("groups", C.c_int), ("top_groups", C.c_int), ("group_top", C.c_int),
+                ("renormalise", C.c_int), ("weight_scale", C.c_float)]
+
+
+class Fp8Tensor(C.Structure):
+    _fields_ = [("ne0", C.c_uint64), ("ne1", C.c_uint64), ("ne2", C.c_uint64),
+                ("data", C.c_void_p), ("scales", C.c_void_p)]
 
 
 # name -> (restype, argtypes); every symbol the public header declares.
@@ -111,6 +124,30 @@ SIGNATURES = {
     "llambda_cuda_moe_session_attach_peers": (C.c_int, [_vp, C.c_int, C.c_int,
                                                         C.POINTER(_vp), _sz]),
     "llambda_cuda_moe_forward_static_scratch": (C.c_int, [C.POINTER(MoeDesc), _vp, _sz, _vp, _vp]),
+    "llambda_cuda_route_device": (C.c_int, [C.POINTER(RouteDesc), C.c_int, _vp, C.c_int64, _vp, _sz,
+                                            _vp, _vp, _vp]),
+    "llambda_cuda_route": (C.c_int, [C.POINTER(RouteDesc), _vp, _vp, _sz, _vp, _vp]),
+    "llambda_cuda_fp8_quantize_device": (C.c_int, [C.c_int, _vp, C.c_int64, _sz, _u64, _vp, _vp,
+                                                   _vp]),
+    "llambda_cuda_fp8_session_create": (C.c_int, [C.POINTER(Fp8Tensor), C.c_int, C.POINTER(_vp)]),
+    "llambda_cuda_fp8_session_destroy": (None, [_vp]),
+    "llambda_cuda_fp8_session_run": (C.c_int, [_vp, _vp, _sz, _vp]),
+    "llambda_cuda_fp8_session_workspace": (_sz, [_vp, _sz]),
+    "llambda_cuda_fp8_session_run_device": (C.c_int, [_vp, C.c_int, _vp, C.c_int64, _sz, C.c_int,
+                                                      _vp, C.c_int64, _vp, _sz, _vp]),
+    "llambda_cuda_fp8_session_run_quantized": (C.c_int, [_vp, _vp, _vp, _sz, C.c_int, _vp,
+                                                         C.c_int64, _vp]),
+    "llambda_cuda_fp8_session_status": (C.c_int, [_vp]),
+    "llambda_cuda_fp8_moe_session_create": (C.c_int, [C.POINTER(Fp8Tensor), C.POINTER(Fp8Tensor),
+                                                      C.POINTER(Fp8Tensor), C.c_int,
+                                                      C.POINTER(_vp)]),
+    "llambda_cuda_fp8_moe_session_destroy": (None, [_vp]),
+    "llambda_cuda_fp8_moe_session_run": (C.c_int, [_vp, _vp, _sz, C.c_int, _vp, _vp, _vp]),
+    "llambda_cuda_fp8_moe_session_workspace": (_sz, [_vp, _sz, C.c_int]),
+    "llambda_cuda_fp8_moe_session_run_device": (C.c_int, [_vp, C.c_int, _vp, C.c_int64, _sz,
+                                                          C.c_int, _vp, _vp, C.c_int, _vp,
+                                                          C.c_int64, _vp, _sz, _vp]),
+    "llambda_cuda_fp8_moe_session_status": (C.c_int, [_vp]),
     "llambda_cuda_synth_fill_device": (C.c_int, [C.c_int, _u64, _u64, _u64, _sz, C.c_float, _vp,
                                                  _vp]),
 }

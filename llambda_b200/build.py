@@ -16,9 +16,9 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllambda_cuda.so")
 
-CU_SOURCES = ["gemv.cu", "moe.cu", "prefill.cu", "gguf.cu", "capi.cu"]
+CU_SOURCES = ["gemv.cu", "moe.cu", "prefill.cu", "fp8.cu", "route.cu", "gguf.cu", "capi.cu"]
 C_SOURCES = ["sha256.c"]
-HEADERS = ["common.cuh", "engine.cuh", "kernels.h", "synth.h"]
+HEADERS = ["common.cuh", "engine.cuh", "kernels.h", "mma.cuh", "synth.h", "tcgen05.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden",

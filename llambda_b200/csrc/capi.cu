@@ -1313,6 +1313,520 @@ int llambda_cuda_synth_fill_device(int type, uint64_t seed, uint64_t stream_id, 
   });
 }
 
+// ------------------------------------------------------------------ routing, 8-bit floating point
+
+}  // extern "C"
+
+namespace {
+
+bool is_bf16(int type, const char* what) {
+  if (type != LLAMBDA_CUDA_TYPE_F32 && type != LLAMBDA_CUDA_TYPE_BF16)
+    throw Failure(std::string(what) + ": element type must be F32 or BF16, got tag " +
+                  std::to_string(type));
+  return type == LLAMBDA_CUDA_TYPE_BF16;
+}
+
+// The device whose memory p is; an address the GPU cannot read is an error
+// here rather than a fault there.
+int device_of(const void* p, const char* what) {
+  cudaPointerAttributes a{};
+  const cudaError_t e = cudaPointerGetAttributes(&a, p);
+  if (e != cudaSuccess) cudaGetLastError();
+  if (e != cudaSuccess || (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged))
+    throw Failure(std::string(what) + " must be device memory.");
+  return a.device;
+}
+
+void require_on(const void* p, int device, const char* what) {
+  const int d = device_of(p, what);
+  if (d != device)
+    throw Failure(std::string(what) + " is on device " + std::to_string(d) + ", not " +
+                  std::to_string(device) + ".");
+}
+
+void require_align(const void* p, size_t n, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % n)
+    throw Failure(std::string(what) + " must be " + std::to_string(n) + "-byte aligned.");
+}
+
+int token_count(size_t tokens) {
+  if (tokens == 0 || tokens > (1u << 24))
+    throw Failure("The token count must be in 1.." + std::to_string(1u << 24) + ".");
+  return (int)tokens;
+}
+
+// A row-major operand [tokens][cols] of element type `type` and row stride ld.
+void require_operand(int type, const void* p, int64_t ld, size_t tokens, uint64_t cols, int device,
+                     const char* what) {
+  const bool bf16 = is_bf16(type, what);
+  require_on(p, device, what);
+  require_align(p, bf16 ? 2 : 4, what);
+  if (tokens > 1 && ld < (int64_t)cols)
+    throw Failure(std::string(what) + ": the row stride is smaller than a row.");
+}
+
+lb::RouteParams route_params(const llambda_cuda_route_desc* d) {
+  if (!d) throw Failure("A routing descriptor is required.");
+  if (d->experts < 1 || d->experts > 1024) throw Failure("Expert count must be in 1..1024.");
+  if (d->score != LLAMBDA_CUDA_SCORE_SOFTMAX && d->score != LLAMBDA_CUDA_SCORE_SIGMOID)
+    throw Failure("Unknown routing score " + std::to_string(d->score));
+  if (d->groups < 1 || d->groups > 32 || d->experts % d->groups)
+    throw Failure("The experts must form 1..32 equal groups.");
+  if (d->top_groups < 1 || d->top_groups > d->groups)
+    throw Failure("top_groups must be in 1..groups.");
+  const int size = d->experts / d->groups;
+  if (d->group_top != 1 && d->group_top != 2) throw Failure("group_top must be 1 or 2.");
+  if (d->top_groups < d->groups && d->group_top > size)
+    throw Failure("group_top 2 needs at least two experts in a group.");
+  if (d->top_k < 1 || d->top_k > 32 || d->top_k > d->top_groups * size)
+    throw Failure("top_k must be in 1..32 and at most the experts of top_groups groups.");
+  return lb::RouteParams{d->experts,    d->top_k,     d->score == LLAMBDA_CUDA_SCORE_SOFTMAX,
+                         d->groups,     d->top_groups, d->group_top,
+                         d->renormalise ? 1 : 0, d->weight_scale};
+}
+
+size_t f8_quant_bytes(uint64_t cols, size_t tokens, size_t* scales_at) {
+  const size_t q = (tokens * (size_t)lb::f8_pad16((long)cols) + 255) & ~size_t(255);
+  if (scales_at) *scales_at = q;
+  return q + (((cols + 127) / 128 * (size_t)lb::f8_pad4((long)tokens) * 4 + 255) & ~size_t(255));
+}
+
+// Device copies owned by a session, freed with it.
+struct F8Owner {
+  int device = 0;
+  cudaStream_t stream = nullptr;
+  int* status = nullptr;
+  std::vector<void*> owned;
+  std::mutex mu;
+  DevBuf din, dout, dwork, dsel, dw;
+  void open() {
+    device = current_device();
+    require_b200(device);
+    cuda_check(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking), "cudaStreamCreate");
+    cuda_check(cudaMalloc(&status, sizeof(int)), "cudaMalloc");
+    cuda_check(cudaMemsetAsync(status, 0, sizeof(int), stream), "memset");
+  }
+  ~F8Owner() {
+    if (stream) cudaStreamDestroy(stream);
+    if (status) cudaFree(status);
+    for (void* p : owned) cudaFree(p);
+  }
+  lb::F8Matrix matrix(const llambda_cuda_fp8_tensor& t, bool on_device, const char* what) {
+    const std::string name(what);
+    if (!t.data || !t.scales) throw Failure(name + ": data and scales are required.");
+    const uint64_t ne2 = t.ne2 ? t.ne2 : 1;
+    if (!t.ne0 || !t.ne1) throw Failure(name + ": dimensions must be positive.");
+    if (t.ne0 > (1u << 24) || t.ne1 > (1u << 24) || ne2 > 1024) throw Failure(name + " is too large.");
+    lb::F8Matrix m{};
+    m.cols = (int)t.ne0;
+    m.rows = (int)t.ne1;
+    m.experts = (int)ne2;
+    m.pitch = lb::f8_pad16(m.cols);
+    const size_t rows = (size_t)t.ne1 * ne2;
+    const size_t nscales = ne2 * ((t.ne1 + 127) / 128) * ((t.ne0 + 127) / 128);
+    if (on_device) {
+      if (t.ne0 % 16)
+        throw Failure(name + ": e4m3 rows in device memory need a multiple of 16 columns, got " +
+                      std::to_string(t.ne0));
+      require_on(t.data, device, (name + " data").c_str());
+      require_on(t.scales, device, (name + " scales").c_str());
+      require_align(t.data, 16, (name + " data").c_str());
+      require_align(t.scales, 4, (name + " scales").c_str());
+      m.data = static_cast<const uint8_t*>(t.data);
+      m.scales = t.scales;
+      // the borrowed memory may still be being written on the default stream
+      cuda_check(cudaStreamSynchronize(nullptr), "synchronize");
+    } else {
+      void* d = dev_alloc(rows * m.pitch);
+      owned.push_back(d);
+      void* s = dev_alloc(nscales * 4);
+      owned.push_back(s);
+      cuda_check(cudaMemcpy2DAsync(d, m.pitch, t.data, t.ne0, t.ne0, rows, cudaMemcpyHostToDevice,
+                                   stream),
+                 "upload tensor");
+      cuda_check(cudaMemcpyAsync(s, t.scales, nscales * 4, cudaMemcpyHostToDevice, stream),
+                 "upload scales");
+      m.data = static_cast<const uint8_t*>(d);
+      m.scales = static_cast<const float*>(s);
+    }
+    unsigned* bad = nullptr;
+    unsigned host = 0;
+    cuda_check(cudaMalloc(&bad, sizeof(unsigned)), "cudaMalloc");
+    cudaError_t e = cudaMemsetAsync(bad, 0, sizeof(unsigned), stream);
+    if (e == cudaSuccess) e = lb::f8_check_scales(m.scales, nscales, bad, stream);
+    if (e == cudaSuccess)
+      e = cudaMemcpyAsync(&host, bad, sizeof(unsigned), cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    cudaFree(bad);
+    cuda_check(e, "scale check");
+    if (host) throw Failure(name + ": " + std::to_string(host) + " scale(s) are not finite.");
+    cuda_check(lb::f8_prepare(&m), "tensor map");
+    return m;
+  }
+  // Reads and clears the status word; the stream's work is waited for.
+  int take_status() {
+    int v = 0;
+    cuda_check(cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost), "status copy");
+    if (v) cuda_check(cudaMemset(status, 0, sizeof(int)), "clear status");
+    return v;
+  }
+  void finish(void* out, const void* dev, size_t bytes, const char* what) {
+    cuda_check(cudaMemcpyAsync(out, dev, bytes, cudaMemcpyDeviceToHost, stream), "output copy");
+    cuda_check(cudaStreamSynchronize(stream), what);
+    if (const int v = take_status())
+      throw Failure(std::string(what) + ": a wait inside a kernel timed out (device status " +
+                    std::to_string(v) + ").");
+  }
+};
+
+void require_workspace(const void* p, size_t have, size_t need, int device) {
+  if (have < need)
+    throw Failure("The workspace has " + std::to_string(have) + " bytes; this call needs " +
+                  std::to_string(need) + ".");
+  require_on(p, device, "workspace");
+  require_align(p, 256, "workspace");
+}
+
+template <typename S>
+void destroy_owner(S* s) {
+  if (!s) return;
+  try {
+    DeviceGuard g(s->device);
+    if (s->stream) cudaStreamSynchronize(s->stream);
+    delete s;
+  } catch (...) {
+    delete s;
+  }
+}
+
+}  // namespace
+
+struct llambda_cuda_fp8_session : F8Owner {
+  lb::F8Matrix w{};
+};
+
+struct llambda_cuda_fp8_moe_session : F8Owner {
+  lb::F8Moe m{};
+};
+
+namespace {
+
+void moe_call_sizes(const llambda_cuda_fp8_moe_session* s, size_t tokens, int top_k) {
+  token_count(tokens);
+  if (top_k < 1 || top_k > 1024) throw Failure("top_k must be in 1..1024.");
+  if (tokens * (size_t)top_k > (1u << 26)) throw Failure("Too many (token, expert) entries.");
+  (void)s;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llambda_cuda_route_device(const llambda_cuda_route_desc* desc, int logits_type,
+                              const void* device_logits, int64_t ld, const float* device_bias,
+                              size_t tokens, int32_t* device_selected, float* device_weights,
+                              void* cuda_stream) {
+  return guarded([&] {
+    const lb::RouteParams r = route_params(desc);
+    if (!device_logits || !device_selected || !device_weights)
+      throw Failure("Logits and outputs are required.");
+    const int T = token_count(tokens);
+    const int dev = device_of(device_logits, "logits");
+    DeviceGuard g(dev);
+    require_operand(logits_type, device_logits, ld, tokens, r.experts, dev, "logits");
+    require_on(device_selected, dev, "selected");
+    require_on(device_weights, dev, "weights");
+    require_align(device_selected, 4, "selected");
+    require_align(device_weights, 4, "weights");
+    if (device_bias) {
+      require_on(device_bias, dev, "bias");
+      require_align(device_bias, 4, "bias");
+    }
+    cuda_check(lb::launch_route(r, is_bf16(logits_type, "logits"), device_logits, ld, device_bias,
+                                T, device_selected, device_weights,
+                                static_cast<cudaStream_t>(cuda_stream)),
+               "routing launch");
+    return 0;
+  });
+}
+
+int llambda_cuda_route(const llambda_cuda_route_desc* desc, const float* logits, const float* bias,
+                       size_t tokens, int32_t* selected, float* weights) {
+  return guarded([&] {
+    const lb::RouteParams r = route_params(desc);
+    if (!logits || !selected || !weights) throw Failure("Logits and outputs are required.");
+    const int T = token_count(tokens);
+    require_b200(current_device());
+    const size_t lb_ = tokens * r.experts * 4, ob = tokens * r.top_k * 4;
+    DevBuf dl, db, ds, dw;
+    float* l = static_cast<float*>(dl.get(lb_));
+    float* b = bias ? static_cast<float*>(db.get((size_t)r.experts * 4)) : nullptr;
+    int* s = static_cast<int*>(ds.get(ob));
+    float* w = static_cast<float*>(dw.get(ob));
+    cuda_check(cudaMemcpy(l, logits, lb_, cudaMemcpyHostToDevice), "logits copy");
+    if (b) cuda_check(cudaMemcpy(b, bias, (size_t)r.experts * 4, cudaMemcpyHostToDevice), "bias copy");
+    cuda_check(lb::launch_route(r, false, l, r.experts, b, T, s, w, nullptr), "routing launch");
+    cuda_check(cudaMemcpy(selected, s, ob, cudaMemcpyDeviceToHost), "routing");
+    cuda_check(cudaMemcpy(weights, w, ob, cudaMemcpyDeviceToHost), "routing");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_quantize_device(int type, const void* device_x, int64_t ldx, size_t tokens,
+                                     uint64_t cols, void* device_q, float* device_scales,
+                                     void* cuda_stream) {
+  return guarded([&] {
+    if (!device_x || !device_q || !device_scales) throw Failure("Input and outputs are required.");
+    const int T = token_count(tokens);
+    if (!cols || cols > (1u << 24)) throw Failure("The column count must be in 1..16777216.");
+    const int dev = device_of(device_x, "input");
+    DeviceGuard g(dev);
+    require_operand(type, device_x, ldx, tokens, cols, dev, "input");
+    require_on(device_q, dev, "quantised output");
+    require_on(device_scales, dev, "scales");
+    require_align(device_q, 16, "quantised output");
+    require_align(device_scales, 16, "scales");
+    cuda_check(lb::launch_f8_quant(is_bf16(type, "input"), device_x, ldx, T, (int)cols,
+                                   static_cast<uint8_t*>(device_q), lb::f8_pad16((long)cols),
+                                   device_scales, lb::f8_pad4(T), nullptr, 0,
+                                   static_cast<cudaStream_t>(cuda_stream)),
+               "quantise launch");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor, int on_device,
+                                    llambda_cuda_fp8_session** result) {
+  if (!result) {
+    set_error("A result pointer is required.");
+    return -1;
+  }
+  *result = nullptr;
+  return guarded([&] {
+    if (!tensor) throw Failure("A tensor is required.");
+    if (tensor->ne2 > 1) throw Failure("A projection has one matrix.");
+    auto s = new llambda_cuda_fp8_session();
+    try {
+      s->open();
+      s->w = s->matrix(*tensor, on_device != 0, "projection tensor");
+    } catch (...) {
+      delete s;
+      throw;
+    }
+    *result = s;
+    return 0;
+  });
+}
+
+void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session* session) { destroy_owner(session); }
+
+size_t llambda_cuda_fp8_session_workspace(const llambda_cuda_fp8_session* s, size_t tokens) {
+  return s && tokens ? f8_quant_bytes(s->w.cols, tokens, nullptr) : 0;
+}
+
+static void f8_project_call(llambda_cuda_fp8_session* s, bool x_bf16, const void* x, int64_t ldx,
+                            int T, bool out_bf16, void* out, int64_t ldo, void* work,
+                            cudaStream_t st) {
+  size_t at = 0;
+  f8_quant_bytes(s->w.cols, T, &at);
+  uint8_t* q = static_cast<uint8_t*>(work);
+  float* sc = reinterpret_cast<float*>(q + at);
+  cuda_check(lb::launch_f8_quant(x_bf16, x, ldx, T, s->w.cols, q, lb::f8_pad16(s->w.cols), sc,
+                                 lb::f8_pad4(T), nullptr, 0, st),
+             "quantise launch");
+  cuda_check(lb::launch_f8_project(s->w, q, sc, T, out_bf16, out, ldo, s->status, st),
+             "product launch");
+}
+
+int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* s, const float* x, size_t tokens,
+                                 float* out) {
+  if (!s || !x || !out) {
+    set_error("Session, input and output are required.");
+    return -1;
+  }
+  return guarded([&] {
+    const int T = token_count(tokens);
+    std::lock_guard<std::mutex> lock(s->mu);
+    DeviceGuard g(s->device);
+    const size_t in = tokens * s->w.cols * 4, ob = tokens * s->w.rows * 4;
+    float* din = static_cast<float*>(s->din.get(in));
+    float* dout = static_cast<float*>(s->dout.get(ob));
+    void* work = s->dwork.get(f8_quant_bytes(s->w.cols, tokens, nullptr));
+    cuda_check(cudaMemcpyAsync(din, x, in, cudaMemcpyHostToDevice, s->stream), "input copy");
+    f8_project_call(s, false, din, s->w.cols, T, false, dout, s->w.rows, work, s->stream);
+    s->finish(out, dout, ob, "e4m3 product");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_session_run_device(llambda_cuda_fp8_session* s, int x_type,
+                                        const void* device_x, int64_t ldx, size_t tokens,
+                                        int out_type, void* device_out, int64_t ldo,
+                                        void* workspace, size_t workspace_bytes,
+                                        void* cuda_stream) {
+  if (!s || !device_x || !device_out || !workspace) {
+    set_error("Session, device input/output and a workspace are required.");
+    return -1;
+  }
+  return guarded([&] {
+    const int T = token_count(tokens);
+    DeviceGuard g(s->device);
+    require_operand(x_type, device_x, ldx, tokens, s->w.cols, s->device, "input");
+    require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
+    require_workspace(workspace, workspace_bytes, f8_quant_bytes(s->w.cols, tokens, nullptr),
+                      s->device);
+    f8_project_call(s, is_bf16(x_type, "input"), device_x, ldx, T, is_bf16(out_type, "output"),
+                    device_out, ldo, workspace, static_cast<cudaStream_t>(cuda_stream));
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_session_run_quantized(llambda_cuda_fp8_session* s, const void* device_q,
+                                           const float* device_scales, size_t tokens, int out_type,
+                                           void* device_out, int64_t ldo, void* cuda_stream) {
+  if (!s || !device_q || !device_scales || !device_out) {
+    set_error("Session, quantised input, scales and output are required.");
+    return -1;
+  }
+  return guarded([&] {
+    const int T = token_count(tokens);
+    DeviceGuard g(s->device);
+    require_on(device_q, s->device, "quantised input");
+    require_on(device_scales, s->device, "scales");
+    require_align(device_q, 16, "quantised input");
+    require_align(device_scales, 16, "scales");
+    require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
+    cuda_check(lb::launch_f8_project(s->w, static_cast<const uint8_t*>(device_q), device_scales, T,
+                                     is_bf16(out_type, "output"), device_out, ldo, s->status,
+                                     static_cast<cudaStream_t>(cuda_stream)),
+               "product launch");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_session_status(llambda_cuda_fp8_session* s) {
+  if (!s) {
+    set_error("A session is required.");
+    return -1;
+  }
+  return guarded([&] {
+    DeviceGuard g(s->device);
+    return s->take_status();
+  });
+}
+
+int llambda_cuda_fp8_moe_session_create(const llambda_cuda_fp8_tensor* gate,
+                                        const llambda_cuda_fp8_tensor* up,
+                                        const llambda_cuda_fp8_tensor* down, int on_device,
+                                        llambda_cuda_fp8_moe_session** result) {
+  if (!result) {
+    set_error("A result pointer is required.");
+    return -1;
+  }
+  *result = nullptr;
+  return guarded([&] {
+    if (!up || !down) throw Failure("The up and down tensors are required.");
+    const bool gated = gate && gate->data;
+    auto n2 = [](const llambda_cuda_fp8_tensor* t) { return t->ne2 ? t->ne2 : 1; };
+    if (gated && (gate->ne0 != up->ne0 || gate->ne1 != up->ne1 || n2(gate) != n2(up)))
+      throw Failure("The gate tensor's dimensions differ from the up tensor's.");
+    if (down->ne0 != up->ne1 || n2(down) != n2(up))
+      throw Failure("The down tensor does not fit the up tensor.");
+    auto s = new llambda_cuda_fp8_moe_session();
+    try {
+      s->open();
+      if (gated) s->m.gate = s->matrix(*gate, on_device != 0, "gate tensor");
+      s->m.up = s->matrix(*up, on_device != 0, "up tensor");
+      s->m.down = s->matrix(*down, on_device != 0, "down tensor");
+    } catch (...) {
+      delete s;
+      throw;
+    }
+    *result = s;
+    return 0;
+  });
+}
+
+void llambda_cuda_fp8_moe_session_destroy(llambda_cuda_fp8_moe_session* session) {
+  destroy_owner(session);
+}
+
+size_t llambda_cuda_fp8_moe_session_workspace(const llambda_cuda_fp8_moe_session* s, size_t tokens,
+                                              int top_k) {
+  if (!s || !tokens || top_k < 1) return 0;
+  return lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes;
+}
+
+int llambda_cuda_fp8_moe_session_run(llambda_cuda_fp8_moe_session* s, const float* x, size_t tokens,
+                                     int top_k, const int32_t* selected, const float* weights,
+                                     float* out) {
+  if (!s || !x || !selected || !weights || !out) {
+    set_error("Session, input, selection, weights and output are required.");
+    return -1;
+  }
+  return guarded([&] {
+    moe_call_sizes(s, tokens, top_k);
+    std::lock_guard<std::mutex> lock(s->mu);
+    DeviceGuard g(s->device);
+    const int H = s->m.up.cols, O = s->m.down.rows;
+    const size_t in = tokens * H * 4, ob = tokens * O * 4, eb = tokens * top_k * 4;
+    float* din = static_cast<float*>(s->din.get(in));
+    float* dout = static_cast<float*>(s->dout.get(ob));
+    int* dsel = static_cast<int*>(s->dsel.get(eb));
+    float* dw = static_cast<float*>(s->dw.get(eb));
+    void* work = s->dwork.get(lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes);
+    cuda_check(cudaMemcpyAsync(din, x, in, cudaMemcpyHostToDevice, s->stream), "input copy");
+    cuda_check(cudaMemcpyAsync(dsel, selected, eb, cudaMemcpyHostToDevice, s->stream), "copy");
+    cuda_check(cudaMemcpyAsync(dw, weights, eb, cudaMemcpyHostToDevice, s->stream), "copy");
+    cuda_check(lb::launch_f8_moe(s->m, false, din, H, (int)tokens, top_k, dsel, dw, false, dout, O,
+                                 work, s->status, s->stream),
+               "experts launch");
+    s->finish(out, dout, ob, "routed experts");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_moe_session_run_device(llambda_cuda_fp8_moe_session* s, int x_type,
+                                            const void* device_x, int64_t ldx, size_t tokens,
+                                            int top_k, const int32_t* device_selected,
+                                            const float* device_weights, int out_type,
+                                            void* device_out, int64_t ldo, void* workspace,
+                                            size_t workspace_bytes, void* cuda_stream) {
+  if (!s || !device_x || !device_selected || !device_weights || !device_out || !workspace) {
+    set_error("Session, device input, selection, weights, output and a workspace are required.");
+    return -1;
+  }
+  return guarded([&] {
+    moe_call_sizes(s, tokens, top_k);
+    DeviceGuard g(s->device);
+    require_operand(x_type, device_x, ldx, tokens, s->m.up.cols, s->device, "input");
+    require_operand(out_type, device_out, ldo, tokens, s->m.down.rows, s->device, "output");
+    require_on(device_selected, s->device, "selected");
+    require_on(device_weights, s->device, "weights");
+    require_align(device_selected, 4, "selected");
+    require_align(device_weights, 4, "weights");
+    require_workspace(workspace, workspace_bytes,
+                      lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes, s->device);
+    cuda_check(lb::launch_f8_moe(s->m, is_bf16(x_type, "input"), device_x, ldx, (int)tokens, top_k,
+                                 device_selected, device_weights, is_bf16(out_type, "output"),
+                                 device_out, ldo, workspace, s->status,
+                                 static_cast<cudaStream_t>(cuda_stream)),
+               "experts launch");
+    return 0;
+  });
+}
+
+int llambda_cuda_fp8_moe_session_status(llambda_cuda_fp8_moe_session* s) {
+  if (!s) {
+    set_error("A session is required.");
+    return -1;
+  }
+  return guarded([&] {
+    DeviceGuard g(s->device);
+    return s->take_status();
+  });
+}
+
 }  // extern "C"
 
 // The GGUF loader (gguf.cu) reports through the same thread-local last error.

@@ -1,0 +1,807 @@
+// 8-bit floating point (e4m3) products with one fp32 scale per block of 128,
+// on the tcgen05 tensor cores: the dense projection and the routed experts'
+// feed-forward, with the quantiser of their activations.
+//
+// Mathematics.  A row of activations x is cut into blocks of 128 columns; per
+// block b, s[b] = max|x| / 448 and q = e4m3(x / s[b]).  A weight matrix W has
+// one scale per 128 x 128 block.  A product is
+//   y[t][n] = sum_b (s[t][b] * sw[n / 128][b]) * (sum_{k in b} q[t][k] * W[n][k]):
+// the inner sums are the tensor cores' (exact products, fp32 sums in tensor
+// memory), the outer one fp32 FMAs in registers.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <mutex>
+
+#include "engine.cuh"
+#include "kernels.h"
+#include "tcgen05.cuh"
+
+namespace lb {
+
+namespace {
+
+constexpr int kF8M = 128;         // weight rows per tile (the MMA's M)
+constexpr int kF8Block = 128;     // columns per scale, bytes per staged row
+constexpr int kF8EpiWarps = 8;    // two warpgroups, half of the tokens each
+constexpr int kF8Threads = (4 + kF8EpiWarps) * 32;
+constexpr int kF8Scales = 8;      // ring of staged activation scales
+constexpr int kF8MaxBuf = 4;      // ring of accumulators in tensor memory
+
+enum F8Mode {
+  kF8Out,      // y to out (fp32 or bf16)
+  kF8Act,      // activation of gate and up, quantised: the down product's input
+  kF8Partial,  // y to the row of its (token, rank) entry
+};
+
+// e4m3 of v as a byte: round to nearest even, NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3_byte(float v) {
+  return (uint32_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
+// The scale of a block whose largest magnitude has the bits `amax` (a NaN's
+// bits are above infinity's, so a maximum over bits keeps a NaN).  A block of
+// zeros, or of values too small to scale, takes the smallest normal number.
+__device__ __forceinline__ float block_scale(uint32_t amax) {
+  const float s = __fdiv_rn(__uint_as_float(amax), 448.0f);
+  return s < FLT_MIN ? FLT_MIN : s;
+}
+
+// ------------------------------------------------------------ quantiser
+
+__device__ __forceinline__ void load4(const float* p, bool vec, int n, float* v) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.0f;
+  }
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, int n, float* v) {
+  if (vec) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+    v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
+  }
+}
+
+// One warp per (token, block of 128 columns), four columns a lane.  q has rows
+// of q_pitch bytes (a multiple of 16, zeros past cols), scales the layout
+// [block][s_pitch] the products read with bulk copies.  With `rows` the
+// token's row goes to its k grouped rows (those that are not negative);
+// without, to row t, and the scales of rows [tokens, s_pitch) are zeroed.
+template <typename T>
+__global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, long ldx,
+                                                       int tokens, int cols, uint8_t* q,
+                                                       long q_pitch, float* scales, long s_pitch,
+                                                       const int* rows, int k, int vec) {
+  griddep_wait();
+  griddep_launch();
+  const int lane = threadIdx.x & 31;
+  const int blocks = (cols + kF8Block - 1) / kF8Block;
+  const long n = (rows ? (long)tokens : s_pitch) * blocks;
+  for (long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (long)gridDim.x * 8) {
+    const long t = i / blocks;
+    const int b = (int)(i - t * blocks);
+    if (t >= tokens) {
+      if (lane == 0) scales[b * s_pitch + t] = 0.0f;
+      continue;
+    }
+    const int c = b * kF8Block + 4 * lane;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < cols) load4(x + t * ldx + c, vec && c + 4 <= cols, cols - c, v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    const float s = block_scale(__reduce_max_sync(0xffffffffu, m));
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= e4m3_byte(__fdiv_rn(v[j], s)) << (8 * j);
+    if (!rows) {
+      if (c < q_pitch) *reinterpret_cast<uint32_t*>(q + t * q_pitch + c) = w;
+      if (lane == 0) scales[b * s_pitch + t] = s;
+    } else {
+      for (int j = 0; j < k; ++j) {
+        const int r = __ldcg(rows + t * k + j);
+        if (r < 0) continue;
+        if (c < q_pitch) *reinterpret_cast<uint32_t*>(q + r * q_pitch + c) = w;
+        if (lane == 0) scales[b * s_pitch + r] = s;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ products
+
+struct F8Maps {
+  CUtensorMap x, w0, w1;
+};
+
+struct F8Pass {
+  int rows, rblocks, kblocks;    // weight rows of one expert, their blocks, blocks of K
+  const float *ws0, *ws1;        // weight scales [expert][rblocks][kblocks]
+  const float* xs;               // activation scales [kblocks][xs_pitch]
+  long xs_pitch;
+  int tokens, chunks;            // dense: rows of x and their tiles of NT
+  const int4* tiles;             // grouped: {first row, rows, expert, 0} of each chunk,
+  const int* nchunks;            //   null when dense
+  void* out;                     // kF8Out
+  long ldo;
+  int out_bf16;
+  uint8_t* hq;                   // kF8Act: quantised activations and their scales
+  long h_pitch;
+  float* hs;
+  long hs_pitch;
+  float* partial;                // kF8Partial: rows of partial by entry
+  long ldp;
+  const int* entry;
+  int* status;
+};
+
+struct F8Sync {
+  uint64_t full[16], empty[16];
+  uint64_t sfull[kF8Scales], sempty[kF8Scales];
+  uint64_t tfull[kF8MaxBuf], tempty[kF8MaxBuf], done;
+  uint32_t tmem;
+  int abort;
+};
+
+template <int NT, int MATS>
+struct F8Cfg {
+  static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
+  static constexpr uint32_t kStage = MATS * kA + NT * kF8Block;
+  static constexpr int kStages = (int)(200u * 1024u / kStage) > 12 ? 12 : (int)(200u * 1024u / kStage);
+  static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
+  static constexpr int kBufs = 512 / kAcc > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc;
+  static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kF8Scales * NT * 4 +
+                                  2 * 4 * NT * 4 + sizeof(F8Sync);
+};
+
+// Instruction descriptor, kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), A and
+// B e4m3 (bits 7-9 and 10-12 = 0), both K-major, N >> 3 in bits 17-22, M >> 4
+// in bits 24-28.
+__device__ __forceinline__ uint32_t f8_idesc(int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kF8M >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] . B[smem]^T over 32 columns of K.
+__device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// 8 consecutive fp32 columns of this thread's tensor-memory lane (no wait).
+__device__ __forceinline__ void tmem_ld8_issue(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+// Waits for this thread's tensor-memory loads; the registers pass through so
+// that no use of them moves above the wait.
+__device__ __forceinline__ void tmem_wait_ld8(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
+struct F8Tile {
+  int row0, count, expert, rb;  // first row of x, valid rows, expert, row block
+};
+
+// Tiles in the order the CTAs take them.  Dense: the token chunks of one row
+// block next to each other, so its weights come from L2 after the first.
+// Grouped: the row blocks of one chunk next to each other.
+template <int NT>
+__device__ __forceinline__ F8Tile f8_tile(const F8Pass& p, int tile) {
+  F8Tile t;
+  if (p.tiles) {
+    const int c = tile / p.rblocks;
+    const int4 v = __ldcg(p.tiles + c);
+    t.row0 = v.x, t.count = v.y, t.expert = v.z, t.rb = tile - c * p.rblocks;
+  } else {
+    t.rb = tile / p.chunks;
+    t.row0 = (tile - t.rb * p.chunks) * NT;
+    t.count = min(NT, p.tokens - t.row0);
+    t.expert = 0;
+  }
+  return t;
+}
+
+__device__ __forceinline__ float silu(float g) { return __fdiv_rn(g, 1.0f + expf(-g)); }
+
+// One CTA per SM, persistent over tiles of 128 weight rows x NT rows of x (M is
+// the weights' side, so one token costs a tile of 16 columns, and an expert's
+// few tokens no more).  Warp 0 stages weights and activations by TMA, warp 2
+// the activations' scales, warp 1's first lane issues the MMAs of one block of
+// K into the next of kBufs accumulators, and eight warps add the accumulators,
+// scaled, into registers: lane r of the tensor memory is weight row r, so the
+// weight scale is one number per block and thread.
+template <int NT, int MATS, int MODE>
+__global__ void __launch_bounds__(kF8Threads, 1)
+    f8_gemm_kernel(const __grid_constant__ F8Maps maps, const F8Pass p) {
+  using C = F8Cfg<NT, MATS>;
+  constexpr int NC = NT / 2;  // tokens per epilogue thread
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  float* s_scale = reinterpret_cast<float*>(stages + (size_t)C::kStages * C::kStage);
+  uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + kF8Scales * NT);  // [parity][quadrant][NT]
+  F8Sync* sy = reinterpret_cast<F8Sync*>(s_amax + 2 * 4 * NT);
+  volatile int* abort = &sy->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&sy->full[s], 1);
+      mbar_init(&sy->empty[s], 1);
+    }
+    for (int s = 0; s < kF8Scales; ++s) {
+      mbar_init(&sy->sfull[s], 1);
+      mbar_init(&sy->sempty[s], kF8EpiWarps);
+    }
+    for (int b = 0; b < C::kBufs; ++b) {
+      mbar_init(&sy->tfull[b], 1);
+      mbar_init(&sy->tempty[b], kF8EpiWarps);
+    }
+    mbar_init(&sy->done, 1);
+    sy->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&sy->tmem, C::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sy->tmem;
+  griddep_wait();
+  griddep_launch();
+  const int ntiles = (p.tiles ? __ldcg(p.nchunks) : p.chunks) * p.rblocks;
+
+  if (warp == 0) {  // ------------------------------------- weights, activations
+    if (lane == 0) {
+      RingPos rp;
+      int q = 0;
+      uint32_t last_phase[C::kStages] = {};
+      for (int tile = blockIdx.x; tile < ntiles && !*abort; tile += gridDim.x) {
+        const F8Tile t = f8_tile<NT>(p, tile);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (q >= C::kStages &&
+              !mbar_wait_or_abort(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort))
+            break;
+          uint8_t* st = stages + (size_t)rp.s * C::kStage;
+          uint64_t* bar = &sy->full[rp.s];
+          mbar_expect_tx(bar, C::kStage);
+          tma_load_3d(st, &maps.w0, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+          if (MATS == 2)
+            tma_load_3d(st + C::kA, &maps.w1, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+          tma_load_2d(st + MATS * C::kA, &maps.x, kb * kF8Block, t.row0, bar);
+          last_phase[rp.s] = rp.phase;
+          ++q;
+          rp.next(C::kStages);
+        }
+      }
+      // copies still in flight land before the CTA exits (bounded)
+      for (int s = 0; s < C::kStages && s < q; ++s) mbar_wait(&sy->full[s], last_phase[s], nullptr);
+    }
+    __syncwarp();
+  } else if (warp == 2) {  // -------------------------------------------- scales
+    if (lane == 0) {
+      RingPos rp;
+      int q = 0;
+      uint32_t last_phase[kF8Scales] = {};
+      for (int tile = blockIdx.x; tile < ntiles && !*abort; tile += gridDim.x) {
+        const F8Tile t = f8_tile<NT>(p, tile);
+        // row0 and the pitch are multiples of 4; columns past the pitch keep
+        // what an earlier tile left and belong to no valid row
+        const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (q >= kF8Scales &&
+              !mbar_wait_or_abort(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort))
+            break;
+          mbar_expect_tx(&sy->sfull[rp.s], bytes);
+          tma_load_1d(s_scale + rp.s * NT, p.xs + kb * p.xs_pitch + t.row0, bytes,
+                      &sy->sfull[rp.s]);
+          last_phase[rp.s] = rp.phase;
+          ++q;
+          rp.next(kF8Scales);
+        }
+      }
+      for (int s = 0; s < kF8Scales && s < q; ++s) mbar_wait(&sy->sfull[s], last_phase[s], nullptr);
+    }
+    __syncwarp();
+  } else if (warp == 1) {  // ----------------------------------------------- MMA
+    if (lane == 0) {
+      RingPos rp, ap;
+      int q = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+        const F8Tile t = f8_tile<NT>(p, tile);
+        const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = (q < C::kBufs ||
+                mbar_spin_or_abort(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
+               mbar_spin_or_abort(&sy->full[rp.s], rp.phase, p.status, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint8_t* st = stages + (size_t)rp.s * C::kStage;
+          const uint64_t bd = sw128_desc(st + MATS * C::kA);
+#pragma unroll
+          for (int mat = 0; mat < MATS; ++mat) {
+            const uint64_t ad = sw128_desc(st + mat * C::kA);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // K steps of 32 bytes
+              tc_mma_f8(tmem + ap.s * C::kAcc + mat * NT, ad + 2 * j, bd + 2 * j, idesc, j != 0);
+          }
+          tc_commit(&sy->empty[rp.s]);
+          tc_commit(&sy->tfull[ap.s]);
+          ++q;
+          rp.next(C::kStages);
+          ap.next(C::kBufs);
+        }
+      }
+      // every MMA issued has completed before the tensor memory is freed
+      tc_commit(&sy->done);
+      mbar_wait(&sy->done, 0, nullptr);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {  // ------------------------------------------ epilogue
+    const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane;
+    const uint32_t lane_base = (uint32_t)(32 * quad) << 16;
+    RingPos ap, sp;
+    bool ok = true;
+    int parity = 0;
+    for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, parity ^= 1) {
+      const F8Tile t = f8_tile<NT>(p, tile);
+      const int mine = min(NC, t.count - half * NC);  // valid tokens of this thread, may be <= 0
+      const long ws_row = ((long)t.expert * p.rblocks + t.rb) * p.kblocks;
+      float2 acc[MATS][NC / 2];
+#pragma unroll
+      for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) acc[m][c] = make_float2(0.0f, 0.0f);
+      float wl[MATS];  // weight scales of 32 blocks, one a lane
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if ((kb & 31) == 0) {
+          const bool in = kb + lane < p.kblocks;
+          wl[0] = in ? __ldg(p.ws0 + ws_row + kb + lane) : 0.0f;
+          if (MATS == 2) wl[MATS - 1] = in ? __ldg(p.ws1 + ws_row + kb + lane) : 0.0f;
+        }
+        float sw[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) sw[m] = __shfl_sync(0xffffffffu, wl[m], kb & 31);
+        ok = mbar_wait_or_abort(&sy->sfull[sp.s], sp.phase, p.status, abort) &&
+             mbar_wait_or_abort(&sy->tfull[ap.s], ap.phase, p.status, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float* sc = s_scale + sp.s * NT + half * NC;
+        constexpr int CH = NC < 16 ? NC : 16;  // columns loaded together
+#pragma unroll
+        for (int c0 = 0; c0 < NC; c0 += CH) {
+          if (c0 < mine) {  // warp-uniform
+            uint32_t d[MATS][CH];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+              for (int j = 0; j < CH; j += 8)
+                tmem_ld8_issue(tmem + lane_base + ap.s * C::kAcc + m * NT + half * NC + c0 + j,
+                               d[m] + j);
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+              for (int j = 0; j < CH; j += 8) tmem_wait_ld8(d[m] + j);
+#pragma unroll
+            for (int j = 0; j < CH; j += 4) {
+              const float4 sx = *reinterpret_cast<const float4*>(sc + c0 + j);
+#pragma unroll
+              for (int m = 0; m < MATS; ++m) {
+                ffma2(acc[m][(c0 + j) / 2], __uint_as_float(d[m][j]),
+                      __uint_as_float(d[m][j + 1]), sx.x * sw[m], sx.y * sw[m]);
+                ffma2(acc[m][(c0 + j) / 2 + 1], __uint_as_float(d[m][j + 2]),
+                      __uint_as_float(d[m][j + 3]), sx.z * sw[m], sx.w * sw[m]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sy->tempty[ap.s]);
+          mbar_arrive(&sy->sempty[sp.s]);
+        }
+        ap.next(C::kBufs);
+        sp.next(kF8Scales);
+      }
+      if (!ok) break;
+      const int row = t.rb * kF8M + r;
+      const int tok0 = t.row0 + half * NC;
+      if (MODE == kF8Out) {
+        if (row < p.rows) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (c < mine) {
+              const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
+              const long o = (long)(tok0 + c) * p.ldo + row;
+              if (p.out_bf16)
+                static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(y);
+              else
+                static_cast<float*>(p.out)[o] = y;
+            }
+        }
+      } else if (MODE == kF8Partial) {
+        if (row < p.rows) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (c < mine) {
+              const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
+              p.partial[(long)__ldcg(p.entry + tok0 + c) * p.ldp + row] = y;
+            }
+        }
+      } else {
+        // the 128 rows of this tile are one block of the next product's K:
+        // its scale per token is a maximum over the four warps of this half
+        uint32_t* am = s_amax + parity * 4 * NT + half * NC;
+        float h[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float u = c & 1 ? acc[MATS - 1][c / 2].y : acc[MATS - 1][c / 2].x;
+          const float g = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
+          if (MATS == 2) {
+            h[c] = silu(g) * u;
+          } else {
+            const float v = u < 0.0f ? 0.0f : u;  // a NaN stays
+            h[c] = v * v;
+          }
+          if (row >= p.rows) h[c] = 0.0f;
+          if (c < mine) {
+            const uint32_t a =
+                __reduce_max_sync(0xffffffffu, __float_as_uint(h[c]) & 0x7fffffffu);
+            if (lane == 0) am[quad * NT + c] = a;
+          }
+        }
+        named_bar_sync(1 + half, 128);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          if (c < mine) {
+            const float s = block_scale(
+                max(max(am[c], am[NT + c]), max(am[2 * NT + c], am[3 * NT + c])));
+            p.hq[(long)(tok0 + c) * p.h_pitch + row] = (uint8_t)e4m3_byte(__fdiv_rn(h[c], s));
+            if (r == 0) p.hs[t.rb * p.hs_pitch + tok0 + c] = s;
+          }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// ------------------------------------------------------------ experts
+
+// One CTA: groups the entries (token t, rank j; id t * k + j) by expert.
+// Every expert's rows start at a multiple of 4 (the scales' bulk copies start
+// on 16 bytes); chunks of at most nt rows go to tiles in expert order.
+// Entries whose expert is outside [0, E) get row -1.  The order within an
+// expert follows arrival and changes no value: every row is computed alone.
+__global__ void __launch_bounds__(1024) f8_plan_kernel(const int* __restrict__ sel, int n, int E,
+                                                       int nt, int* row_of, int* entry,
+                                                       int4* tiles, int* nchunks) {
+  __shared__ int s_count[1024], s_row[1024], s_warp[2][32];
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  s_count[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) {
+    const int e = sel[i];
+    row_of[i] = e >= 0 && e < E ? atomicAdd(&s_count[e], 1) : -1;
+  }
+  __syncthreads();
+  const int cnt = s_count[tid], pad = (cnt + 3) & ~3, ch = (cnt + nt - 1) / nt;
+  int a = pad, b = ch;  // inclusive scans over the experts
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int va = __shfl_up_sync(0xffffffffu, a, o), vb = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += va, b += vb;
+  }
+  if (lane == 31) s_warp[0][warp] = a, s_warp[1][warp] = b;
+  __syncthreads();
+  if (warp == 0) {
+    int va = s_warp[0][lane], vb = s_warp[1][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int wa = __shfl_up_sync(0xffffffffu, va, o), wb = __shfl_up_sync(0xffffffffu, vb, o);
+      if (lane >= o) va += wa, vb += wb;
+    }
+    s_warp[0][lane] = va, s_warp[1][lane] = vb;
+  }
+  __syncthreads();
+  const int row = a - pad + (warp ? s_warp[0][warp - 1] : 0);
+  const int chunk = b - ch + (warp ? s_warp[1][warp - 1] : 0);
+  s_row[tid] = row;
+  for (int c = 0; c < ch; ++c)
+    tiles[chunk + c] = make_int4(row + c * nt, min(nt, cnt - c * nt), tid, 0);
+  if (tid == 1023) *nchunks = s_warp[1][31];
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) {
+    const int pos = row_of[i];
+    if (pos < 0) continue;
+    const int r = s_row[sel[i]] + pos;
+    row_of[i] = r;
+    entry[r] = i;
+  }
+}
+
+// out[t] = sum over ranks j, in order, of weight * partial row; entries with
+// row -1 add nothing.  Four columns a thread.
+__global__ void __launch_bounds__(256) f8_combine_kernel(const float* partial, long ldp,
+                                                         const int* row_of, const float* weights,
+                                                         int k, int cols, void* out, long ldo,
+                                                         int out_bf16) {
+  griddep_wait();
+  griddep_launch();
+  const long t = blockIdx.x;
+  for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < k; ++j) {
+      if (__ldcg(row_of + t * k + j) < 0) continue;
+      const float w = weights[t * k + j];
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(partial + (t * k + j) * ldp + c));
+      a[0] = fmaf(w, v.x, a[0]), a[1] = fmaf(w, v.y, a[1]);
+      a[2] = fmaf(w, v.z, a[2]), a[3] = fmaf(w, v.w, a[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < cols) {
+        if (out_bf16)
+          static_cast<__nv_bfloat16*>(out)[t * ldo + c + i] = __float2bfloat16_rn(a[i]);
+        else
+          static_cast<float*>(out)[t * ldo + c + i] = a[i];
+      }
+  }
+}
+
+__global__ void f8_check_scales_kernel(const float* s, size_t n, unsigned* bad) {
+  unsigned c = 0;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n;
+       i += (size_t)gridDim.x * blockDim.x)
+    c += !isfinite(s[i]);
+  if (c) atomicAdd(bad, c);
+}
+
+// ------------------------------------------------------------ host side
+
+PFN_cuTensorMapEncodeTiled_v12000 f8_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  return encode;
+}
+
+bool f8_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+               const cuuint64_t* strides, int box_rows) {
+  const auto encode = f8_encoder();
+  if (!encode) return false;
+  const cuuint32_t box[3] = {(cuuint32_t)kF8Block, (cuuint32_t)box_rows, 1}, elem[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides,
+                box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Weights as [experts][rows][cols] bytes, a tile's box 128 x 128; what lies
+// past the rows or columns of an expert reads as zeros.
+bool f8_weight_map(CUtensorMap* map, const F8Matrix& w) {
+  const cuuint64_t dims[3] = {(cuuint64_t)w.cols, (cuuint64_t)w.rows, (cuuint64_t)w.experts};
+  const cuuint64_t strides[2] = {(cuuint64_t)w.pitch, (cuuint64_t)w.pitch * w.rows};
+  return f8_encode(map, w.data, 3, dims, strides, kF8M);
+}
+
+bool f8_rows_map(CUtensorMap* map, const void* q, long pitch, long rows, int cols, int nt) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  return f8_encode(map, q, 2, dims, strides, nt);
+}
+
+template <int NT, int MATS, int MODE>
+cudaError_t launch_f8_gemm(const F8Maps& maps, const F8Pass& p, long tiles, cudaStream_t s) {
+  auto kern = f8_gemm_kernel<NT, MATS, MODE>;
+  constexpr size_t smem = F8Cfg<NT, MATS>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = (unsigned)std::min<long>(tiles, sm_count());
+  return launch_pdl(kern, dim3(grid), dim3(kF8Threads), smem, s, maps, p);
+}
+
+template <int MATS, int MODE>
+cudaError_t launch_f8_pass(int nt, const F8Maps& maps, const F8Pass& p, long tiles,
+                           cudaStream_t s) {
+  switch (nt) {
+    case 16: return launch_f8_gemm<16, MATS, MODE>(maps, p, tiles, s);
+    case 32: return launch_f8_gemm<32, MATS, MODE>(maps, p, tiles, s);
+    case 64: return launch_f8_gemm<64, MATS, MODE>(maps, p, tiles, s);
+    default: return launch_f8_gemm<128, MATS, MODE>(maps, p, tiles, s);
+  }
+}
+
+int f8_chunk(long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+int f8_blocks(long n) { return (int)((n + kF8Block - 1) / kF8Block); }
+
+template <typename T>
+cudaError_t quant_t(const T* x, long ldx, int tokens, int cols, uint8_t* q, long q_pitch,
+                    float* scales, long s_pitch, const int* rows, int k, cudaStream_t st) {
+  const int vec = ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
+  const long warps = (rows ? (long)tokens : s_pitch) * f8_blocks(cols);
+  const unsigned grid = (unsigned)std::min<long>((warps + 7) / 8, (long)sm_count() * 16);
+  return launch_pdl(f8_quant_kernel<T>, dim3(grid), dim3(256), 0, st, x, ldx, tokens, cols, q,
+                    q_pitch, scales, s_pitch, rows, k, vec);
+}
+
+}  // namespace
+
+cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
+                            long q_pitch, float* scales, long s_pitch, const int* rows, int k,
+                            cudaStream_t st) {
+  return bf16 ? quant_t(static_cast<const __nv_bfloat16*>(x), ldx, tokens, cols, q, q_pitch,
+                        scales, s_pitch, rows, k, st)
+              : quant_t(static_cast<const float*>(x), ldx, tokens, cols, q, q_pitch, scales,
+                        s_pitch, rows, k, st);
+}
+
+cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaStream_t st) {
+  f8_check_scales_kernel<<<(unsigned)std::min<size_t>((n + 255) / 256, 1024), 256, 0, st>>>(
+      scales, n, bad);
+  return cudaGetLastError();
+}
+
+cudaError_t f8_prepare(F8Matrix* w) {
+  return f8_weight_map(&w->map, *w) ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
+                              bool out_bf16, void* out, long ldo, int* status, cudaStream_t st) {
+  F8Maps maps;
+  const int nt = f8_chunk(tokens);
+  maps.w0 = maps.w1 = w.map;
+  if (!f8_rows_map(&maps.x, q, f8_pad16(w.cols), tokens, w.cols, nt)) return cudaErrorInvalidValue;
+  F8Pass p{};
+  p.rows = w.rows;
+  p.rblocks = f8_blocks(w.rows);
+  p.kblocks = f8_blocks(w.cols);
+  p.ws0 = w.scales;
+  p.xs = scales;
+  p.xs_pitch = f8_pad4(tokens);
+  p.tokens = tokens;
+  p.chunks = (tokens + nt - 1) / nt;
+  p.out = out;
+  p.ldo = ldo;
+  p.out_bf16 = out_bf16;
+  p.status = status;
+  return launch_f8_pass<1, kF8Out>(nt, maps, p, (long)p.chunks * p.rblocks, st);
+}
+
+F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k) {
+  F8MoeLayout L;
+  const long n = tokens * k, groups = std::min<long>(n, m.up.experts);
+  L.rows = f8_pad4(n + 3 * groups);
+  L.max_chunks = n / 16 + groups;
+  auto take = [off = size_t(0)](size_t bytes) mutable {
+    const size_t at = off;
+    off += (bytes + 255) & ~size_t(255);
+    return at;
+  };
+  L.hp = (long)f8_blocks(m.up.rows) * kF8Block;
+  L.row_of = take((size_t)n * 4);
+  L.entry = take((size_t)L.rows * 4);
+  L.tiles = take((size_t)L.max_chunks * 16);
+  L.nchunks = take(4);
+  L.xq = take((size_t)L.rows * f8_pad16(m.up.cols));
+  L.xs = take((size_t)f8_blocks(m.up.cols) * L.rows * 4);
+  L.hq = take((size_t)L.rows * L.hp);
+  L.hs = take((size_t)f8_blocks(m.up.rows) * L.rows * 4);
+  L.ldp = f8_pad4(m.down.rows);
+  L.partial = take((size_t)n * L.ldp * 4);
+  L.bytes = take(0);
+  return L;
+}
+
+cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, int tokens, int k,
+                          const int* sel, const float* weights, bool out_bf16, void* out, long ldo,
+                          void* work, int* status, cudaStream_t st) {
+  const F8MoeLayout L = f8_moe_layout(m, tokens, k);
+  uint8_t* base = static_cast<uint8_t*>(work);
+  int* row_of = reinterpret_cast<int*>(base + L.row_of);
+  int* entry = reinterpret_cast<int*>(base + L.entry);
+  int4* tiles = reinterpret_cast<int4*>(base + L.tiles);
+  int* nchunks = reinterpret_cast<int*>(base + L.nchunks);
+  float* partial = reinterpret_cast<float*>(base + L.partial);
+  const long n = (long)tokens * k;
+  // chunks of an expert's tokens: half again the average, so most experts take one
+  const int nt = f8_chunk((3 * n / std::min<long>(n, m.up.experts) + 1) / 2);
+  const long chunks = n / nt + std::min<long>(n, m.up.experts);
+  cudaError_t e = launch_pdl(f8_plan_kernel, dim3(1), dim3(1024), 0, st, sel, (int)n, m.up.experts,
+                             nt, row_of, entry, tiles, nchunks);
+  if (e != cudaSuccess) return e;
+  e = launch_f8_quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
+                      reinterpret_cast<float*>(base + L.xs), L.rows, row_of, k, st);
+  if (e != cudaSuccess) return e;
+  F8Maps maps;
+  F8Pass p{};
+  maps.w0 = m.gate.data ? m.gate.map : m.up.map;
+  maps.w1 = m.up.map;
+  if (!f8_rows_map(&maps.x, base + L.xq, f8_pad16(m.up.cols), L.rows, m.up.cols, nt))
+    return cudaErrorInvalidValue;
+  p.rows = m.up.rows;
+  p.rblocks = f8_blocks(m.up.rows);
+  p.kblocks = f8_blocks(m.up.cols);
+  p.ws0 = m.gate.data ? m.gate.scales : m.up.scales;
+  p.ws1 = m.up.scales;
+  p.xs = reinterpret_cast<const float*>(base + L.xs);
+  p.xs_pitch = L.rows;
+  p.tiles = tiles;
+  p.nchunks = nchunks;
+  p.hq = base + L.hq;
+  p.h_pitch = L.hp;
+  p.hs = reinterpret_cast<float*>(base + L.hs);
+  p.hs_pitch = L.rows;
+  p.status = status;
+  e = m.gate.data ? launch_f8_pass<2, kF8Act>(nt, maps, p, chunks * p.rblocks, st)
+                  : launch_f8_pass<1, kF8Act>(nt, maps, p, chunks * p.rblocks, st);
+  if (e != cudaSuccess) return e;
+  F8Pass d{};
+  maps.w0 = maps.w1 = m.down.map;
+  if (!f8_rows_map(&maps.x, base + L.hq, L.hp, L.rows, m.down.cols, nt))
+    return cudaErrorInvalidValue;
+  d.rows = m.down.rows;
+  d.rblocks = f8_blocks(m.down.rows);
+  d.kblocks = f8_blocks(m.down.cols);
+  d.ws0 = m.down.scales;
+  d.xs = p.hs;
+  d.xs_pitch = L.rows;
+  d.tiles = tiles;
+  d.nchunks = nchunks;
+  d.partial = partial;
+  d.ldp = L.ldp;
+  d.entry = entry;
+  d.status = status;
+  e = launch_f8_pass<1, kF8Partial>(nt, maps, d, chunks * d.rblocks, st);
+  if (e != cudaSuccess) return e;
+  const unsigned gy = (unsigned)std::max(1, std::min((m.down.rows + 1023) / 1024, 64));
+  return launch_pdl(f8_combine_kernel, dim3((unsigned)tokens, gy), dim3(256), 0, st, partial,
+                    L.ldp, row_of, weights, k, m.down.rows, out, ldo, (int)out_bf16);
+}
+
+}  // namespace lb

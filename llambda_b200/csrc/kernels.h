@@ -294,4 +294,62 @@ cudaError_t launch_prefill_passes(const MoeDevice& m, const MoeWork& w, const fl
 cudaError_t launch_moe_dispatch(const MoeDevice& m, const MoeWork& w, const float* x, int T,
                                 float* out, cudaStream_t stream, const cudaEvent_t* marks);
 
+// ------------------------------------------------------------ 8-bit floating point
+
+// E4M3 matrices with one fp32 scale per 128 x 128 block (the last block of an
+// axis may be partial): data [experts][rows][pitch] bytes (pitch a multiple of
+// 16, at least cols), scales [experts][ceil(rows / 128)][ceil(cols / 128)].
+struct F8Matrix {
+  const uint8_t* data;
+  const float* scales;
+  int rows, cols, experts;
+  long pitch;
+  CUtensorMap map;  // filled by f8_prepare
+};
+
+// Routed experts: y = down . act, act = silu(gate . x) * (up . x), or
+// relu(up . x)^2 without gate (gate.data null).
+struct F8Moe {
+  F8Matrix gate, up, down;
+};
+
+// Workspace of one call of the routed experts.
+struct F8MoeLayout {
+  long rows, max_chunks, hp, ldp;
+  size_t row_of, entry, tiles, nchunks, xq, xs, hq, hs, partial, bytes;
+};
+
+inline long f8_pad16(long n) { return (n + 15) & ~15L; }
+inline long f8_pad4(long n) { return (n + 3) & ~3L; }
+
+cudaError_t f8_prepare(F8Matrix* w);
+// Counts the scales that are not finite into *bad (device memory).
+cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaStream_t st);
+// Rows of x (fp32 or bf16, row stride ldx) to e4m3 with one scale per 128
+// columns: q rows of q_pitch bytes, scales [ceil(cols / 128)][s_pitch].  With
+// `rows`, token t goes to the grouped rows rows[t * k + j] that are not
+// negative; without, to row t.
+cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
+                            long q_pitch, float* scales, long s_pitch, const int* rows, int k,
+                            cudaStream_t st);
+// out[t][n] = w . x for quantised rows (pitch f8_pad16(cols), scales' pitch
+// f8_pad4(tokens)).
+cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
+                              bool out_bf16, void* out, long ldo, int* status, cudaStream_t st);
+F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k);
+cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, int tokens, int k,
+                          const int* sel, const float* weights, bool out_bf16, void* out, long ldo,
+                          void* work, int* status, cudaStream_t st);
+
+// ------------------------------------------------------------ routing
+
+// Choice of experts (route.cu): see llambda_cuda_route_desc.
+struct RouteParams {
+  int experts, top_k, softmax, groups, top_groups, group_top, renormalise;
+  float scale;
+};
+cudaError_t launch_route(const RouteParams& r, bool bf16, const void* logits, long ld,
+                         const float* bias, int tokens, int* selected, float* weights,
+                         cudaStream_t st);
+
 }  // namespace lb

@@ -1,0 +1,403 @@
+"""Choice of experts and 8-bit floating point products on CUDA torch tensors.
+
+The device entry points of include/llambda_cuda.h for routers and weights other
+than llambda's own two architectures and GGML blocks: `route_experts` turns
+router logits into experts and weights, `fp8_quantize` turns activations into
+e4m3 with a scale per row and 128 columns, `Fp8ProjectionSession` and
+`Fp8MoeSession` multiply them by e4m3 weights with a scale per 128 x 128 block.
+As everywhere in this package there is no CPU fallback: a refused argument is a
+ValueError, a failed call a LlambdaCudaError.
+
+Device calls run on `stream` (default: the current stream of the tensors'
+device); memory they return or need for working is allocated on that stream, so
+they may be captured into a CUDA graph and overlap on different streams.  Torch
+is only plumbing here (allocation and streams).  The inputs are read, never
+differentiated: a tensor that requires grad is refused while autograd records.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+
+import numpy as np
+
+from . import _native as N
+
+BLOCK = 128  # columns (and weight rows) per scale
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _pad(n: int, m: int) -> int:
+    return -(-n // m) * m
+
+
+def _device_tensor(t, name: str, dtypes, ndim: int, shape=None, device=None, contiguous=False):
+    """Checks a CUDA tensor: type, rank, shape (None: any), unit stride along the last axis."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, "
+                         f"got {str(t.dtype)[6:]}")
+    if t.dim() != ndim or (shape is not None and
+                           any(w is not None and w != g for w, g in zip(shape, t.shape))):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"{tuple('any' if s is None else s for s in shape or (None,) * ndim)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad; these operators have no backward pass")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if contiguous:
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    elif t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride along its last axis")
+    if 0 in t.shape:
+        raise ValueError(f"{name} is empty (a positive token count is required)")
+    return t
+
+
+def _tag(dtype) -> int:
+    return N.TYPE_BF16 if dtype == _torch().bfloat16 else N.TYPE_F32
+
+
+def _floats():
+    torch = _torch()
+    return torch.float32, torch.bfloat16
+
+
+def _on(stream, device):
+    """(context that makes `stream` current, its raw handle); None: the current stream."""
+    torch = _torch()
+    if stream is None:
+        return contextlib.nullcontext(), torch.cuda.current_stream(device).cuda_stream
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    return torch.cuda.stream(stream), stream.cuda_stream
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _out(out, rows: int, cols: int, dtype, device, name="out"):
+    torch = _torch()
+    if out is None:
+        return torch.empty(rows, cols, dtype=dtype, device=device)
+    return _device_tensor(out, name, _floats(), 2, (rows, cols), device)
+
+
+# ------------------------------------------------------------------ routing
+
+
+def _route_desc(experts, top_k, score, groups, top_groups, group_top, renormalise, weight_scale):
+    scores = {"softmax": N.SCORE_SOFTMAX, "sigmoid": N.SCORE_SIGMOID}
+    if score not in scores:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    return N.RouteDesc(experts, top_k, scores[score], groups, top_groups, group_top,
+                       int(bool(renormalise)), weight_scale)
+
+
+def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int = 1,
+                  top_groups: int = 1, group_top: int = 1, renormalise: bool = True,
+                  weight_scale: float = 1.0, stream=None):
+    """(selected int32 [T, top_k], weights float32 [T, top_k]) of router logits
+    [T, experts] (float32 or bfloat16 CUDA tensor, rows of any stride; or a
+    numpy array, then numpy arrays come back).
+
+    Scores are the softmax or sigmoid of a token's logits; the choice goes by
+    score + bias (float32 [experts]), within the `top_groups` best of `groups`
+    equal groups, a group's rank being its largest choice (group_top 1) or the
+    sum of its two largest (2).  Experts come in decreasing order, equal ones by
+    index; the order is that of exact scores.  Weights are the scores without
+    bias, divided by their sum with `renormalise`, times `weight_scale`.  An
+    expert with a logit of -inf has score 0 and is chosen last."""
+    if not hasattr(logits, "data_ptr"):
+        return _route_host(logits, bias, _route_desc(
+            np.shape(logits)[-1], top_k, score, groups, top_groups, group_top, renormalise,
+            weight_scale))
+    torch = _torch()
+    _device_tensor(logits, "logits", _floats(), 2)
+    T, E = logits.shape
+    dev = logits.device
+    if bias is not None:
+        _device_tensor(bias, "bias", (torch.float32,), 1, (E,), dev)
+    desc = _route_desc(E, top_k, score, groups, top_groups, group_top, renormalise, weight_scale)
+    if not 1 <= top_k <= E:
+        raise ValueError(f"top_k must be in 1..{E}, got {top_k}")
+    ctx, raw = _on(stream, dev)
+    with ctx:
+        selected = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+        weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    N._check(N.lib().llambda_cuda_route_device(
+        C.byref(desc), _tag(logits.dtype), logits.data_ptr(), _row_stride(logits),
+        bias.data_ptr() if bias is not None else None, T, selected.data_ptr(), weights.data_ptr(),
+        raw))
+    return selected, weights
+
+
+def _route_host(logits, bias, desc):
+    logits = N._f32(logits)
+    if logits.ndim != 2 or 0 in logits.shape:
+        raise ValueError("logits must be [tokens][experts] with a positive token count")
+    if bias is not None:
+        bias = N._f32(bias)
+        if bias.shape != (desc.experts,):
+            raise ValueError(f"bias must have shape ({desc.experts},)")
+    if not 1 <= desc.top_k <= desc.experts:
+        raise ValueError(f"top_k must be in 1..{desc.experts}, got {desc.top_k}")
+    T = logits.shape[0]
+    selected = np.empty((T, desc.top_k), np.int32)
+    weights = np.empty((T, desc.top_k), np.float32)
+    N._check(N.lib().llambda_cuda_route(
+        C.byref(desc), logits.ctypes.data, bias.ctypes.data if bias is not None else None, T,
+        selected.ctypes.data, weights.ctypes.data))
+    return selected, weights
+
+
+# ------------------------------------------------------------------ 8-bit floating point
+
+
+def fp8_quantize(x, *, stream=None):
+    """(q, scales) of x [T, cols] (float32 or bfloat16): q float8_e4m3fn
+    [T, cols rounded up to 16] with zeros past cols, scales float32
+    [ceil(cols / 128), T rounded up to 4] with zeros past T, so that x[t, c] is
+    about q[t, c] * scales[c // 128, t].  scale = max(max|x| / 448, 2^-126) of
+    the row's block, q = e4m3(x / scale), everything rounded to nearest."""
+    torch = _torch()
+    _device_tensor(x, "x", _floats(), 2)
+    T, cols = x.shape
+    ctx, raw = _on(stream, x.device)
+    with ctx:
+        q = torch.empty(T, _pad(cols, 16), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty(_blocks(cols), _pad(T, 4), dtype=torch.float32, device=x.device)
+    N._check(N.lib().llambda_cuda_fp8_quantize_device(
+        _tag(x.dtype), x.data_ptr(), _row_stride(x), T, cols, q.data_ptr(), scales.data_ptr(), raw))
+    return q, scales
+
+
+def _device_weights(pair, name: str, ndim: int, device=None):
+    """Checks (weights, scales) in device memory."""
+    torch = _torch()
+    w, s = pair
+    _device_tensor(w, f"{name} weights", (torch.float8_e4m3fn, torch.uint8), ndim, device=device,
+                   contiguous=True)
+    want = tuple(w.shape[:-2]) + (_blocks(w.shape[-2]), _blocks(w.shape[-1]))
+    _device_tensor(s, f"{name} scales", (torch.float32,), ndim, want, w.device, contiguous=True)
+    return w, s
+
+
+def _host_weights(pair, name: str, ndim: int):
+    w, s = pair
+    w = np.ascontiguousarray(w)
+    if w.dtype.itemsize != 1 or w.ndim != ndim or 0 in w.shape:
+        raise ValueError(f"{name} weights must be e4m3 bytes with {ndim} axes")
+    w = w.view(np.uint8)
+    s = N._f32(s)
+    want = w.shape[:-2] + (_blocks(w.shape[-2]), _blocks(w.shape[-1]))
+    if s.shape != want:
+        raise ValueError(f"{name} scales have shape {s.shape}, expected {want}")
+    return w, s
+
+
+def _fp8_tensor(shape, data: int, scales: int):
+    ne2 = shape[0] if len(shape) == 3 else 1
+    return N.Fp8Tensor(shape[-1], shape[-2], ne2, data, scales)
+
+
+class _Fp8Session:
+    """What both kinds of session share: the handle and the memory it borrows."""
+    _destroy = _status = ""
+
+    def status(self) -> int:
+        """The device-side status word, cleared by reading: 0, or 2 after a wait
+        inside a kernel timed out."""
+        rc = getattr(N.lib(), self._status)(self._h)
+        if rc < 0:
+            raise N.LlambdaCudaError(N.last_error())
+        return rc
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            getattr(N.lib(), self._destroy)(self._h)
+            self._h = None
+        self._keep = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _handle(self):
+        if not self._h:
+            raise ValueError("the session is closed")
+        return self._h
+
+
+class Fp8ProjectionSession(_Fp8Session):
+    """One e4m3 matrix [rows][cols] with a scale per 128 x 128 block, resident on
+    the GPU: run* returns x . W^T."""
+    _destroy = "llambda_cuda_fp8_session_destroy"
+    _status = "llambda_cuda_fp8_session_status"
+
+    def __init__(self, handle, rows: int, cols: int, device=None, keep=None):
+        self._h, self._keep = handle, keep
+        self.rows, self.cols, self.device = rows, cols, device
+
+    @classmethod
+    def _create(cls, w, s, data, scales, on_device, device, keep):
+        h = C.c_void_p()
+        t = _fp8_tensor(w.shape, data, scales)
+        N._check(N.lib().llambda_cuda_fp8_session_create(C.byref(t), on_device, C.byref(h)))
+        return cls(h, w.shape[0], w.shape[1], device, keep)
+
+    @classmethod
+    def from_tensor(cls, weights, scales):
+        """Copies host arrays: weights [rows][cols] of e4m3 bytes, scales
+        [ceil(rows / 128)][ceil(cols / 128)] float32."""
+        w, s = _host_weights((weights, scales), "projection", 2)
+        return cls._create(w, s, w.ctypes.data, s.ctypes.data, 0, None, None)
+
+    @classmethod
+    def from_device(cls, weights, scales):
+        """Borrows CUDA tensors (kept alive by the session): weights
+        float8_e4m3fn or uint8, cols a multiple of 16."""
+        w, s = _device_weights((weights, scales), "projection", 2)
+        with _torch().cuda.device(w.device):
+            return cls._create(w, s, w.data_ptr(), s.data_ptr(), 1, w.device, (w, s))
+
+    def run(self, x: np.ndarray) -> np.ndarray:
+        """Host arrays: x [T][cols] (or one vector) -> [T][rows] float32."""
+        x = N._f32(x)
+        one = x.ndim == 1
+        x = x.reshape(1, -1) if one else x
+        if x.ndim != 2 or x.shape[1] != self.cols or not x.size:
+            raise ValueError(f"x must be [tokens][{self.cols}]")
+        out = np.empty((x.shape[0], self.rows), np.float32)
+        N._check(N.lib().llambda_cuda_fp8_session_run(self._handle(), x.ctypes.data, x.shape[0],
+                                                      out.ctypes.data))
+        return out[0] if one else out
+
+    def run_device(self, x, out=None, *, out_dtype=None, stream=None):
+        """x [T, cols] (float32 or bfloat16 CUDA tensor) -> out [T, rows], made
+        of `out_dtype` (default x's) unless given."""
+        torch = _torch()
+        h = self._handle()
+        _device_tensor(x, "x", _floats(), 2, (None, self.cols), self.device)
+        T = x.shape[0]
+        ctx, raw = _on(stream, x.device)
+        with ctx:
+            out = _out(out, T, self.rows, out_dtype or x.dtype, x.device)
+            nbytes = N.lib().llambda_cuda_fp8_session_workspace(h, T)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N._check(N.lib().llambda_cuda_fp8_session_run_device(
+            h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, _tag(out.dtype), out.data_ptr(),
+            _row_stride(out), work.data_ptr(), nbytes, raw))
+        return out
+
+    def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):
+        """As run_device over what fp8_quantize returned for `tokens` rows of
+        `cols` columns (several projections of one input quantise it once)."""
+        torch = _torch()
+        h = self._handle()
+        _device_tensor(q, "q", (torch.float8_e4m3fn, torch.uint8), 2, (tokens, _pad(self.cols, 16)),
+                       self.device, contiguous=True)
+        _device_tensor(scales, "scales", (torch.float32,), 2, (_blocks(self.cols), _pad(tokens, 4)),
+                       q.device, contiguous=True)
+        ctx, raw = _on(stream, q.device)
+        with ctx:
+            out = _out(out, tokens, self.rows, out_dtype or torch.float32, q.device)
+        N._check(N.lib().llambda_cuda_fp8_session_run_quantized(
+            h, q.data_ptr(), scales.data_ptr(), tokens, _tag(out.dtype), out.data_ptr(),
+            _row_stride(out), raw))
+        return out
+
+
+class Fp8MoeSession(_Fp8Session):
+    """The routed experts of one layer in e4m3: expert e of an input x gives
+    down_e . q(h), h = silu(gate_e . x) * (up_e . x), or relu(up_e . x)^2 without
+    gate, x and h quantised as by fp8_quantize.  up and gate are [E][I][H], down
+    [E][O][I], each a pair (weights, scales [E][ceil(rows/128)][ceil(cols/128)])."""
+    _destroy = "llambda_cuda_fp8_moe_session_destroy"
+    _status = "llambda_cuda_fp8_moe_session_status"
+
+    def __init__(self, handle, experts: int, hidden: int, out_features: int, device=None,
+                 keep=None):
+        self._h, self._keep = handle, keep
+        self.experts, self.hidden, self.out_features = experts, hidden, out_features
+        self.device = device
+
+    @classmethod
+    def _create(cls, up, down, gate, ptr, on_device, device):
+        ts = [_fp8_tensor(p[0].shape, ptr(p[0]), ptr(p[1])) if p is not None
+              else N.Fp8Tensor(0, 0, 0, None, None) for p in (gate, up, down)]
+        h = C.c_void_p()
+        N._check(N.lib().llambda_cuda_fp8_moe_session_create(
+            C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h)))
+        E, _, H = up[0].shape
+        return cls(h, E, H, down[0].shape[1], device, (up, down, gate) if on_device else None)
+
+    @classmethod
+    def from_tensor(cls, up, down, gate=None):
+        """Copies host arrays of e4m3 bytes and float32 scales."""
+        up, down = _host_weights(up, "up", 3), _host_weights(down, "down", 3)
+        gate = _host_weights(gate, "gate", 3) if gate is not None else None
+        return cls._create(up, down, gate, lambda a: a.ctypes.data, 0, None)
+
+    @classmethod
+    def from_device(cls, up, down, gate=None):
+        """Borrows CUDA tensors (kept alive by the session), H and I multiples
+        of 16."""
+        up = _device_weights(up, "up", 3)
+        dev = up[0].device
+        down = _device_weights(down, "down", 3, dev)
+        gate = _device_weights(gate, "gate", 3, dev) if gate is not None else None
+        with _torch().cuda.device(dev):
+            return cls._create(up, down, gate, lambda t: t.data_ptr(), 1, dev)
+
+    def run(self, x: np.ndarray, selected: np.ndarray, weights: np.ndarray) -> np.ndarray:
+        """Host arrays: x [T][H], selected and weights [T][k] -> [T][O] float32."""
+        x, weights = N._f32(x), N._f32(weights)
+        selected = np.ascontiguousarray(selected, dtype=np.int32)
+        if x.ndim != 2 or x.shape[1] != self.hidden or not x.size:
+            raise ValueError(f"x must be [tokens][{self.hidden}]")
+        if selected.ndim != 2 or selected.shape[0] != x.shape[0] or not selected.size \
+                or weights.shape != selected.shape:
+            raise ValueError("selected and weights must both be [tokens][k]")
+        out = np.empty((x.shape[0], self.out_features), np.float32)
+        N._check(N.lib().llambda_cuda_fp8_moe_session_run(
+            self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
+            weights.ctypes.data, out.ctypes.data))
+        return out
+
+    def run_device(self, x, selected, weights, out=None, *, out_dtype=None, stream=None):
+        """x [T, H] (float32 or bfloat16), selected int32 and weights float32
+        [T, k] (route_experts' results) -> out [T, O] = the weighted sum over a
+        token's entries, made of `out_dtype` (default x's) unless given.  Entries
+        whose expert is outside 0..E-1 add nothing."""
+        torch = _torch()
+        h = self._handle()
+        _device_tensor(x, "x", _floats(), 2, (None, self.hidden), self.device)
+        T, dev = x.shape[0], x.device
+        _device_tensor(selected, "selected", (torch.int32,), 2, (T, None), dev, contiguous=True)
+        k = selected.shape[1]
+        _device_tensor(weights, "weights", (torch.float32,), 2, (T, k), dev, contiguous=True)
+        ctx, raw = _on(stream, dev)
+        with ctx:
+            out = _out(out, T, self.out_features, out_dtype or x.dtype, dev)
+            nbytes = N.lib().llambda_cuda_fp8_moe_session_workspace(h, T, k)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        N._check(N.lib().llambda_cuda_fp8_moe_session_run_device(
+            h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, k, selected.data_ptr(),
+            weights.data_ptr(), _tag(out.dtype), out.data_ptr(), _row_stride(out), work.data_ptr(),
+            nbytes, raw))
+        return out
