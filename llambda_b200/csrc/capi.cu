@@ -84,11 +84,17 @@ int current_device() {
 }
 
 void require_b200(int dev) {
+  // the attributes cost microseconds, the full properties milliseconds
+  int major = 0, minor = 0;
+  cuda_check(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev),
+             "cudaDeviceGetAttribute");
+  cuda_check(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev),
+             "cudaDeviceGetAttribute");
+  if (major == 10 && minor == 0) return;
   cudaDeviceProp p;
   cuda_check(cudaGetDeviceProperties(&p, dev), "cudaGetDeviceProperties");
-  if (p.major != 10 || p.minor != 0)
-    throw Failure(std::string("device ") + p.name + " is sm_" + std::to_string(p.major) +
-                  std::to_string(p.minor) + "; this library is built for sm_100a (B200)");
+  throw Failure(std::string("device ") + p.name + " is sm_" + std::to_string(p.major) +
+                std::to_string(p.minor) + "; this library is built for sm_100a (B200)");
 }
 
 // Device allocation with 256 bytes of slack: the Q6_K loaders read up to
@@ -1391,20 +1397,25 @@ size_t f8_quant_bytes(uint64_t cols, size_t tokens, size_t* scales_at) {
   return q + (((cols + 127) / 128 * (size_t)lb::f8_pad4((long)tokens) * 4 + 255) & ~size_t(255));
 }
 
-// Device copies owned by a session, freed with it.
+// What both kinds of session own.  The stream is for the host-buffer calls
+// and made by the first of them; a session over borrowed tensors holds one
+// small allocation, the status word and the counter of the scale checks.
 struct F8Owner {
   int device = 0;
   cudaStream_t stream = nullptr;
-  int* status = nullptr;
+  int* status = nullptr;  // [0] status, [1] scales that are not finite
   std::vector<void*> owned;
   std::mutex mu;
   DevBuf din, dout, dwork, dsel, dw;
   void open() {
     device = current_device();
     require_b200(device);
-    cuda_check(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking), "cudaStreamCreate");
-    cuda_check(cudaMalloc(&status, sizeof(int)), "cudaMalloc");
-    cuda_check(cudaMemsetAsync(status, 0, sizeof(int), stream), "memset");
+    cuda_check(cudaMalloc(&status, 2 * sizeof(int)), "cudaMalloc");
+    cuda_check(cudaMemset(status, 0, 2 * sizeof(int)), "memset");
+  }
+  void open_stream() {
+    if (!stream)
+      cuda_check(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking), "cudaStreamCreate");
   }
   ~F8Owner() {
     if (stream) cudaStreamDestroy(stream);
@@ -1434,34 +1445,28 @@ struct F8Owner {
       require_align(t.scales, 4, (name + " scales").c_str());
       m.data = static_cast<const uint8_t*>(t.data);
       m.scales = t.scales;
-      // the borrowed memory may still be being written on the default stream
-      cuda_check(cudaStreamSynchronize(nullptr), "synchronize");
     } else {
       void* d = dev_alloc(rows * m.pitch);
       owned.push_back(d);
-      void* s = dev_alloc(nscales * 4);
-      owned.push_back(s);
-      cuda_check(cudaMemcpy2DAsync(d, m.pitch, t.data, t.ne0, t.ne0, rows, cudaMemcpyHostToDevice,
-                                   stream),
+      void* sc = dev_alloc(nscales * 4);
+      owned.push_back(sc);
+      cuda_check(cudaMemcpy2D(d, m.pitch, t.data, t.ne0, t.ne0, rows, cudaMemcpyHostToDevice),
                  "upload tensor");
-      cuda_check(cudaMemcpyAsync(s, t.scales, nscales * 4, cudaMemcpyHostToDevice, stream),
-                 "upload scales");
+      cuda_check(cudaMemcpy(sc, t.scales, nscales * 4, cudaMemcpyHostToDevice), "upload scales");
       m.data = static_cast<const uint8_t*>(d);
-      m.scales = static_cast<const float*>(s);
+      m.scales = static_cast<const float*>(sc);
     }
-    unsigned* bad = nullptr;
-    unsigned host = 0;
-    cuda_check(cudaMalloc(&bad, sizeof(unsigned)), "cudaMalloc");
-    cudaError_t e = cudaMemsetAsync(bad, 0, sizeof(unsigned), stream);
-    if (e == cudaSuccess) e = lb::f8_check_scales(m.scales, nscales, bad, stream);
-    if (e == cudaSuccess)
-      e = cudaMemcpyAsync(&host, bad, sizeof(unsigned), cudaMemcpyDeviceToHost, stream);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    cudaFree(bad);
-    cuda_check(e, "scale check");
-    if (host) throw Failure(name + ": " + std::to_string(host) + " scale(s) are not finite.");
+    cuda_check(lb::f8_check_scales(m.scales, nscales, reinterpret_cast<unsigned*>(status + 1),
+                                   cudaStreamLegacy),
+               "scale check");
     cuda_check(lb::f8_prepare(&m), "tensor map");
     return m;
+  }
+  // After the last matrix: the result of the scale checks.
+  void checked() {
+    int bad = 0;
+    cuda_check(cudaMemcpy(&bad, status + 1, sizeof(int), cudaMemcpyDeviceToHost), "scale check");
+    if (bad) throw Failure(std::to_string(bad) + " block scale(s) are not finite.");
   }
   // Reads and clears the status word; the stream's work is waited for.
   int take_status() {
@@ -1587,8 +1592,7 @@ int llambda_cuda_fp8_quantize_device(int type, const void* device_x, int64_t ldx
     require_align(device_q, 16, "quantised output");
     require_align(device_scales, 16, "scales");
     cuda_check(lb::launch_f8_quant(is_bf16(type, "input"), device_x, ldx, T, (int)cols,
-                                   static_cast<uint8_t*>(device_q), lb::f8_pad16((long)cols),
-                                   device_scales, lb::f8_pad4(T), nullptr, 0,
+                                   static_cast<uint8_t*>(device_q), device_scales,
                                    static_cast<cudaStream_t>(cuda_stream)),
                "quantise launch");
     return 0;
@@ -1609,6 +1613,7 @@ int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor, int o
     try {
       s->open();
       s->w = s->matrix(*tensor, on_device != 0, "projection tensor");
+      s->checked();
     } catch (...) {
       delete s;
       throw;
@@ -1631,9 +1636,7 @@ static void f8_project_call(llambda_cuda_fp8_session* s, bool x_bf16, const void
   f8_quant_bytes(s->w.cols, T, &at);
   uint8_t* q = static_cast<uint8_t*>(work);
   float* sc = reinterpret_cast<float*>(q + at);
-  cuda_check(lb::launch_f8_quant(x_bf16, x, ldx, T, s->w.cols, q, lb::f8_pad16(s->w.cols), sc,
-                                 lb::f8_pad4(T), nullptr, 0, st),
-             "quantise launch");
+  cuda_check(lb::launch_f8_quant(x_bf16, x, ldx, T, s->w.cols, q, sc, st), "quantise launch");
   cuda_check(lb::launch_f8_project(s->w, q, sc, T, out_bf16, out, ldo, s->status, st),
              "product launch");
 }
@@ -1648,6 +1651,7 @@ int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* s, const float* x, si
     const int T = token_count(tokens);
     std::lock_guard<std::mutex> lock(s->mu);
     DeviceGuard g(s->device);
+    s->open_stream();
     const size_t in = tokens * s->w.cols * 4, ob = tokens * s->w.rows * 4;
     float* din = static_cast<float*>(s->din.get(in));
     float* dout = static_cast<float*>(s->dout.get(ob));
@@ -1738,6 +1742,7 @@ int llambda_cuda_fp8_moe_session_create(const llambda_cuda_fp8_tensor* gate,
       if (gated) s->m.gate = s->matrix(*gate, on_device != 0, "gate tensor");
       s->m.up = s->matrix(*up, on_device != 0, "up tensor");
       s->m.down = s->matrix(*down, on_device != 0, "down tensor");
+      s->checked();
     } catch (...) {
       delete s;
       throw;
@@ -1768,6 +1773,7 @@ int llambda_cuda_fp8_moe_session_run(llambda_cuda_fp8_moe_session* s, const floa
     moe_call_sizes(s, tokens, top_k);
     std::lock_guard<std::mutex> lock(s->mu);
     DeviceGuard g(s->device);
+    s->open_stream();
     const int H = s->m.up.cols, O = s->m.down.rows;
     const size_t in = tokens * H * 4, ob = tokens * O * 4, eb = tokens * top_k * 4;
     float* din = static_cast<float*>(s->din.get(in));

@@ -16,6 +16,8 @@
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "engine.cuh"
 #include "kernels.h"
@@ -41,6 +43,10 @@ enum F8Mode {
 // e4m3 of v as a byte: round to nearest even, NaN stays NaN.
 __device__ __forceinline__ uint32_t e4m3_byte(float v) {
   return (uint32_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
 // The scale of a block whose largest magnitude has the bits `amax` (a NaN's
@@ -73,48 +79,125 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, int n, f
   }
 }
 
-// One warp per (token, block of 128 columns), four columns a lane.  q has rows
-// of q_pitch bytes (a multiple of 16, zeros past cols), scales the layout
-// [block][s_pitch] the products read with bulk copies.  With `rows` the
-// token's row goes to its k grouped rows (those that are not negative);
-// without, to row t, and the scales of rows [tokens, s_pitch) are zeroed.
-template <typename T>
+// Where a token's quantised row goes: row t, or the grouped rows of its k
+// entries (those whose expert is in [0, E)), row_start[expert] + pos[entry].
+struct F8Rows {
+  const int *sel, *pos, *row_start;  // null: row t
+  int* entry;                        // receives the entry of each grouped row
+  int k, E;
+};
+
+constexpr int kQuantBlocks = 4;  // blocks of one token per warp
+
+// One warp per token and kQuantBlocks blocks of 128 columns, four columns a
+// lane and block, every load issued before the first is used.  q has rows of
+// q_pitch bytes (a multiple of 16, zeros past cols), scales the layout
+// [block][s_pitch] the products read with bulk copies; ungrouped, the scales
+// of rows [tokens, s_pitch) are zeroed.
+//
+// x / s has to be the correctly rounded quotient (a quotient a bit off turns
+// over the ties of bf16 inputs).  With r the correctly rounded 1 / s and q0 =
+// x * r, q0 + r * (x - q0 * s) is it (Markstein, IBM J. Res. Dev. 34, 1990),
+// three instructions a value, as long as nothing underflows; blocks whose
+// scale is outside [2^-80, 2^100] divide.
+//
+// Bound by memory; the four blocks' scales are computed side by side on the
+// lanes, one division and one reciprocal for all.
+template <typename T, bool GROUPED>
 __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, long ldx,
                                                        int tokens, int cols, uint8_t* q,
-                                                       long q_pitch, float* scales, long s_pitch,
-                                                       const int* rows, int k, int vec) {
+                                                       int q_pitch, float* scales, int s_pitch,
+                                                       F8Rows rows, int vec) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
   const int blocks = (cols + kF8Block - 1) / kF8Block;
-  const long n = (rows ? (long)tokens : s_pitch) * blocks;
-  for (long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (long)gridDim.x * 8) {
-    const long t = i / blocks;
-    const int b = (int)(i - t * blocks);
-    if (t >= tokens) {
-      if (lane == 0) scales[b * s_pitch + t] = 0.0f;
-      continue;
+  const unsigned per = (blocks + kQuantBlocks - 1) / kQuantBlocks;
+  const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int t = (int)(unit / per), b0 = (int)(unit - t * per) * kQuantBlocks;
+  if (t >= (GROUPED ? tokens : s_pitch)) return;
+  const bool mine = lane < kQuantBlocks && b0 + lane < blocks;  // this lane's scale exists
+  float* sp = scales + (long)(b0 + lane) * s_pitch;
+  if (t >= tokens) {
+    if (mine) sp[t] = 0.0f;
+    return;
+  }
+  const int c0 = b0 * kF8Block + 4 * lane;
+  const T* src = x + t * ldx + c0;
+  const bool whole = (b0 + kQuantBlocks) * kF8Block <= cols;
+  float v[kQuantBlocks][4];
+  if (vec && whole) {
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) load4(src + i * kF8Block, true, 4, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const int c = c0 + i * kF8Block;
+      v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+      if (c < cols) load4(src + i * kF8Block, vec && c + 4 <= cols, cols - c, v[i]);
     }
-    const int c = b * kF8Block + 4 * lane;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < cols) load4(x + t * ldx + c, vec && c + 4 <= cols, cols - c, v);
+  }
+  uint32_t am = 0;  // lane i: the largest magnitude of block i
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks; ++i) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-    const float s = block_scale(__reduce_max_sync(0xffffffffu, m));
-    uint32_t w = 0;
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == i) am = m;
+  }
+  const float s_own = block_scale(am);
+  const float r_own = __frcp_rn(s_own);
+  const bool plain = __all_sync(0xffffffffu,
+                                !mine || am == 0 || (s_own >= 0x1p-80f && s_own <= 0x1p100f));
+  uint32_t w[kQuantBlocks];
+  if (plain) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w |= e4m3_byte(__fdiv_rn(v[j], s)) << (8 * j);
-    if (!rows) {
-      if (c < q_pitch) *reinterpret_cast<uint32_t*>(q + t * q_pitch + c) = w;
-      if (lane == 0) scales[b * s_pitch + t] = s;
-    } else {
-      for (int j = 0; j < k; ++j) {
-        const int r = __ldcg(rows + t * k + j);
-        if (r < 0) continue;
-        if (c < q_pitch) *reinterpret_cast<uint32_t*>(q + r * q_pitch + c) = w;
-        if (lane == 0) scales[b * s_pitch + r] = s;
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const float s = __shfl_sync(0xffffffffu, s_own, i), r = __shfl_sync(0xffffffffu, r_own, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float q0 = __fmul_rn(v[i][j], r);
+        v[i][j] = fmaf(r, fmaf(-q0, s, v[i][j]), q0);
       }
+      w[i] = e4m3_pair(v[i][0], v[i][1]) | e4m3_pair(v[i][2], v[i][3]) << 16;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const float s = __shfl_sync(0xffffffffu, s_own, i);
+      uint32_t wi = 0;
+#pragma unroll
+      for (int ii = 0; ii < kQuantBlocks; ++ii)
+        if (ii == i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wi |= e4m3_byte(__fdiv_rn(v[ii][j], s)) << (8 * j);
+#pragma unroll
+      for (int ii = 0; ii < kQuantBlocks; ++ii)
+        if (ii == i) w[ii] = wi;
+    }
+  }
+  auto store = [&](long o) {
+    uint32_t* dst = reinterpret_cast<uint32_t*>(q + o * q_pitch + c0);
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kQuantBlocks; ++i) dst[i * (kF8Block / 4)] = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kQuantBlocks; ++i)
+        if (c0 + i * kF8Block < q_pitch) dst[i * (kF8Block / 4)] = w[i];
+    }
+    if (mine) sp[o] = s_own;
+  };
+  if (!GROUPED) {
+    store(t);
+  } else {
+    for (int j = 0; j < rows.k; ++j) {
+      const int id = t * rows.k + j, e = __ldg(rows.sel + id);
+      if (e < 0 || e >= rows.E) continue;
+      const int o = __ldcg(rows.row_start + e) + __ldcg(rows.pos + id);
+      if (b0 == 0 && lane == 0) rows.entry[o] = id;
+      store(o);
     }
   }
 }
@@ -209,6 +292,33 @@ __device__ __forceinline__ void tmem_wait_ld8(uint32_t* r) {
                : "memory");
 }
 
+// Bounded wait of the product kernel's pipelines: a try_wait without a time
+// hint returns as soon as the phase completes.
+__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, int* status,
+                                        volatile int* abort) {
+  auto attempt = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n "
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  if (attempt()) return true;
+  const uint64_t t0 = global_ns();
+  for (;;) {
+    for (int i = 0; i < 16; ++i)
+      if (attempt()) return true;
+    if (*abort) return false;
+    if (global_ns() - t0 >= kWaitLimitNs) break;
+  }
+  if (status) atomicOr(status, 2);
+  *abort = 1;
+  return false;
+}
+
 struct F8Tile {
   int row0, count, expert, rb;  // first row of x, valid rows, expert, row block
 };
@@ -288,7 +398,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         const F8Tile t = f8_tile<NT>(p, tile);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (q >= C::kStages &&
-              !mbar_wait_or_abort(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort))
+              !f8_wait(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort))
             break;
           uint8_t* st = stages + (size_t)rp.s * C::kStage;
           uint64_t* bar = &sy->full[rp.s];
@@ -318,7 +428,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (q >= kF8Scales &&
-              !mbar_wait_or_abort(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort))
+              !f8_wait(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort))
             break;
           mbar_expect_tx(&sy->sfull[rp.s], bytes);
           tma_load_1d(s_scale + rp.s * NT, p.xs + kb * p.xs_pitch + t.row0, bytes,
@@ -341,8 +451,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = (q < C::kBufs ||
-                mbar_spin_or_abort(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
-               mbar_spin_or_abort(&sy->full[rp.s], rp.phase, p.status, abort);
+                f8_wait(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
+               f8_wait(&sy->full[rp.s], rp.phase, p.status, abort);
           if (!ok) break;
           tc_fence_after();
           const uint8_t* st = stages + (size_t)rp.s * C::kStage;
@@ -382,6 +492,12 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 #pragma unroll
         for (int c = 0; c < NC / 2; ++c) acc[m][c] = make_float2(0.0f, 0.0f);
       float wl[MATS];  // weight scales of 32 blocks, one a lane
+      int ent[(NC + 31) / 32];  // entries of this thread's tokens, 32 a register
+      if (MODE == kF8Partial) {
+#pragma unroll
+        for (int i = 0; i < (NC + 31) / 32; ++i)
+          ent[i] = 32 * i + lane < mine ? __ldcg(p.entry + t.row0 + half * NC + 32 * i + lane) : 0;
+      }
       for (int kb = 0; kb < p.kblocks; ++kb) {
         if ((kb & 31) == 0) {
           const bool in = kb + lane < p.kblocks;
@@ -391,13 +507,15 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         float sw[MATS];
 #pragma unroll
         for (int m = 0; m < MATS; ++m) sw[m] = __shfl_sync(0xffffffffu, wl[m], kb & 31);
-        ok = mbar_wait_or_abort(&sy->sfull[sp.s], sp.phase, p.status, abort) &&
-             mbar_wait_or_abort(&sy->tfull[ap.s], ap.phase, p.status, abort);
+        ok = f8_wait(&sy->sfull[sp.s], sp.phase, p.status, abort) &&
+             f8_wait(&sy->tfull[ap.s], ap.phase, p.status, abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         const float* sc = s_scale + sp.s * NT + half * NC;
-        constexpr int CH = NC < 16 ? NC : 16;  // columns loaded together
+        // columns loaded together: all of them while the registers last, since the
+        // loads of a second group wait for the first
+        constexpr int CH = NC < 64 / MATS ? NC : 64 / MATS;
 #pragma unroll
         for (int c0 = 0; c0 < NC; c0 += CH) {
           if (c0 < mine) {  // warp-uniform
@@ -417,10 +535,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
               const float4 sx = *reinterpret_cast<const float4*>(sc + c0 + j);
 #pragma unroll
               for (int m = 0; m < MATS; ++m) {
-                ffma2(acc[m][(c0 + j) / 2], __uint_as_float(d[m][j]),
-                      __uint_as_float(d[m][j + 1]), sx.x * sw[m], sx.y * sw[m]);
-                ffma2(acc[m][(c0 + j) / 2 + 1], __uint_as_float(d[m][j + 2]),
-                      __uint_as_float(d[m][j + 3]), sx.z * sw[m], sx.w * sw[m]);
+                const float2 w = make_float2(sw[m], sw[m]);
+                acc[m][(c0 + j) / 2] =
+                    __ffma2_rn(make_float2(__uint_as_float(d[m][j]), __uint_as_float(d[m][j + 1])),
+                               __fmul2_rn(make_float2(sx.x, sx.y), w), acc[m][(c0 + j) / 2]);
+                acc[m][(c0 + j) / 2 + 1] = __ffma2_rn(
+                    make_float2(__uint_as_float(d[m][j + 2]), __uint_as_float(d[m][j + 3])),
+                    __fmul2_rn(make_float2(sx.z, sx.w), w), acc[m][(c0 + j) / 2 + 1]);
               }
             }
           }
@@ -451,14 +572,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             }
         }
       } else if (MODE == kF8Partial) {
-        if (row < p.rows) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
-            if (c < mine) {
-              const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
-              p.partial[(long)__ldcg(p.entry + tok0 + c) * p.ldp + row] = y;
-            }
-        }
+        for (int c = 0; c < NC; ++c)
+          if (c < mine) {  // warp-uniform
+            const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
+            const long id = __shfl_sync(0xffffffffu, ent[c / 32], c & 31);
+            if (row < p.rows) p.partial[id * p.ldp + row] = y;
+          }
       } else {
         // the 128 rows of this tile are one block of the next product's K:
         // its scale per token is a maximum over the four warps of this half
@@ -503,23 +623,29 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
 // ------------------------------------------------------------ experts
 
-// One CTA: groups the entries (token t, rank j; id t * k + j) by expert.
-// Every expert's rows start at a multiple of 4 (the scales' bulk copies start
-// on 16 bytes); chunks of at most nt rows go to tiles in expert order.
-// Entries whose expert is outside [0, E) get row -1.  The order within an
-// expert follows arrival and changes no value: every row is computed alone.
+// One CTA: groups the entries (token t, rank j; id t * k + j) by expert:
+// entry i's row is row_start[expert] + pos[i].  Every expert's rows start at a
+// multiple of 4 (the scales' bulk copies start on 16 bytes); chunks of at most
+// nt rows go to tiles in expert order.  Entries whose expert is outside [0, E)
+// are in no group.  The order within an expert follows arrival and changes no
+// value: every row is computed alone.
 __global__ void __launch_bounds__(1024) f8_plan_kernel(const int* __restrict__ sel, int n, int E,
-                                                       int nt, int* row_of, int* entry,
+                                                       int nt, int* pos, int* row_start,
                                                        int4* tiles, int* nchunks) {
-  __shared__ int s_count[1024], s_row[1024], s_warp[2][32];
+  constexpr int kPer = 8;  // entries of a thread whose loads are in flight together
+  __shared__ int s_count[1024], s_warp[2][32];
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   s_count[tid] = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += 1024) {
-    const int e = sel[i];
-    row_of[i] = e >= 0 && e < E ? atomicAdd(&s_count[e], 1) : -1;
+  for (int i0 = tid; i0 < n; i0 += 1024 * kPer) {
+    int e[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) e[j] = i0 + 1024 * j < n ? sel[i0 + 1024 * j] : -1;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (e[j] >= 0 && e[j] < E) pos[i0 + 1024 * j] = atomicAdd(&s_count[e[j]], 1);
   }
   __syncthreads();
   const int cnt = s_count[tid], pad = (cnt + 3) & ~3, ch = (cnt + nt - 1) / nt;
@@ -543,25 +669,18 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const int* __restrict__ s
   __syncthreads();
   const int row = a - pad + (warp ? s_warp[0][warp - 1] : 0);
   const int chunk = b - ch + (warp ? s_warp[1][warp - 1] : 0);
-  s_row[tid] = row;
+  if (tid < E) row_start[tid] = row;
   for (int c = 0; c < ch; ++c)
     tiles[chunk + c] = make_int4(row + c * nt, min(nt, cnt - c * nt), tid, 0);
   if (tid == 1023) *nchunks = s_warp[1][31];
-  __syncthreads();
-  for (int i = tid; i < n; i += 1024) {
-    const int pos = row_of[i];
-    if (pos < 0) continue;
-    const int r = s_row[sel[i]] + pos;
-    row_of[i] = r;
-    entry[r] = i;
-  }
 }
 
-// out[t] = sum over ranks j, in order, of weight * partial row; entries with
-// row -1 add nothing.  Four columns a thread.
+// out[t] = sum over ranks j, in order, of weight * partial row; entries whose
+// expert is outside [0, E) add nothing.  Four columns a thread.
 __global__ void __launch_bounds__(256) f8_combine_kernel(const float* partial, long ldp,
-                                                         const int* row_of, const float* weights,
-                                                         int k, int cols, void* out, long ldo,
+                                                         const int* sel, int E,
+                                                         const float* weights, int k, int cols,
+                                                         void* out, long ldo,
                                                          int out_bf16) {
   griddep_wait();
   griddep_launch();
@@ -569,7 +688,8 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* partial, l
   for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int j = 0; j < k; ++j) {
-      if (__ldcg(row_of + t * k + j) < 0) continue;
+      const int e = sel[t * k + j];
+      if (e < 0 || e >= E) continue;
       const float w = weights[t * k + j];
       const float4 v = __ldcg(reinterpret_cast<const float4*>(partial + (t * k + j) * ldp + c));
       a[0] = fmaf(w, v.x, a[0]), a[1] = fmaf(w, v.y, a[1]);
@@ -635,11 +755,25 @@ bool f8_rows_map(CUtensorMap* map, const void* q, long pitch, long rows, int col
   return f8_encode(map, q, 2, dims, strides, nt);
 }
 
+// Raises a kernel's shared-memory limit, once per kernel and device.
+cudaError_t f8_allow_smem(const void* kern, size_t bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kern, dev})) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.insert({kern, dev});
+  return e;
+}
+
 template <int NT, int MATS, int MODE>
 cudaError_t launch_f8_gemm(const F8Maps& maps, const F8Pass& p, long tiles, cudaStream_t s) {
   auto kern = f8_gemm_kernel<NT, MATS, MODE>;
   constexpr size_t smem = F8Cfg<NT, MATS>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)std::min<long>(tiles, sm_count());
   return launch_pdl(kern, dim3(grid), dim3(kF8Threads), smem, s, maps, p);
@@ -662,23 +796,29 @@ int f8_blocks(long n) { return (int)((n + kF8Block - 1) / kF8Block); }
 
 template <typename T>
 cudaError_t quant_t(const T* x, long ldx, int tokens, int cols, uint8_t* q, long q_pitch,
-                    float* scales, long s_pitch, const int* rows, int k, cudaStream_t st) {
+                    float* scales, long s_pitch, const F8Rows& rows, cudaStream_t st) {
   const int vec = ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
-  const long warps = (rows ? (long)tokens : s_pitch) * f8_blocks(cols);
-  const unsigned grid = (unsigned)std::min<long>((warps + 7) / 8, (long)sm_count() * 16);
-  return launch_pdl(f8_quant_kernel<T>, dim3(grid), dim3(256), 0, st, x, ldx, tokens, cols, q,
-                    q_pitch, scales, s_pitch, rows, k, vec);
+  const long per = (f8_blocks(cols) + kQuantBlocks - 1) / kQuantBlocks;
+  const long ctas = ((rows.sel ? (long)tokens : s_pitch) * per + 7) / 8;
+  if (ctas > 0x0fffffffL) return cudaErrorInvalidValue;
+  auto kern = rows.sel ? f8_quant_kernel<T, true> : f8_quant_kernel<T, false>;
+  return launch_pdl(kern, dim3((unsigned)ctas), dim3(256), 0, st, x, ldx, tokens, cols, q,
+                    (int)q_pitch, scales, (int)s_pitch, rows, vec);
+}
+
+cudaError_t quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
+                  long q_pitch, float* scales, long s_pitch, const F8Rows& rows, cudaStream_t st) {
+  return bf16 ? quant_t(static_cast<const __nv_bfloat16*>(x), ldx, tokens, cols, q, q_pitch,
+                        scales, s_pitch, rows, st)
+              : quant_t(static_cast<const float*>(x), ldx, tokens, cols, q, q_pitch, scales,
+                        s_pitch, rows, st);
 }
 
 }  // namespace
 
 cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
-                            long q_pitch, float* scales, long s_pitch, const int* rows, int k,
-                            cudaStream_t st) {
-  return bf16 ? quant_t(static_cast<const __nv_bfloat16*>(x), ldx, tokens, cols, q, q_pitch,
-                        scales, s_pitch, rows, k, st)
-              : quant_t(static_cast<const float*>(x), ldx, tokens, cols, q, q_pitch, scales,
-                        s_pitch, rows, k, st);
+                            float* scales, cudaStream_t st) {
+  return quant(bf16, x, ldx, tokens, cols, q, f8_pad16(cols), scales, f8_pad4(tokens), F8Rows{}, st);
 }
 
 cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaStream_t st) {
@@ -724,7 +864,8 @@ F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k) {
     return at;
   };
   L.hp = (long)f8_blocks(m.up.rows) * kF8Block;
-  L.row_of = take((size_t)n * 4);
+  L.pos = take((size_t)n * 4);
+  L.row_start = take((size_t)m.up.experts * 4);
   L.entry = take((size_t)L.rows * 4);
   L.tiles = take((size_t)L.max_chunks * 16);
   L.nchunks = take(4);
@@ -743,7 +884,8 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
                           void* work, int* status, cudaStream_t st) {
   const F8MoeLayout L = f8_moe_layout(m, tokens, k);
   uint8_t* base = static_cast<uint8_t*>(work);
-  int* row_of = reinterpret_cast<int*>(base + L.row_of);
+  int* pos = reinterpret_cast<int*>(base + L.pos);
+  int* row_start = reinterpret_cast<int*>(base + L.row_start);
   int* entry = reinterpret_cast<int*>(base + L.entry);
   int4* tiles = reinterpret_cast<int4*>(base + L.tiles);
   int* nchunks = reinterpret_cast<int*>(base + L.nchunks);
@@ -753,10 +895,11 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   const int nt = f8_chunk((3 * n / std::min<long>(n, m.up.experts) + 1) / 2);
   const long chunks = n / nt + std::min<long>(n, m.up.experts);
   cudaError_t e = launch_pdl(f8_plan_kernel, dim3(1), dim3(1024), 0, st, sel, (int)n, m.up.experts,
-                             nt, row_of, entry, tiles, nchunks);
+                             nt, pos, row_start, tiles, nchunks);
   if (e != cudaSuccess) return e;
-  e = launch_f8_quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
-                      reinterpret_cast<float*>(base + L.xs), L.rows, row_of, k, st);
+  const F8Rows rows{sel, pos, row_start, entry, k, m.up.experts};
+  e = quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
+            reinterpret_cast<float*>(base + L.xs), L.rows, rows, st);
   if (e != cudaSuccess) return e;
   F8Maps maps;
   F8Pass p{};
@@ -801,7 +944,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   if (e != cudaSuccess) return e;
   const unsigned gy = (unsigned)std::max(1, std::min((m.down.rows + 1023) / 1024, 64));
   return launch_pdl(f8_combine_kernel, dim3((unsigned)tokens, gy), dim3(256), 0, st, partial,
-                    L.ldp, row_of, weights, k, m.down.rows, out, ldo, (int)out_bf16);
+                    L.ldp, sel, m.up.experts, weights, k, m.down.rows, out, ldo, (int)out_bf16);
 }
 
 }  // namespace lb

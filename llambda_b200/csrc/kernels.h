@@ -316,7 +316,7 @@ struct F8Moe {
 // Workspace of one call of the routed experts.
 struct F8MoeLayout {
   long rows, max_chunks, hp, ldp;
-  size_t row_of, entry, tiles, nchunks, xq, xs, hq, hs, partial, bytes;
+  size_t pos, row_start, entry, tiles, nchunks, xq, xs, hq, hs, partial, bytes;
 };
 
 inline long f8_pad16(long n) { return (n + 15) & ~15L; }
@@ -326,12 +326,9 @@ cudaError_t f8_prepare(F8Matrix* w);
 // Counts the scales that are not finite into *bad (device memory).
 cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaStream_t st);
 // Rows of x (fp32 or bf16, row stride ldx) to e4m3 with one scale per 128
-// columns: q rows of q_pitch bytes, scales [ceil(cols / 128)][s_pitch].  With
-// `rows`, token t goes to the grouped rows rows[t * k + j] that are not
-// negative; without, to row t.
+// columns: q rows of f8_pad16(cols) bytes, scales [ceil(cols / 128)][f8_pad4(tokens)].
 cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
-                            long q_pitch, float* scales, long s_pitch, const int* rows, int k,
-                            cudaStream_t st);
+                            float* scales, cudaStream_t st);
 // out[t][n] = w . x for quantised rows (pitch f8_pad16(cols), scales' pitch
 // f8_pad4(tokens)).
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,

@@ -57,131 +57,172 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
   return (unsigned long long)hi << 32 | lo;
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
-__device__ __forceinline__ float warp_max_value(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
-}
-
 // The score of a logit; m is the largest logit and z the sum of exp(l - m)
 // (softmax).  A row of -inf only scores 0.
-template <typename F>
-__device__ __forceinline__ F score(const RouteParams& r, float l, float m, F z) {
-  if (l == -INFINITY) return F(0);
-  return r.softmax ? exp_of((F)l - (F)m) / z : F(1) / (F(1) + exp_of(-(F)l));
+__device__ __forceinline__ float score(const RouteParams& r, float l, float m, float z) {
+  if (l == -INFINITY) return 0.0f;
+  return r.softmax ? expf(l - m) / z : 1.0f / (1.0f + expf(-l));
 }
 
-// What the choice goes by.
-template <typename F>
-__device__ __forceinline__ F choice(const RouteParams& r, bool by_logit, const float* bias, float l,
-                                    float m, F z, int e) {
-  if (by_logit || l == -INFINITY) return (F)l;
-  const F s = score<F>(r, l, m, z);
-  return bias ? s + (F)__ldg(bias + e) : s;
+// What the choice goes by, in fp32 (fast exp and division, errors within
+// choice_error) and in fp64.
+__device__ __forceinline__ float choice(const RouteParams& r, const float* bias, float l, float m,
+                                        float z, int e) {
+  if (l == -INFINITY) return l;
+  const float s =
+      r.softmax ? __fdividef(__expf(l - m), z) : __fdividef(1.0f, 1.0f + __expf(-l));
+  return bias ? s + __ldg(bias + e) : s;
+}
+__device__ __forceinline__ double choice(const RouteParams& r, const float* bias, float l, float m,
+                                         double z, int e) {
+  if (l == -INFINITY) return (double)l;
+  const double s = r.softmax ? exp((double)l - (double)m) / z : 1.0 / (1.0 + exp(-(double)l));
+  return bias ? s + (double)__ldg(bias + e) : s;
 }
 
-// Bound on twice the error of an fp32 choice: the score's (expf, the division
-// and, for softmax, the sum of exponentials: 4e-6 of the largest score smax in
-// all) and the rounding of the sum with the bias.
-__device__ __forceinline__ float choice_error(float c, float smax) {
-  return 8e-6f * smax + 2.5e-7f * fabsf(c);
+// Bound on the error of the difference of two fp32 choices.  Sigmoid: __expf
+// is off by (2 + 1.173 |l|) steps at most, which moves s by at most 0.63 steps
+// of 2^-23, the sum by half a step, __fdividef by two.  Softmax, relative to
+// the largest score smax = 1 / z: the exponentials and the division 5e-7 each,
+// z (its exponentials and 37 additions) 4e-6.  Then the rounding of the sums
+// with the bias.
+__device__ __forceinline__ float choice_error(const RouteParams& r, float c, float smax) {
+  return (r.softmax ? 8e-6f * smax : 1e-6f) + 2.5e-7f * fabsf(c);
 }
 
-// The logit of expert e (the same on every lane), from the lane that holds it.
-template <int R>
-__device__ __forceinline__ float expert_logit(const float (&l)[R], int e) {
-  float v = l[0];
+// A lane's two largest keys of those whose bit in `out` is clear, with their
+// places; equal keys in order of place.
+template <int R, typename K>
+__device__ __forceinline__ void two_largest(const K (&key)[R], uint32_t out, K& a, int& ai, K& b,
+                                            int& bi) {
+  a = b = 0;
+  ai = bi = 0;
 #pragma unroll
-  for (int j = 1; j < R; ++j)
-    if (j == e >> 5) v = l[j];
-  return __shfl_sync(kFull, v, e & 31);
+  for (int j = 0; j < R; ++j) {
+    const K v = out >> j & 1u ? K(0) : key[j];
+    if (v > a) {
+      b = a, bi = ai;
+      a = v, ai = j;
+    } else if (v > b) {
+      b = v, bi = j;
+    }
+  }
 }
 
-// The choice of one token by one warp: lane L holds experts L, L + 32, ....
-// Rank i's expert goes to lane i.  F = float: returns false when some deciding
-// comparison was too close (by_logit: the compared values are exact).
+// The choice of one token by one warp: lane L holds experts L * R .. L * R +
+// R - 1, so equal keys go to the lowest lane that has one, and to its lowest j.
+// Rank i's expert goes to lane i (and that of rank top_k, if there is such a
+// lane, to lane top_k).  F = float: returns false when the comparison of the
+// groups was too close, and sets tied on lane i when that of ranks i and i + 1
+// was (by_logit: the compared values are exact).
+//
+// Each round takes the warp's largest key, one reduction over the lanes' own
+// largest.  A lane keeps its two largest and looks for more only when both are
+// gone.  At 8191 tokens, 256 experts in 8 groups, top 8, the search through all
+// of a lane's keys in every round took 27 us.
 template <int R, typename F>
 __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R], const float* bias,
-                                       bool by_logit, float m, F z, int lane, int& sel) {
+                                       bool by_logit, float m, F z, int lane, int& sel,
+                                       bool& tied) {
   using K = decltype(order_key(F(0)));
   const bool check = sizeof(F) == 4 && !by_logit;
+  const float smax = r.softmax ? 1.0f / (float)z : 1.0f;
   K key[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int e = j * 32 + lane;
-    key[j] = e < r.experts ? order_key(choice<F>(r, by_logit, bias, l[j], m, z, e)) : K(0);
+    const int e = lane * R + j;
+    key[j] = e >= r.experts ? K(0)
+             : by_logit     ? order_key((F)l[j])
+                            : order_key(choice(r, bias, l[j], m, z, e));
   }
   bool sure = true;
-  const float smax = r.softmax ? 1.0f / (float)z : 1.0f;
+  uint32_t out = 0;  // this lane's experts that are out
   if (r.top_groups < r.groups) {
-    const int size = r.experts / r.groups;
-    K gkey = 0;  // lane g: group g's score
-    for (int g = 0; g < r.groups; ++g) {
-      const int lo = g * size, hi = lo + size;
-      K a = 0, b = 0;  // this lane's two largest
+    const int size = r.experts / r.groups, span = size / R;
+    K g1 = 0, g2 = 0;  // lane g: group g's two largest
+    if (size % R == 0 && (span & (span - 1)) == 0) {  // whole lanes, a power of two of them
+      K a = 0, b = 0;
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const int e = j * 32 + lane;
-        const K v = e >= lo && e < hi ? key[j] : K(0);
-        b = max(b, min(a, v));
-        a = max(a, v);
+        b = max(b, min(a, key[j]));
+        a = max(a, key[j]);
       }
-      K best = warp_max(a);
-      if (r.group_top == 2) {
-        const unsigned owner = __ballot_sync(kFull, a == best);
-        const K second = warp_max(lane == __ffs(owner) - 1 ? b : a);
-        best = order_key(key_value(best) + key_value(second));
+      for (int o = 1; o < span; o <<= 1) {
+        const K a2 = __shfl_xor_sync(kFull, a, o), b2 = __shfl_xor_sync(kFull, b, o);
+        b = max(min(a, a2), max(b, b2));
+        a = max(a, a2);
       }
-      if (lane == g) gkey = best;
+      g1 = __shfl_sync(kFull, a, lane * span & 31);
+      g2 = __shfl_sync(kFull, b, lane * span & 31);
+    } else {
+      for (int g = 0; g < r.groups; ++g) {
+        const int lo = g * size, hi = lo + size;
+        K a = 0, b = 0;  // this lane's two largest
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          const int e = lane * R + j;
+          const K v = e >= lo && e < hi ? key[j] : K(0);
+          b = max(b, min(a, v));
+          a = max(a, v);
+        }
+        const K first = warp_max(a);
+        const int owner = __ffs(__ballot_sync(kFull, a == first)) - 1;
+        const K second = warp_max(lane == owner ? b : a);
+        if (lane == g) g1 = first, g2 = second;
+      }
     }
-    unsigned kept = 0;
-    K last = 0;
-    for (int i = 0; i < r.top_groups; ++i) {
-      last = warp_max(gkey);
-      const int g = __ffs(__ballot_sync(kFull, gkey == last)) - 1;
-      kept |= 1u << g;
-      if (lane == g) gkey = 0;
+    K gkey = r.group_top == 2 ? order_key(key_value(g1) + key_value(g2)) : g1;
+    if (lane >= r.groups) gkey = 0;
+    int rank = 0;  // groups before this lane's: larger ones, and equal ones of lower index
+    for (int g = 0; g < r.groups; ++g) {
+      const K v = __shfl_sync(kFull, gkey, g);
+      rank += v > gkey || (v == gkey && g < lane);
     }
+    const bool is_group = lane < r.groups;
+    const unsigned kept = __ballot_sync(kFull, is_group && rank < r.top_groups);
     if (check) {
-      // the best group left out against the worst one kept (a NaN compares false)
-      const F in = key_value(last), out = key_value(warp_max(gkey));
-      if (in - out <= F(2) * (F)choice_error((float)in, smax)) sure = false;
+      // the best group left out against the worst one kept, sums of two (a NaN compares false)
+      const int wi = __ffs(__ballot_sync(kFull, is_group && rank == r.top_groups - 1)) - 1;
+      const int bo = __ffs(__ballot_sync(kFull, is_group && rank == r.top_groups)) - 1;
+      const F in = key_value((K)__shfl_sync(kFull, gkey, wi));
+      const F out = key_value((K)__shfl_sync(kFull, gkey, bo));
+      if (in - out <= F(2) * (F)choice_error(r, (float)in, smax)) sure = false;
     }
+    int g = lane * R / size, left = (g + 1) * size - lane * R;  // experts left in group g
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const int e = j * 32 + lane;
-      if (e < r.experts && !(kept >> (e / size) & 1u)) key[j] = 0;
+      if (!(kept >> (g & 31) & 1u)) out |= 1u << j;
+      if (--left == 0) ++g, left = size;
     }
   }
-  K prev = 0;
-  int prev_e = 0;
+  K a, b, mine = 0, next = 0;  // mine: rank `lane`'s key; next: that of rank top_k
+  int ai, bi;
+  two_largest<R>(key, out, a, ai, b, bi);
   for (int i = 0; i <= r.top_k; ++i) {
     if (i == r.top_k && !check) break;
-    K a = 0;
-    int at = 0;
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (key[j] > a) a = key[j], at = j;
     const K best = warp_max(a);
     if (best == 0) break;  // no expert left to compare with
-    const int e = __reduce_min_sync(kFull, a == best ? at * 32 + lane : 0x7fffffff);
-    if (i < r.top_k && lane == i) sel = e;
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (e == j * 32 + lane) key[j] = 0;
-    if (check && i > 0) {
-      const F c = key_value(prev), d = key_value(best);
-      // equal logits and biases are a true tie, which the index decides
-      if (c - d <= (F)choice_error((float)c, smax) &&
-          !(expert_logit(l, prev_e) == expert_logit(l, e) && bias &&
-            __ldg(bias + prev_e) == __ldg(bias + e)))
-        sure = false;
+    const int owner = __ffs(__ballot_sync(kFull, a == best)) - 1;
+    const int e = __shfl_sync(kFull, lane * R + ai, owner);
+    if (i == r.top_k) {
+      next = best;
+      if (lane == r.top_k) sel = e;  // compared with rank top_k - 1 below
+    } else if (lane == i) {
+      sel = e, mine = best;
     }
-    prev = best;
-    prev_e = e;
+    bool dry = false;
+    if (lane == owner) {
+      out |= 1u << ai;
+      a = b, ai = bi, b = 0;
+      dry = a == 0;
+    }
+    if (R > 2 && __any_sync(kFull, dry)) two_largest<R>(key, out, a, ai, b, bi);
+  }
+  if (check) {
+    K after = __shfl_down_sync(kFull, mine, 1);
+    if (lane == r.top_k - 1) after = next;
+    const F c = key_value(mine), d = key_value(after);
+    tied = lane < r.top_k && after != 0 && c - d <= (F)choice_error(r, (float)c, smax);
   }
   return sure;
 }
@@ -191,11 +232,45 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
   return __bfloat162float(p[i]);
 }
 
+// R consecutive logits, in the widest loads their size allows when the rows are aligned.
+template <int R>
+__device__ __forceinline__ void load_logits(const float* p, float (&l)[R]) {
+  if constexpr (R >= 4) {
+#pragma unroll
+    for (int j = 0; j < R; j += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p + j));
+      l[j] = v.x, l[j + 1] = v.y, l[j + 2] = v.z, l[j + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < R; ++j) l[j] = __ldg(p + j);
+  }
+}
+template <int R>
+__device__ __forceinline__ void load_logits(const __nv_bfloat16* p, float (&l)[R]) {
+  if constexpr (R >= 8) {
+#pragma unroll
+    for (int j = 0; j < R; j += 8) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + j));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        l[j + 2 * i] = __uint_as_float(w[i] << 16);
+        l[j + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < R; ++j) l[j] = __bfloat162float(p[j]);
+  }
+}
+
+// One warp per token.  vec: every row starts on 16 bytes.
 template <typename T, int R>
 __global__ void __launch_bounds__(kRouteWarps * 32)
     route_kernel(const RouteParams r, const T* __restrict__ logits, long ld,
                  const float* __restrict__ bias, int tokens, int* __restrict__ selected,
-                 float* __restrict__ weights) {
+                 float* __restrict__ weights, int vec) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
@@ -203,46 +278,60 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
   if (t >= tokens) return;
   const T* row = logits + t * ld;
   float l[R];
-  bool nan = false;
+  if (vec && lane * R + R <= r.experts) {
+    load_logits<R>(row + lane * R, l);
+  } else {
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int e = j * 32 + lane;
-    l[j] = e < r.experts ? logit_at(row, e) : -INFINITY;
-    nan |= isnan(l[j]);
+    for (int j = 0; j < R; ++j)
+      l[j] = lane * R + j < r.experts ? logit_at(row, lane * R + j) : -INFINITY;
   }
+  // softmax: a NaN or +inf logit makes every score of the row NaN
+  bool bad = false;
+  if (r.softmax) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) bad |= !(l[j] < INFINITY);
+    bad = __any_sync(kFull, bad);
+  }
+  const bool by_logit = !bias && (r.top_groups == r.groups || r.group_top == 1) && !bad;
   float m = 0.0f, z = 1.0f;
   if (r.softmax) {
     m = l[0];
 #pragma unroll
     for (int j = 1; j < R; ++j) m = fmaxf(m, l[j]);
-    m = warp_max_value(m);
-    z = 0.0f;
+    m = key_value(warp_max(order_key(m)));
+    if (!by_logit || !r.renormalise) {  // else z divides out of the weights
+      z = 0.0f;
 #pragma unroll
-    for (int j = 0; j < R; ++j) z += l[j] == -INFINITY ? 0.0f : expf(l[j] - m);
-    z = warp_sum(z);
-    nan = isnan(z);  // a NaN or +inf logit makes every score NaN
+      for (int j = 0; j < R; ++j) z += l[j] == -INFINITY ? 0.0f : expf(l[j] - m);
+      z = bad ? __int_as_float(0x7fc00000) : warp_sum(z);
+    }
   }
-  const bool scores_order =
-      !bias && (r.top_groups == r.groups || r.group_top == 1) && !(r.softmax && nan);
   int sel = 0;
-  if (!choose<R, float>(r, l, bias, scores_order, m, z, lane, sel)) {
+  bool tied = false;
+  bool sure = choose<R, float>(r, l, bias, by_logit, m, z, lane, sel, tied);
+  if (__any_sync(kFull, tied)) {
+    // equal logits and biases are a true tie, which the index has decided
+    const float lv = logit_at(row, sel), bv = bias ? __ldg(bias + sel) : 0.0f;
+    const float ln = __shfl_down_sync(kFull, lv, 1), bn = __shfl_down_sync(kFull, bv, 1);
+    sure = sure && !__any_sync(kFull, tied && (lane == 31 || lv != ln || bv != bn));
+  }
+  if (!sure) {
     double zd = 1.0;
     if (r.softmax) {
       zd = 0.0;
 #pragma unroll 1
-      for (int j = 0; j < R; ++j) {
-        const int e = j * 32 + lane;
-        const float v = e < r.experts ? logit_at(row, e) : -INFINITY;
+      for (int e = lane; e < r.experts; e += 32) {
+        const float v = logit_at(row, e);
         zd += v == -INFINITY ? 0.0 : exp((double)v - (double)m);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) zd += __shfl_xor_sync(kFull, zd, o);
     }
-    choose<R, double>(r, l, bias, false, m, zd, lane, sel);
+    choose<R, double>(r, l, bias, false, m, zd, lane, sel, tied);
   }
   // lane i: the weight of rank i
   float s = 0.0f;
-  if (lane < r.top_k) s = score<float>(r, logit_at(row, sel), m, z);
+  if (lane < r.top_k) s = score(r, logit_at(row, sel), m, z);
   float w = s;
   if (r.renormalise) {
     const float sum = warp_sum(s);
@@ -259,8 +348,9 @@ cudaError_t route_t(const RouteParams& r, const T* logits, long ld, const float*
                     int* selected, float* weights, cudaStream_t st) {
   const dim3 grid((unsigned)((tokens + kRouteWarps - 1) / kRouteWarps)), block(kRouteWarps * 32);
   const int per = (r.experts + 31) / 32;
+  const int vec = ld * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0;
   auto go = [&](auto kern) {
-    return launch_pdl(kern, grid, block, 0, st, r, logits, ld, bias, tokens, selected, weights);
+    return launch_pdl(kern, grid, block, 0, st, r, logits, ld, bias, tokens, selected, weights, vec);
   };
   if (per <= 1) return go(route_kernel<T, 1>);
   if (per <= 2) return go(route_kernel<T, 2>);

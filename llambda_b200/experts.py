@@ -16,8 +16,8 @@ differentiated: a tensor that requires grad is refused while autograd records.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -26,9 +26,28 @@ from . import _native as N
 BLOCK = 128  # columns (and weight rows) per scale
 
 
+# A one-token call is a few microseconds of GPU time, so what a call does on the
+# host is kept short: torch is looked up once, the entry points are bound once,
+# and the current stream is read as a raw handle where torch offers that.
+_t = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _t
+    if _t is None:
+        import torch
+        _t = torch
+    return _t
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(N.lib(), name)
+
+
+def _call(name: str, *args) -> None:
+    if _entry(name)(*args) != 0:
+        raise N.LlambdaCudaError(N.last_error() or f"{name} failed")
 
 
 def _blocks(n: int) -> int:
@@ -41,15 +60,16 @@ def _pad(n: int, m: int) -> int:
 
 def _device_tensor(t, name: str, dtypes, ndim: int, shape=None, device=None, contiguous=False):
     """Checks a CUDA tensor: type, rank, shape (None: any), unit stride along the last axis."""
-    torch = _torch()
+    torch = _t or _torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, "
                          f"got {str(t.dtype)[6:]}")
-    if t.dim() != ndim or (shape is not None and
-                           any(w is not None and w != g for w, g in zip(shape, t.shape))):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+    got = t.shape
+    if len(got) != ndim or (shape is not None and
+                            any(w is not None and w != g for w, g in zip(shape, got))):
+        raise ValueError(f"{name} has shape {tuple(got)}, expected "
                          f"{tuple('any' if s is None else s for s in shape or (None,) * ndim)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires grad; these operators have no backward pass")
@@ -58,30 +78,53 @@ def _device_tensor(t, name: str, dtypes, ndim: int, shape=None, device=None, con
     if contiguous:
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-    elif t.shape[-1] > 1 and t.stride(-1) != 1:
+    elif got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
-    if 0 in t.shape:
+    if 0 in got:
         raise ValueError(f"{name} is empty (a positive token count is required)")
     return t
 
 
-def _tag(dtype) -> int:
-    return N.TYPE_BF16 if dtype == _torch().bfloat16 else N.TYPE_F32
-
-
+@functools.lru_cache(maxsize=None)
 def _floats():
     torch = _torch()
     return torch.float32, torch.bfloat16
 
 
-def _on(stream, device):
-    """(context that makes `stream` current, its raw handle); None: the current stream."""
+def _tag(dtype) -> int:
+    return N.TYPE_F32 if dtype is _floats()[0] else N.TYPE_BF16
+
+
+@functools.lru_cache(maxsize=None)
+def _raw_stream():
     torch = _torch()
-    if stream is None:
-        return contextlib.nullcontext(), torch.cuda.current_stream(device).cuda_stream
-    if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(int(stream), device=device)
-    return torch.cuda.stream(stream), stream.cuda_stream
+    return getattr(torch._C, "_cuda_getCurrentRawStream",
+                   lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _Stream:
+    """The raw handle of a call's stream; as a context, makes it current, so
+    that what the call allocates belongs to it."""
+
+    def __init__(self, stream, device):
+        if stream is None:
+            self._ctx, self.raw = None, _raw_stream()(device.index)
+        else:
+            torch = _torch()
+            if not hasattr(stream, "cuda_stream"):
+                stream = torch.cuda.ExternalStream(int(stream), device=device)
+            if stream.device != device:
+                raise ValueError(f"the stream is on {stream.device}, not {device}")
+            self._ctx, self.raw = torch.cuda.stream(stream), stream.cuda_stream
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
 
 
 def _row_stride(t) -> int:
@@ -89,9 +132,10 @@ def _row_stride(t) -> int:
 
 
 def _out(out, rows: int, cols: int, dtype, device, name="out"):
-    torch = _torch()
     if out is None:
-        return torch.empty(rows, cols, dtype=dtype, device=device)
+        if dtype not in _floats():
+            raise ValueError(f"{name} must be float32 or bfloat16, got {str(dtype)[6:]}")
+        return _torch().empty(rows, cols, dtype=dtype, device=device)
     return _device_tensor(out, name, _floats(), 2, (rows, cols), device)
 
 
@@ -133,14 +177,13 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
     desc = _route_desc(E, top_k, score, groups, top_groups, group_top, renormalise, weight_scale)
     if not 1 <= top_k <= E:
         raise ValueError(f"top_k must be in 1..{E}, got {top_k}")
-    ctx, raw = _on(stream, dev)
-    with ctx:
+    with _Stream(stream, dev) as st:
         selected = torch.empty(T, top_k, dtype=torch.int32, device=dev)
         weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
-    N._check(N.lib().llambda_cuda_route_device(
-        C.byref(desc), _tag(logits.dtype), logits.data_ptr(), _row_stride(logits),
+    _call(
+        "llambda_cuda_route_device", C.byref(desc), _tag(logits.dtype), logits.data_ptr(), _row_stride(logits),
         bias.data_ptr() if bias is not None else None, T, selected.data_ptr(), weights.data_ptr(),
-        raw))
+        st.raw)
     return selected, weights
 
 
@@ -157,9 +200,9 @@ def _route_host(logits, bias, desc):
     T = logits.shape[0]
     selected = np.empty((T, desc.top_k), np.int32)
     weights = np.empty((T, desc.top_k), np.float32)
-    N._check(N.lib().llambda_cuda_route(
+    _call("llambda_cuda_route",
         C.byref(desc), logits.ctypes.data, bias.ctypes.data if bias is not None else None, T,
-        selected.ctypes.data, weights.ctypes.data))
+        selected.ctypes.data, weights.ctypes.data)
     return selected, weights
 
 
@@ -175,12 +218,11 @@ def fp8_quantize(x, *, stream=None):
     torch = _torch()
     _device_tensor(x, "x", _floats(), 2)
     T, cols = x.shape
-    ctx, raw = _on(stream, x.device)
-    with ctx:
+    with _Stream(stream, x.device) as st:
         q = torch.empty(T, _pad(cols, 16), dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty(_blocks(cols), _pad(T, 4), dtype=torch.float32, device=x.device)
-    N._check(N.lib().llambda_cuda_fp8_quantize_device(
-        _tag(x.dtype), x.data_ptr(), _row_stride(x), T, cols, q.data_ptr(), scales.data_ptr(), raw))
+    _call("llambda_cuda_fp8_quantize_device",
+        _tag(x.dtype), x.data_ptr(), _row_stride(x), T, cols, q.data_ptr(), scales.data_ptr(), st.raw)
     return q, scales
 
 
@@ -257,7 +299,7 @@ class Fp8ProjectionSession(_Fp8Session):
     def _create(cls, w, s, data, scales, on_device, device, keep):
         h = C.c_void_p()
         t = _fp8_tensor(w.shape, data, scales)
-        N._check(N.lib().llambda_cuda_fp8_session_create(C.byref(t), on_device, C.byref(h)))
+        _call("llambda_cuda_fp8_session_create", C.byref(t), on_device, C.byref(h))
         return cls(h, w.shape[0], w.shape[1], device, keep)
 
     @classmethod
@@ -273,6 +315,8 @@ class Fp8ProjectionSession(_Fp8Session):
         float8_e4m3fn or uint8, cols a multiple of 16."""
         w, s = _device_weights((weights, scales), "projection", 2)
         with _torch().cuda.device(w.device):
+            # weights that a side stream is still writing are checked when written
+            _torch().cuda.current_stream().synchronize()
             return cls._create(w, s, w.data_ptr(), s.data_ptr(), 1, w.device, (w, s))
 
     def run(self, x: np.ndarray) -> np.ndarray:
@@ -283,8 +327,8 @@ class Fp8ProjectionSession(_Fp8Session):
         if x.ndim != 2 or x.shape[1] != self.cols or not x.size:
             raise ValueError(f"x must be [tokens][{self.cols}]")
         out = np.empty((x.shape[0], self.rows), np.float32)
-        N._check(N.lib().llambda_cuda_fp8_session_run(self._handle(), x.ctypes.data, x.shape[0],
-                                                      out.ctypes.data))
+        _call("llambda_cuda_fp8_session_run", self._handle(), x.ctypes.data, x.shape[0],
+                                                      out.ctypes.data)
         return out[0] if one else out
 
     def run_device(self, x, out=None, *, out_dtype=None, stream=None):
@@ -294,14 +338,13 @@ class Fp8ProjectionSession(_Fp8Session):
         h = self._handle()
         _device_tensor(x, "x", _floats(), 2, (None, self.cols), self.device)
         T = x.shape[0]
-        ctx, raw = _on(stream, x.device)
-        with ctx:
+        with _Stream(stream, x.device) as st:
             out = _out(out, T, self.rows, out_dtype or x.dtype, x.device)
             nbytes = N.lib().llambda_cuda_fp8_session_workspace(h, T)
             work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N._check(N.lib().llambda_cuda_fp8_session_run_device(
+        _call("llambda_cuda_fp8_session_run_device",
             h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, _tag(out.dtype), out.data_ptr(),
-            _row_stride(out), work.data_ptr(), nbytes, raw))
+            _row_stride(out), work.data_ptr(), nbytes, st.raw)
         return out
 
     def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):
@@ -313,12 +356,11 @@ class Fp8ProjectionSession(_Fp8Session):
                        self.device, contiguous=True)
         _device_tensor(scales, "scales", (torch.float32,), 2, (_blocks(self.cols), _pad(tokens, 4)),
                        q.device, contiguous=True)
-        ctx, raw = _on(stream, q.device)
-        with ctx:
+        with _Stream(stream, q.device) as st:
             out = _out(out, tokens, self.rows, out_dtype or torch.float32, q.device)
-        N._check(N.lib().llambda_cuda_fp8_session_run_quantized(
+        _call("llambda_cuda_fp8_session_run_quantized",
             h, q.data_ptr(), scales.data_ptr(), tokens, _tag(out.dtype), out.data_ptr(),
-            _row_stride(out), raw))
+            _row_stride(out), st.raw)
         return out
 
 
@@ -341,8 +383,8 @@ class Fp8MoeSession(_Fp8Session):
         ts = [_fp8_tensor(p[0].shape, ptr(p[0]), ptr(p[1])) if p is not None
               else N.Fp8Tensor(0, 0, 0, None, None) for p in (gate, up, down)]
         h = C.c_void_p()
-        N._check(N.lib().llambda_cuda_fp8_moe_session_create(
-            C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h)))
+        _call("llambda_cuda_fp8_moe_session_create",
+            C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h))
         E, _, H = up[0].shape
         return cls(h, E, H, down[0].shape[1], device, (up, down, gate) if on_device else None)
 
@@ -362,6 +404,7 @@ class Fp8MoeSession(_Fp8Session):
         down = _device_weights(down, "down", 3, dev)
         gate = _device_weights(gate, "gate", 3, dev) if gate is not None else None
         with _torch().cuda.device(dev):
+            _torch().cuda.current_stream().synchronize()
             return cls._create(up, down, gate, lambda t: t.data_ptr(), 1, dev)
 
     def run(self, x: np.ndarray, selected: np.ndarray, weights: np.ndarray) -> np.ndarray:
@@ -374,9 +417,9 @@ class Fp8MoeSession(_Fp8Session):
                 or weights.shape != selected.shape:
             raise ValueError("selected and weights must both be [tokens][k]")
         out = np.empty((x.shape[0], self.out_features), np.float32)
-        N._check(N.lib().llambda_cuda_fp8_moe_session_run(
+        _call("llambda_cuda_fp8_moe_session_run",
             self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
-            weights.ctypes.data, out.ctypes.data))
+            weights.ctypes.data, out.ctypes.data)
         return out
 
     def run_device(self, x, selected, weights, out=None, *, out_dtype=None, stream=None):
@@ -391,13 +434,12 @@ class Fp8MoeSession(_Fp8Session):
         _device_tensor(selected, "selected", (torch.int32,), 2, (T, None), dev, contiguous=True)
         k = selected.shape[1]
         _device_tensor(weights, "weights", (torch.float32,), 2, (T, k), dev, contiguous=True)
-        ctx, raw = _on(stream, dev)
-        with ctx:
+        with _Stream(stream, dev) as st:
             out = _out(out, T, self.out_features, out_dtype or x.dtype, dev)
             nbytes = N.lib().llambda_cuda_fp8_moe_session_workspace(h, T, k)
             work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        N._check(N.lib().llambda_cuda_fp8_moe_session_run_device(
+        _call("llambda_cuda_fp8_moe_session_run_device",
             h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, k, selected.data_ptr(),
             weights.data_ptr(), _tag(out.dtype), out.data_ptr(), _row_stride(out), work.data_ptr(),
-            nbytes, raw))
+            nbytes, st.raw)
         return out
