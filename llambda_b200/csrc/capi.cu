@@ -1637,7 +1637,7 @@ static void f8_project_call(llambda_cuda_fp8_session* s, bool x_bf16, const void
   uint8_t* q = static_cast<uint8_t*>(work);
   float* sc = reinterpret_cast<float*>(q + at);
   cuda_check(lb::launch_f8_quant(x_bf16, x, ldx, T, s->w.cols, q, sc, st), "quantise launch");
-  cuda_check(lb::launch_f8_project(s->w, q, sc, T, out_bf16, out, ldo, s->status, st),
+  cuda_check(lb::launch_f8_project(s->w, q, sc, T, out_bf16, out, ldo, true, s->status, st),
              "product launch");
 }
 
@@ -1701,7 +1701,7 @@ int llambda_cuda_fp8_session_run_quantized(llambda_cuda_fp8_session* s, const vo
     require_align(device_scales, 16, "scales");
     require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
     cuda_check(lb::launch_f8_project(s->w, static_cast<const uint8_t*>(device_q), device_scales, T,
-                                     is_bf16(out_type, "output"), device_out, ldo, s->status,
+                                     is_bf16(out_type, "output"), device_out, ldo, false, s->status,
                                      static_cast<cudaStream_t>(cuda_stream)),
                "product launch");
     return 0;

@@ -30,9 +30,10 @@ namespace {
 constexpr int kF8M = 128;         // weight rows per tile (the MMA's M)
 constexpr int kF8Block = 128;     // columns per scale, bytes per staged row
 constexpr int kF8EpiWarps = 8;    // two warpgroups, half of the tokens each
-constexpr int kF8Threads = (4 + kF8EpiWarps) * 32;
+constexpr int kF8Threads = (kF8EpiWarps + 3) * 32;
 constexpr int kF8Scales = 8;      // ring of staged activation scales
 constexpr int kF8MaxBuf = 4;      // ring of accumulators in tensor memory
+constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K
 
 enum F8Mode {
   kF8Out,      // y to out (fp32 or bf16)
@@ -226,6 +227,8 @@ struct F8Pass {
   float* partial;                // kF8Partial: rows of partial by entry
   long ldp;
   const int* entry;
+  int split;                     // CTAs of a cluster share a tile's K (1: no cluster)
+  int early;                     // the weights and tiles are not the previous kernel's output
   int* status;
 };
 
@@ -237,13 +240,18 @@ struct F8Sync {
   int abort;
 };
 
+// Small tiles are bound by the weights' bytes: two CTAs a multiprocessor, so
+// that one loads while the other finishes a tile.  Large ones take the whole
+// shared memory for one.
 template <int NT, int MATS>
 struct F8Cfg {
+  static constexpr int kCtas = NT <= 32 || (NT == 64 && MATS == 1) ? 2 : 1;
+  static constexpr uint32_t kBudget = (kCtas == 2 ? 104u : 200u) * 1024u;
   static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
   static constexpr uint32_t kStage = MATS * kA + NT * kF8Block;
-  static constexpr int kStages = (int)(200u * 1024u / kStage) > 12 ? 12 : (int)(200u * 1024u / kStage);
+  static constexpr int kStages = (int)(kBudget / kStage);
   static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
-  static constexpr int kBufs = 512 / kAcc > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc;
+  static constexpr int kBufs = 512 / kAcc / kCtas > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc / kCtas;
   static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kF8Scales * NT * 4 +
                                   2 * 4 * NT * 4 + sizeof(F8Sync);
@@ -344,15 +352,40 @@ __device__ __forceinline__ F8Tile f8_tile(const F8Pass& p, int tile) {
 
 __device__ __forceinline__ float silu(float g) { return __fdiv_rn(g, 1.0f + expf(-g)); }
 
-// One CTA per SM, persistent over tiles of 128 weight rows x NT rows of x (M is
-// the weights' side, so one token costs a tile of 16 columns, and an expert's
-// few tokens no more).  Warp 0 stages weights and activations by TMA, warp 2
-// the activations' scales, warp 1's first lane issues the MMAs of one block of
-// K into the next of kBufs accumulators, and eight warps add the accumulators,
-// scaled, into registers: lane r of the tensor memory is weight row r, so the
-// weight scale is one number per block and thread.
-template <int NT, int MATS, int MODE>
-__global__ void __launch_bounds__(kF8Threads, 1)
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The cluster address of the same shared-memory object in its CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_ld(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Persistent over tiles of 128 weight rows x NT rows of x (M is the weights'
+// side, so one token costs a tile of 16 columns, and an expert's few tokens no
+// more).  Warp 8 stages weights and activations by TMA, warp 10 the activations'
+// scales, warp 9's first lane issues the MMAs of one block of K into the next
+// of kBufs accumulators, and warps 0-7 add the accumulators, scaled, into
+// registers: lane r of the tensor memory is weight row r, so the weight scale
+// is one number per block and thread.
+//
+// SPLIT: few tiles.  The CTAs of a cluster take a part of the tile's K
+// each, then each adds the sums of its share of the columns from the others'
+// shared memory.
+template <int NT, int MATS, int MODE, bool SPLIT>
+__global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     f8_gemm_kernel(const __grid_constant__ F8Maps maps, const F8Pass p) {
   using C = F8Cfg<NT, MATS>;
   constexpr int NC = NT / 2;  // tokens per epilogue thread
@@ -380,33 +413,54 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     sy->abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(&sy->tmem, C::kCols);
+  if (warp == kF8EpiWarps + 1) tmem_alloc(&sy->tmem, C::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sy->tmem;
-  griddep_wait();
-  griddep_launch();
+  const bool early = p.early && warp == kF8EpiWarps;
+  if (!early) {
+    griddep_wait();
+    griddep_launch();
+  }
   const int ntiles = (p.tiles ? __ldcg(p.nchunks) : p.chunks) * p.rblocks;
+  const uint32_t rank = SPLIT ? cluster_rank() : 0;
+  const int split = SPLIT ? p.split : 1;
+  const int tile0 = (int)blockIdx.x / split, tstep = (int)gridDim.x / split;
+  const int kb0 = (int)rank * p.kblocks / split, kb1 = ((int)rank + 1) * p.kblocks / split;
+  bool synced = false;  // split: this warp has met the others of the cluster
 
-  if (warp == 0) {  // ------------------------------------- weights, activations
+  if (warp == kF8EpiWarps) {  // ------------------------------------- weights, activations
     if (lane == 0) {
       RingPos rp;
-      int q = 0;
+      int q = 0, ahead = 0;
       uint32_t last_phase[C::kStages] = {};
-      for (int tile = blockIdx.x; tile < ntiles && !*abort; tile += gridDim.x) {
+      auto load_weights = [&](int s, int kb, const F8Tile& t) {
+        uint8_t* st = stages + (size_t)s * C::kStage;
+        uint64_t* bar = &sy->full[s];
+        mbar_expect_tx(bar, C::kStage);
+        tma_load_3d(st, &maps.w0, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+        if (MATS == 2)
+          tma_load_3d(st + C::kA, &maps.w1, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+      };
+      if (early) {  // the first tile's weights while the previous kernel still runs
+        if (tile0 < ntiles) {
+          const F8Tile t = f8_tile<NT>(p, tile0);
+          for (; ahead < C::kStages && kb0 + ahead < kb1; ++ahead)
+            load_weights(ahead, kb0 + ahead, t);
+        }
+        griddep_wait();
+        griddep_launch();
+      }
+      for (int tile = tile0; tile < ntiles && !*abort; tile += tstep) {
         const F8Tile t = f8_tile<NT>(p, tile);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (q >= C::kStages &&
               !f8_wait(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort))
             break;
-          uint8_t* st = stages + (size_t)rp.s * C::kStage;
-          uint64_t* bar = &sy->full[rp.s];
-          mbar_expect_tx(bar, C::kStage);
-          tma_load_3d(st, &maps.w0, kb * kF8Block, t.rb * kF8M, t.expert, bar);
-          if (MATS == 2)
-            tma_load_3d(st + C::kA, &maps.w1, kb * kF8Block, t.rb * kF8M, t.expert, bar);
-          tma_load_2d(st + MATS * C::kA, &maps.x, kb * kF8Block, t.row0, bar);
+          if (q >= ahead) load_weights(rp.s, kb, t);
+          tma_load_2d(stages + (size_t)rp.s * C::kStage + MATS * C::kA, &maps.x, kb * kF8Block,
+                      t.row0, &sy->full[rp.s]);
           last_phase[rp.s] = rp.phase;
           ++q;
           rp.next(C::kStages);
@@ -416,17 +470,17 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       for (int s = 0; s < C::kStages && s < q; ++s) mbar_wait(&sy->full[s], last_phase[s], nullptr);
     }
     __syncwarp();
-  } else if (warp == 2) {  // -------------------------------------------- scales
+  } else if (warp == kF8EpiWarps + 2) {  // -------------------------------------------- scales
     if (lane == 0) {
       RingPos rp;
       int q = 0;
       uint32_t last_phase[kF8Scales] = {};
-      for (int tile = blockIdx.x; tile < ntiles && !*abort; tile += gridDim.x) {
+      for (int tile = tile0; tile < ntiles && !*abort; tile += tstep) {
         const F8Tile t = f8_tile<NT>(p, tile);
         // row0 and the pitch are multiples of 4; columns past the pitch keep
         // what an earlier tile left and belong to no valid row
         const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (q >= kF8Scales &&
               !f8_wait(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort))
             break;
@@ -441,15 +495,15 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       for (int s = 0; s < kF8Scales && s < q; ++s) mbar_wait(&sy->sfull[s], last_phase[s], nullptr);
     }
     __syncwarp();
-  } else if (warp == 1) {  // ----------------------------------------------- MMA
+  } else if (warp == kF8EpiWarps + 1) {  // ----------------------------------------------- MMA
     if (lane == 0) {
       RingPos rp, ap;
       int q = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+      for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
         const F8Tile t = f8_tile<NT>(p, tile);
         const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           ok = (q < C::kBufs ||
                 f8_wait(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
                f8_wait(&sy->full[rp.s], rp.phase, p.status, abort);
@@ -476,13 +530,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       mbar_wait(&sy->done, 0, nullptr);
     }
     __syncwarp();
-  } else if (warp >= 4) {  // ------------------------------------------ epilogue
-    const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane;
+  } else {  // ------------------------------------------ epilogue
+    const int quad = warp & 3, half = warp >> 2, r = 32 * quad + lane;
     const uint32_t lane_base = (uint32_t)(32 * quad) << 16;
     RingPos ap, sp;
     bool ok = true;
     int parity = 0;
-    for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, parity ^= 1) {
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep, parity ^= 1) {
       const F8Tile t = f8_tile<NT>(p, tile);
       const int mine = min(NC, t.count - half * NC);  // valid tokens of this thread, may be <= 0
       const long ws_row = ((long)t.expert * p.rblocks + t.rb) * p.kblocks;
@@ -491,6 +545,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       for (int m = 0; m < MATS; ++m)
 #pragma unroll
         for (int c = 0; c < NC / 2; ++c) acc[m][c] = make_float2(0.0f, 0.0f);
+      auto own = [&](int c) { return !SPLIT || (c & (p.split - 1)) == (int)rank; };
       float wl[MATS];  // weight scales of 32 blocks, one a lane
       int ent[(NC + 31) / 32];  // entries of this thread's tokens, 32 a register
       if (MODE == kF8Partial) {
@@ -498,24 +553,26 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int i = 0; i < (NC + 31) / 32; ++i)
           ent[i] = 32 * i + lane < mine ? __ldcg(p.entry + t.row0 + half * NC + 32 * i + lane) : 0;
       }
-      for (int kb = 0; kb < p.kblocks; ++kb) {
-        if ((kb & 31) == 0) {
-          const bool in = kb + lane < p.kblocks;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (((kb - kb0) & 31) == 0) {
+          const bool in = kb + lane < kb1;
           wl[0] = in ? __ldg(p.ws0 + ws_row + kb + lane) : 0.0f;
           if (MATS == 2) wl[MATS - 1] = in ? __ldg(p.ws1 + ws_row + kb + lane) : 0.0f;
         }
         float sw[MATS];
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) sw[m] = __shfl_sync(0xffffffffu, wl[m], kb & 31);
+        for (int m = 0; m < MATS; ++m) sw[m] = __shfl_sync(0xffffffffu, wl[m], (kb - kb0) & 31);
         ok = f8_wait(&sy->sfull[sp.s], sp.phase, p.status, abort) &&
              f8_wait(&sy->tfull[ap.s], ap.phase, p.status, abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         const float* sc = s_scale + sp.s * NT + half * NC;
-        // columns loaded together: all of them while the registers last, since the
-        // loads of a second group wait for the first
-        constexpr int CH = NC < 64 / MATS ? NC : 64 / MATS;
+        // columns loaded together, as many as the registers hold: the loads of a
+        // second group wait for the first
+        constexpr int CH = MATS == 2 && NT == 128 ? 8
+                           : C::kCtas == 2        ? (NC < 16 / MATS ? NC : 16 / MATS)
+                                                  : (NC < 64 / MATS ? NC : 64 / MATS);
 #pragma unroll
         for (int c0 = 0; c0 < NC; c0 += CH) {
           if (c0 < mine) {  // warp-uniform
@@ -556,13 +613,47 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         sp.next(kF8Scales);
       }
       if (!ok) break;
+      if (SPLIT) {
+        // every product of this CTA is in registers, so the stages are free; CTA
+        // `rank` finishes the columns that are `rank` modulo split, adding the
+        // others' sums to its own in the order of their ranks from its own on
+        float* red = reinterpret_cast<float*>(stages) + (half * NC) * kF8M + r;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (c < mine && !own(c))
+              red[(m * NT + c) * kF8M] = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
+        cluster_sync();
+        synced = true;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (c < mine && own(c)) {  // warp-uniform
+              float v[kF8MaxSplit];
+#pragma unroll
+              for (int k = 1; k < kF8MaxSplit; ++k)
+                if (k < split)
+                  v[k] = cluster_ld(
+                      cluster_map(red + (m * NT + c) * kF8M, (rank + k) & (split - 1)));
+              float y = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
+#pragma unroll
+              for (int k = 1; k < kF8MaxSplit; ++k)
+                if (k < split) y += v[k];
+              if (c & 1)
+                acc[m][c / 2].y = y;
+              else
+                acc[m][c / 2].x = y;
+            }
+      }
       const int row = t.rb * kF8M + r;
       const int tok0 = t.row0 + half * NC;
       if (MODE == kF8Out) {
         if (row < p.rows) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (c < mine) {
+            if (c < mine && own(c)) {
               const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
               const long o = (long)(tok0 + c) * p.ldo + row;
               if (p.out_bf16)
@@ -574,7 +665,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       } else if (MODE == kF8Partial) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          if (c < mine) {  // warp-uniform
+          if (c < mine && own(c)) {  // warp-uniform
             const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
             const long id = __shfl_sync(0xffffffffu, ent[c / 32], c & 31);
             if (row < p.rows) p.partial[id * p.ldp + row] = y;
@@ -595,7 +686,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             h[c] = v * v;
           }
           if (row >= p.rows) h[c] = 0.0f;
-          if (c < mine) {
+          if (c < mine && own(c)) {
             const uint32_t a =
                 __reduce_max_sync(0xffffffffu, __float_as_uint(h[c]) & 0x7fffffffu);
             if (lane == 0) am[quad * NT + c] = a;
@@ -604,7 +695,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         named_bar_sync(1 + half, 128);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          if (c < mine) {
+          if (c < mine && own(c)) {
             const float s = block_scale(
                 max(max(am[c], am[NT + c]), max(am[2 * NT + c], am[3 * NT + c])));
             p.hq[(long)(tok0 + c) * p.h_pitch + row] = (uint8_t)e4m3_byte(__fdiv_rn(h[c], s));
@@ -613,9 +704,14 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       }
     }
   }
+  if (SPLIT) {
+    __syncwarp();
+    if (!synced) cluster_sync();
+    cluster_sync();  // the others have read this CTA's sums
+  }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == kF8EpiWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kCols);
   }
@@ -769,14 +865,36 @@ cudaError_t f8_allow_smem(const void* kern, size_t bytes) {
   return e;
 }
 
+// tiles: an upper bound.  Where they leave CTAs idle, clusters share a tile's K
+// as long as the CTAs stay resident together and each has about two blocks
+// (one token by 14336 x 4096: 17.0 us unsplit, __SPLIT__ in two).
 template <int NT, int MATS, int MODE>
-cudaError_t launch_f8_gemm(const F8Maps& maps, const F8Pass& p, long tiles, cudaStream_t s) {
-  auto kern = f8_gemm_kernel<NT, MATS, MODE>;
-  constexpr size_t smem = F8Cfg<NT, MATS>::kSmem;
-  const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), smem);
+cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_t s) {
+  using C = F8Cfg<NT, MATS>;
+  const long slots = (long)sm_count() * C::kCtas;
+  p.split = 1;
+  if (NT <= 64)
+    while (p.split < kF8MaxSplit && tiles * p.split * 2 <= slots && p.split * 2 <= (p.kblocks + 1) / 2)
+      p.split *= 2;
+  auto kern = f8_gemm_kernel<NT, MATS, MODE, false>;
+  if constexpr (NT <= 64)
+    if (p.split > 1) kern = f8_gemm_kernel<NT, MATS, MODE, true>;
+  const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), C::kSmem);
   if (e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)std::min<long>(tiles, sm_count());
-  return launch_pdl(kern, dim3(grid), dim3(kF8Threads), smem, s, maps, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : std::min(tiles, slots)));
+  cfg.blockDim = dim3(kF8Threads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = p.split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, maps, p);
 }
 
 template <int MATS, int MODE>
@@ -832,7 +950,8 @@ cudaError_t f8_prepare(F8Matrix* w) {
 }
 
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
-                              bool out_bf16, void* out, long ldo, int* status, cudaStream_t st) {
+                              bool out_bf16, void* out, long ldo, bool after_quant, int* status,
+                              cudaStream_t st) {
   F8Maps maps;
   const int nt = f8_chunk(tokens);
   maps.w0 = maps.w1 = w.map;
@@ -849,6 +968,7 @@ cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* 
   p.out = out;
   p.ldo = ldo;
   p.out_bf16 = out_bf16;
+  p.early = after_quant;
   p.status = status;
   return launch_f8_pass<1, kF8Out>(nt, maps, p, (long)p.chunks * p.rblocks, st);
 }
@@ -920,6 +1040,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   p.h_pitch = L.hp;
   p.hs = reinterpret_cast<float*>(base + L.hs);
   p.hs_pitch = L.rows;
+  p.early = 1;
   p.status = status;
   e = m.gate.data ? launch_f8_pass<2, kF8Act>(nt, maps, p, chunks * p.rblocks, st)
                   : launch_f8_pass<1, kF8Act>(nt, maps, p, chunks * p.rblocks, st);
@@ -939,6 +1060,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   d.partial = partial;
   d.ldp = L.ldp;
   d.entry = entry;
+  d.early = 1;
   d.status = status;
   e = launch_f8_pass<1, kF8Partial>(nt, maps, d, chunks * d.rblocks, st);
   if (e != cudaSuccess) return e;

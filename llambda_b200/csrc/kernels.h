@@ -330,9 +330,12 @@ cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaSt
 cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int cols, uint8_t* q,
                             float* scales, cudaStream_t st);
 // out[t][n] = w . x for quantised rows (pitch f8_pad16(cols), scales' pitch
-// f8_pad4(tokens)).
+// f8_pad4(tokens)).  after_quant: the kernel before in the stream is this
+// library's quantiser, which has waited for whatever wrote the weights, so the
+// first of them may be loaded before it ends.
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
-                              bool out_bf16, void* out, long ldo, int* status, cudaStream_t st);
+                              bool out_bf16, void* out, long ldo, bool after_quant, int* status,
+                              cudaStream_t st);
 F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k);
 cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, int tokens, int k,
                           const int* sel, const float* weights, bool out_bf16, void* out, long ldo,

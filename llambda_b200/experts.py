@@ -58,41 +58,62 @@ def _pad(n: int, m: int) -> int:
     return -(-n // m) * m
 
 
-def _device_tensor(t, name: str, dtypes, ndim: int, shape=None, device=None, contiguous=False):
-    """Checks a CUDA tensor: type, rank, shape (None: any), unit stride along the last axis."""
+def _device_tensor(t, name: str, dtypes, shape, device=None, contiguous=False):
+    """Checks a CUDA tensor: type, shape (None: any), unit stride along the last axis."""
     torch = _t or _torch()
+    try:  # the usual case in few steps; what fails it is looked at below
+        if (t.is_cuda and t.dtype in dtypes and t.shape == shape and t.is_contiguous()
+                and t.numel() and (device is None or t.device == device)
+                and not t.requires_grad):
+            return t
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, "
                          f"got {str(t.dtype)[6:]}")
     got = t.shape
-    if len(got) != ndim or (shape is not None and
-                            any(w is not None and w != g for w, g in zip(shape, got))):
+    if len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
         raise ValueError(f"{name} has shape {tuple(got)}, expected "
-                         f"{tuple('any' if s is None else s for s in shape or (None,) * ndim)}")
+                         f"{tuple('any' if s is None else s for s in shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires grad; these operators have no backward pass")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not {device}")
+    if 0 in got:
+        raise ValueError(f"{name} is empty (a positive token count is required)")
     if contiguous:
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
     elif got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
-    if 0 in got:
-        raise ValueError(f"{name} is empty (a positive token count is required)")
     return t
 
 
-@functools.lru_cache(maxsize=None)
+def _matrix(t, name: str, cols=None, device=None):
+    """Checks a float32 or bfloat16 operand [tokens][cols]; its (rows, columns, row stride)."""
+    try:
+        shape = t.shape
+        rows, want = shape if cols is None else (shape[0], cols)
+    except (AttributeError, ValueError, IndexError, TypeError):
+        rows, want = None, cols
+    _device_tensor(t, name, _FLOATS or _floats(), (rows, want), device)
+    return rows, want, t.stride(0) if rows > 1 else want
+
+
+_FLOATS = ()
+
+
 def _floats():
+    global _FLOATS
     torch = _torch()
-    return torch.float32, torch.bfloat16
+    _FLOATS = (torch.float32, torch.bfloat16)
+    return _FLOATS
 
 
 def _tag(dtype) -> int:
-    return N.TYPE_F32 if dtype is _floats()[0] else N.TYPE_BF16
+    return N.TYPE_F32 if dtype is _FLOATS[0] else N.TYPE_BF16
 
 
 @functools.lru_cache(maxsize=None)
@@ -102,52 +123,41 @@ def _raw_stream():
                    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class _Stream:
-    """The raw handle of a call's stream; as a context, makes it current, so
-    that what the call allocates belongs to it."""
-
-    def __init__(self, stream, device):
-        if stream is None:
-            self._ctx, self.raw = None, _raw_stream()(device.index)
-        else:
-            torch = _torch()
-            if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream), device=device)
-            if stream.device != device:
-                raise ValueError(f"the stream is on {stream.device}, not {device}")
-            self._ctx, self.raw = torch.cuda.stream(stream), stream.cuda_stream
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-
-
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _on(stream, device, allocate):
+    """(raw handle of the call's stream, allocate()'s result with that stream
+    current, so that what the call allocates belongs to it)."""
+    if stream is None:
+        return _raw_stream()(device.index), allocate()
+    torch = _torch()
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, not {device}")
+    with torch.cuda.stream(stream):
+        return stream.cuda_stream, allocate()
 
 
 def _out(out, rows: int, cols: int, dtype, device, name="out"):
     if out is None:
-        if dtype not in _floats():
+        if dtype not in _FLOATS:
             raise ValueError(f"{name} must be float32 or bfloat16, got {str(dtype)[6:]}")
-        return _torch().empty(rows, cols, dtype=dtype, device=device)
-    return _device_tensor(out, name, _floats(), 2, (rows, cols), device)
+        return _t.empty((rows, cols), dtype=dtype, device=device), cols
+    _device_tensor(out, name, _FLOATS, (rows, cols), device)
+    return out, out.stride(0) if rows > 1 else cols
 
 
 # ------------------------------------------------------------------ routing
 
 
+@functools.lru_cache(maxsize=256)  # descriptors are constants, built once per set of options
 def _route_desc(experts, top_k, score, groups, top_groups, group_top, renormalise, weight_scale):
     scores = {"softmax": N.SCORE_SOFTMAX, "sigmoid": N.SCORE_SIGMOID}
     if score not in scores:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
-    return N.RouteDesc(experts, top_k, scores[score], groups, top_groups, group_top,
-                       int(bool(renormalise)), weight_scale)
+    if not 1 <= top_k <= experts:
+        raise ValueError(f"top_k must be in 1..{experts}, got {top_k}")
+    return C.pointer(N.RouteDesc(experts, top_k, scores[score], groups, top_groups, group_top,
+                                 int(bool(renormalise)), weight_scale))
 
 
 def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int = 1,
@@ -168,41 +178,34 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
         return _route_host(logits, bias, _route_desc(
             np.shape(logits)[-1], top_k, score, groups, top_groups, group_top, renormalise,
             weight_scale))
-    torch = _torch()
-    _device_tensor(logits, "logits", _floats(), 2)
-    T, E = logits.shape
+    T, E, ld = _matrix(logits, "logits")
     dev = logits.device
     if bias is not None:
-        _device_tensor(bias, "bias", (torch.float32,), 1, (E,), dev)
+        _device_tensor(bias, "bias", (_t.float32,), (E,), dev)
     desc = _route_desc(E, top_k, score, groups, top_groups, group_top, renormalise, weight_scale)
-    if not 1 <= top_k <= E:
-        raise ValueError(f"top_k must be in 1..{E}, got {top_k}")
-    with _Stream(stream, dev) as st:
-        selected = torch.empty(T, top_k, dtype=torch.int32, device=dev)
-        weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
-    _call(
-        "llambda_cuda_route_device", C.byref(desc), _tag(logits.dtype), logits.data_ptr(), _row_stride(logits),
-        bias.data_ptr() if bias is not None else None, T, selected.data_ptr(), weights.data_ptr(),
-        st.raw)
+    raw, (selected, weights) = _on(stream, dev, lambda: (
+        _t.empty((T, top_k), dtype=_t.int32, device=dev),
+        _t.empty((T, top_k), dtype=_t.float32, device=dev)))
+    _call("llambda_cuda_route_device", desc, _tag(logits.dtype), logits.data_ptr(), ld,
+          bias.data_ptr() if bias is not None else None, T, selected.data_ptr(),
+          weights.data_ptr(), raw)
     return selected, weights
 
 
 def _route_host(logits, bias, desc):
     logits = N._f32(logits)
+    E, k = desc.contents.experts, desc.contents.top_k
     if logits.ndim != 2 or 0 in logits.shape:
         raise ValueError("logits must be [tokens][experts] with a positive token count")
     if bias is not None:
         bias = N._f32(bias)
-        if bias.shape != (desc.experts,):
-            raise ValueError(f"bias must have shape ({desc.experts},)")
-    if not 1 <= desc.top_k <= desc.experts:
-        raise ValueError(f"top_k must be in 1..{desc.experts}, got {desc.top_k}")
+        if bias.shape != (E,):
+            raise ValueError(f"bias must have shape ({E},)")
     T = logits.shape[0]
-    selected = np.empty((T, desc.top_k), np.int32)
-    weights = np.empty((T, desc.top_k), np.float32)
-    _call("llambda_cuda_route",
-        C.byref(desc), logits.ctypes.data, bias.ctypes.data if bias is not None else None, T,
-        selected.ctypes.data, weights.ctypes.data)
+    selected, weights = np.empty((T, k), np.int32), np.empty((T, k), np.float32)
+    _call("llambda_cuda_route", desc, logits.ctypes.data,
+          bias.ctypes.data if bias is not None else None, T, selected.ctypes.data,
+          weights.ctypes.data)
     return selected, weights
 
 
@@ -215,14 +218,13 @@ def fp8_quantize(x, *, stream=None):
     [ceil(cols / 128), T rounded up to 4] with zeros past T, so that x[t, c] is
     about q[t, c] * scales[c // 128, t].  scale = max(max|x| / 448, 2^-126) of
     the row's block, q = e4m3(x / scale), everything rounded to nearest."""
-    torch = _torch()
-    _device_tensor(x, "x", _floats(), 2)
-    T, cols = x.shape
-    with _Stream(stream, x.device) as st:
-        q = torch.empty(T, _pad(cols, 16), dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty(_blocks(cols), _pad(T, 4), dtype=torch.float32, device=x.device)
-    _call("llambda_cuda_fp8_quantize_device",
-        _tag(x.dtype), x.data_ptr(), _row_stride(x), T, cols, q.data_ptr(), scales.data_ptr(), st.raw)
+    T, cols, ldx = _matrix(x, "x")
+    dev = x.device
+    raw, (q, scales) = _on(stream, dev, lambda: (
+        _t.empty((T, _pad(cols, 16)), dtype=_t.float8_e4m3fn, device=dev),
+        _t.empty((_blocks(cols), _pad(T, 4)), dtype=_t.float32, device=dev)))
+    _call("llambda_cuda_fp8_quantize_device", _tag(x.dtype), x.data_ptr(), ldx, T, cols,
+          q.data_ptr(), scales.data_ptr(), raw)
     return q, scales
 
 
@@ -230,10 +232,10 @@ def _device_weights(pair, name: str, ndim: int, device=None):
     """Checks (weights, scales) in device memory."""
     torch = _torch()
     w, s = pair
-    _device_tensor(w, f"{name} weights", (torch.float8_e4m3fn, torch.uint8), ndim, device=device,
+    _device_tensor(w, f"{name} weights", (torch.float8_e4m3fn, torch.uint8), (None,) * ndim, device,
                    contiguous=True)
     want = tuple(w.shape[:-2]) + (_blocks(w.shape[-2]), _blocks(w.shape[-1]))
-    _device_tensor(s, f"{name} scales", (torch.float32,), ndim, want, w.device, contiguous=True)
+    _device_tensor(s, f"{name} scales", (torch.float32,), want, w.device, contiguous=True)
     return w, s
 
 
@@ -334,33 +336,31 @@ class Fp8ProjectionSession(_Fp8Session):
     def run_device(self, x, out=None, *, out_dtype=None, stream=None):
         """x [T, cols] (float32 or bfloat16 CUDA tensor) -> out [T, rows], made
         of `out_dtype` (default x's) unless given."""
-        torch = _torch()
         h = self._handle()
-        _device_tensor(x, "x", _floats(), 2, (None, self.cols), self.device)
-        T = x.shape[0]
-        with _Stream(stream, x.device) as st:
-            out = _out(out, T, self.rows, out_dtype or x.dtype, x.device)
-            nbytes = N.lib().llambda_cuda_fp8_session_workspace(h, T)
-            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _call("llambda_cuda_fp8_session_run_device",
-            h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, _tag(out.dtype), out.data_ptr(),
-            _row_stride(out), work.data_ptr(), nbytes, st.raw)
+        T, _, ldx = _matrix(x, "x", self.cols, self.device)
+        dev = x.device
+        nbytes = _entry("llambda_cuda_fp8_session_workspace")(h, T)
+        raw, ((out, ldo), work) = _on(stream, dev, lambda: (
+            _out(out, T, self.rows, out_dtype or x.dtype, dev),
+            _t.empty(nbytes, dtype=_t.uint8, device=dev)))
+        _call("llambda_cuda_fp8_session_run_device", h, _tag(x.dtype), x.data_ptr(), ldx, T,
+              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr(), nbytes, raw)
         return out
 
     def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):
         """As run_device over what fp8_quantize returned for `tokens` rows of
         `cols` columns (several projections of one input quantise it once)."""
         torch = _torch()
+        _floats()
         h = self._handle()
-        _device_tensor(q, "q", (torch.float8_e4m3fn, torch.uint8), 2, (tokens, _pad(self.cols, 16)),
+        _device_tensor(q, "q", (torch.float8_e4m3fn, torch.uint8), (tokens, _pad(self.cols, 16)),
                        self.device, contiguous=True)
-        _device_tensor(scales, "scales", (torch.float32,), 2, (_blocks(self.cols), _pad(tokens, 4)),
+        _device_tensor(scales, "scales", (torch.float32,), (_blocks(self.cols), _pad(tokens, 4)),
                        q.device, contiguous=True)
-        with _Stream(stream, q.device) as st:
-            out = _out(out, tokens, self.rows, out_dtype or torch.float32, q.device)
-        _call("llambda_cuda_fp8_session_run_quantized",
-            h, q.data_ptr(), scales.data_ptr(), tokens, _tag(out.dtype), out.data_ptr(),
-            _row_stride(out), st.raw)
+        raw, (out, ldo) = _on(stream, q.device, lambda: _out(
+            out, tokens, self.rows, out_dtype or torch.float32, q.device))
+        _call("llambda_cuda_fp8_session_run_quantized", h, q.data_ptr(), scales.data_ptr(), tokens,
+              _tag(out.dtype), out.data_ptr(), ldo, raw)
         return out
 
 
@@ -427,19 +427,17 @@ class Fp8MoeSession(_Fp8Session):
         [T, k] (route_experts' results) -> out [T, O] = the weighted sum over a
         token's entries, made of `out_dtype` (default x's) unless given.  Entries
         whose expert is outside 0..E-1 add nothing."""
-        torch = _torch()
         h = self._handle()
-        _device_tensor(x, "x", _floats(), 2, (None, self.hidden), self.device)
-        T, dev = x.shape[0], x.device
-        _device_tensor(selected, "selected", (torch.int32,), 2, (T, None), dev, contiguous=True)
-        k = selected.shape[1]
-        _device_tensor(weights, "weights", (torch.float32,), 2, (T, k), dev, contiguous=True)
-        with _Stream(stream, dev) as st:
-            out = _out(out, T, self.out_features, out_dtype or x.dtype, dev)
-            nbytes = N.lib().llambda_cuda_fp8_moe_session_workspace(h, T, k)
-            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _call("llambda_cuda_fp8_moe_session_run_device",
-            h, _tag(x.dtype), x.data_ptr(), _row_stride(x), T, k, selected.data_ptr(),
-            weights.data_ptr(), _tag(out.dtype), out.data_ptr(), _row_stride(out), work.data_ptr(),
-            nbytes, st.raw)
+        T, _, ldx = _matrix(x, "x", self.hidden, self.device)
+        dev = x.device
+        k = selected.shape[1] if getattr(selected, "ndim", 0) == 2 else None
+        _device_tensor(selected, "selected", (_t.int32,), (T, k), dev, contiguous=True)
+        _device_tensor(weights, "weights", (_t.float32,), (T, k), dev, contiguous=True)
+        nbytes = _entry("llambda_cuda_fp8_moe_session_workspace")(h, T, k)
+        raw, ((out, ldo), work) = _on(stream, dev, lambda: (
+            _out(out, T, self.out_features, out_dtype or x.dtype, dev),
+            _t.empty(nbytes, dtype=_t.uint8, device=dev)))
+        _call("llambda_cuda_fp8_moe_session_run_device", h, _tag(x.dtype), x.data_ptr(), ldx, T, k,
+              selected.data_ptr(), weights.data_ptr(), _tag(out.dtype), out.data_ptr(), ldo,
+              work.data_ptr(), nbytes, raw)
         return out
