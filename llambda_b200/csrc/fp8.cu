@@ -327,6 +327,20 @@ __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, int* sta
   return false;
 }
 
+// After a wait that gave up: copies that are still in flight land before the
+// CTA's memory goes (otherwise the MMAs have waited for every copy).
+__device__ __forceinline__ void f8_linger() {
+  const uint64_t t0 = global_ns();
+  while (global_ns() - t0 < 1000000) {
+  }
+}
+
+// f8_wait by a whole warp, with a result that is the same on every lane.
+__device__ __forceinline__ bool f8_wait_warp(uint64_t* bar, uint32_t parity, int* status,
+                                             volatile int* abort) {
+  return __all_sync(0xffffffffu, f8_wait(bar, parity, status, abort));
+}
+
 struct F8Tile {
   int row0, count, expert, rb;  // first row of x, valid rows, expert, row block
 };
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
   uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + kF8Scales * NT);  // [parity][quadrant][NT]
   F8Sync* sy = reinterpret_cast<F8Sync*>(s_amax + 2 * 4 * NT);
   volatile int* abort = &sy->abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&sy->full[s], 1);
@@ -417,7 +431,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sy->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sy->tmem, 0);
   const bool early = p.early && warp == kF8EpiWarps;
   if (!early) {
     griddep_wait();
@@ -431,104 +445,100 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
   bool synced = false;  // split: this warp has met the others of the cluster
 
   if (warp == kF8EpiWarps) {  // ------------------------------------- weights, activations
-    if (lane == 0) {
-      RingPos rp;
-      int q = 0, ahead = 0;
-      uint32_t last_phase[C::kStages] = {};
-      auto load_weights = [&](int s, int kb, const F8Tile& t) {
-        uint8_t* st = stages + (size_t)s * C::kStage;
-        uint64_t* bar = &sy->full[s];
-        mbar_expect_tx(bar, C::kStage);
-        tma_load_3d(st, &maps.w0, kb * kF8Block, t.rb * kF8M, t.expert, bar);
-        if (MATS == 2)
-          tma_load_3d(st + C::kA, &maps.w1, kb * kF8Block, t.rb * kF8M, t.expert, bar);
-      };
-      if (early) {  // the first tile's weights while the previous kernel still runs
-        if (tile0 < ntiles) {
-          const F8Tile t = f8_tile<NT>(p, tile0);
-          for (; ahead < C::kStages && kb0 + ahead < kb1; ++ahead)
-            load_weights(ahead, kb0 + ahead, t);
-        }
-        griddep_wait();
-        griddep_launch();
+    const bool one = elect_one();
+    RingPos rp;
+    int q = 0, ahead = 0;
+    auto load_weights = [&](int s, int kb, const F8Tile& t) {
+      uint8_t* st = stages + (size_t)s * C::kStage;
+      uint64_t* bar = &sy->full[s];
+      mbar_expect_tx(bar, C::kStage);
+      tma_load_3d(st, &maps.w0, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+      if (MATS == 2)
+        tma_load_3d(st + C::kA, &maps.w1, kb * kF8Block, t.rb * kF8M, t.expert, bar);
+    };
+    if (early) {  // the first tile's weights while the previous kernel still runs
+      if (tile0 < ntiles) {
+        const F8Tile t = f8_tile<NT>(p, tile0);
+        for (; ahead < C::kStages && kb0 + ahead < kb1; ++ahead)
+          if (one) load_weights(ahead, kb0 + ahead, t);
       }
-      for (int tile = tile0; tile < ntiles && !*abort; tile += tstep) {
-        const F8Tile t = f8_tile<NT>(p, tile);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (q >= C::kStages &&
-              !f8_wait(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort))
-            break;
+      griddep_wait();
+      griddep_launch();
+    }
+    bool ok = true;
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+      const F8Tile t = f8_tile<NT>(p, tile);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = q < C::kStages || f8_wait_warp(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort);
+        if (!ok) break;
+        if (one) {
           if (q >= ahead) load_weights(rp.s, kb, t);
           tma_load_2d(stages + (size_t)rp.s * C::kStage + MATS * C::kA, &maps.x, kb * kF8Block,
                       t.row0, &sy->full[rp.s]);
-          last_phase[rp.s] = rp.phase;
-          ++q;
-          rp.next(C::kStages);
         }
+        ++q;
+        rp.next(C::kStages);
       }
-      // copies still in flight land before the CTA exits (bounded)
-      for (int s = 0; s < C::kStages && s < q; ++s) mbar_wait(&sy->full[s], last_phase[s], nullptr);
     }
     __syncwarp();
   } else if (warp == kF8EpiWarps + 2) {  // -------------------------------------------- scales
-    if (lane == 0) {
-      RingPos rp;
-      int q = 0;
-      uint32_t last_phase[kF8Scales] = {};
-      for (int tile = tile0; tile < ntiles && !*abort; tile += tstep) {
-        const F8Tile t = f8_tile<NT>(p, tile);
-        // row0 and the pitch are multiples of 4; columns past the pitch keep
-        // what an earlier tile left and belong to no valid row
-        const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (q >= kF8Scales &&
-              !f8_wait(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort))
-            break;
+    const bool one = elect_one();
+    RingPos rp;
+    int q = 0;
+    bool ok = true;
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+      const F8Tile t = f8_tile<NT>(p, tile);
+      // row0 and the pitch are multiples of 4; columns past the pitch keep
+      // what an earlier tile left and belong to no valid row
+      const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = q < kF8Scales || f8_wait_warp(&sy->sempty[rp.s], rp.phase ^ 1u, p.status, abort);
+        if (!ok) break;
+        if (one) {
           mbar_expect_tx(&sy->sfull[rp.s], bytes);
           tma_load_1d(s_scale + rp.s * NT, p.xs + kb * p.xs_pitch + t.row0, bytes,
                       &sy->sfull[rp.s]);
-          last_phase[rp.s] = rp.phase;
-          ++q;
-          rp.next(kF8Scales);
         }
+        ++q;
+        rp.next(kF8Scales);
       }
-      for (int s = 0; s < kF8Scales && s < q; ++s) mbar_wait(&sy->sfull[s], last_phase[s], nullptr);
     }
     __syncwarp();
   } else if (warp == kF8EpiWarps + 1) {  // ----------------------------------------------- MMA
-    if (lane == 0) {
-      RingPos rp, ap;
-      int q = 0;
-      bool ok = true;
-      for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-        const F8Tile t = f8_tile<NT>(p, tile);
-        const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = (q < C::kBufs ||
-                f8_wait(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
-               f8_wait(&sy->full[rp.s], rp.phase, p.status, abort);
-          if (!ok) break;
-          tc_fence_after();
-          const uint8_t* st = stages + (size_t)rp.s * C::kStage;
-          const uint64_t bd = sw128_desc(st + MATS * C::kA);
+    const bool one = elect_one();
+    RingPos rp, ap;
+    int q = 0;
+    bool ok = true;
+    const uint64_t desc = sw128_desc(stages);
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+      const F8Tile t = f8_tile<NT>(p, tile);
+      const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = (q < C::kBufs || f8_wait_warp(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
+             f8_wait_warp(&sy->full[rp.s], rp.phase, p.status, abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t ad = desc + (uint32_t)rp.s * (C::kStage >> 4);
+        const uint64_t bd = ad + (MATS * C::kA >> 4);
+        const uint32_t d = tmem + ap.s * C::kAcc;
+        if (one) {
 #pragma unroll
-          for (int mat = 0; mat < MATS; ++mat) {
-            const uint64_t ad = sw128_desc(st + mat * C::kA);
+          for (int mat = 0; mat < MATS; ++mat)
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // K steps of 32 bytes
-              tc_mma_f8(tmem + ap.s * C::kAcc + mat * NT, ad + 2 * j, bd + 2 * j, idesc, j != 0);
-          }
+              tc_mma_f8(d + mat * NT, ad + mat * (C::kA >> 4) + 2 * j, bd + 2 * j, idesc, j != 0);
           tc_commit(&sy->empty[rp.s]);
           tc_commit(&sy->tfull[ap.s]);
-          ++q;
-          rp.next(C::kStages);
-          ap.next(C::kBufs);
         }
+        __syncwarp();
+        ++q;
+        rp.next(C::kStages);
+        ap.next(C::kBufs);
       }
-      // every MMA issued has completed before the tensor memory is freed
-      tc_commit(&sy->done);
-      mbar_wait(&sy->done, 0, nullptr);
     }
+    // every MMA issued has completed before the tensor memory is freed
+    if (one) tc_commit(&sy->done);
+    mbar_wait(&sy->done, 0, nullptr);
     __syncwarp();
   } else {  // ------------------------------------------ epilogue
     const int quad = warp & 3, half = warp >> 2, r = 32 * quad + lane;
@@ -704,6 +714,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
       }
     }
   }
+  if (*abort) f8_linger();
   if (SPLIT) {
     __syncwarp();
     if (!synced) cluster_sync();
@@ -714,6 +725,320 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
   if (warp == kF8EpiWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// ------------------------------------------------------------ large products
+
+// Many tokens: tiles of 256 tokens x 256 weight rows, each by a pair of CTAs
+// (cta_group::2).  CTA r of the pair stages tokens [128 r, 128 r + 128) and
+// weight rows [128 r, 128 r + 128) of the tile, 32 KB a block of K; the pair's
+// MMA reads both and leaves 128 tokens x 256 columns of fp32 sums in each CTA's
+// tensor memory, twice, so that a block's MMAs run while the one before is
+// added up.  What bounds the unpaired 128 x 128 form is the way from L2: it
+// reads 32 KB for a quarter of the products (2048 tokens by 14336 x 4096:
+// 264 us; pairs __BIG__ us).
+//
+// Here M is the tokens' side: a thread of the epilogue has one token and 64
+// columns of one weight block, so a block of K has one factor a thread and 32
+// packed FMAs are about all it costs.
+constexpr int kBigStages = 5;
+constexpr int kBigEpi = 16;  // epilogue warps: a tile's 256 columns in four parts
+constexpr int kBigThreads = (kBigEpi + 2) * 32;
+constexpr uint32_t kBigStage = 2 * kF8M * kF8Block;
+constexpr int kBigPitch = 17;  // words of a staged output row, one more than it holds
+
+struct BigSync {
+  uint64_t full[kBigStages], empty[kBigStages], tfull[2], tempty[2], done;
+  uint64_t sfull[kF8Scales], sempty[kF8Scales];
+  uint32_t tmem;
+  int abort;
+};
+constexpr size_t kBigSmem = 1024 + (size_t)kBigStages * kBigStage + kF8Scales * kF8M * 4 +
+                            kBigEpi * 32 * kBigPitch * 4 + sizeof(BigSync);
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_addr(dst)),
+               "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols)
+               : "memory");
+}
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrives on `bar` of both CTAs once every MMA this thread issued before has completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Tensor copies into this CTA's shared memory that complete on the barrier at
+// the cluster address `bar` of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int x, int y,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const void* tmap, int x, int y, int z,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// Arrival on either CTA's barrier.  It orders tensor-memory loads (complete,
+// and fenced) before the MMAs of whoever waits, no ordinary memory, so it needs
+// no release at cluster scope, which costs a memory barrier of about 1500
+// clocks (with it, the whole product ran at that pace: 275 us).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// 16 consecutive fp32 columns of this thread's tensor-memory lane (no wait).
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
+    f8_big_kernel(const __grid_constant__ F8Maps maps, const F8Pass p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  float* s_scale = reinterpret_cast<float*>(stages + kBigStages * kBigStage);
+  uint32_t* s_out = reinterpret_cast<uint32_t*>(s_scale + kF8Scales * kF8M);
+  BigSync* sy = reinterpret_cast<BigSync*>(s_out + kBigEpi * 32 * kBigPitch);
+  volatile int* abort = &sy->abort;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kBigStages; ++s) {
+      mbar_init(&sy->full[s], 1);
+      mbar_init(&sy->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sy->tfull[b], 1);
+      mbar_init(&sy->tempty[b], 2 * kBigEpi);
+    }
+    for (int s = 0; s < kF8Scales; ++s) {
+      mbar_init(&sy->sfull[s], 1);
+      mbar_init(&sy->sempty[s], kBigEpi);
+    }
+    mbar_init(&sy->done, 1);
+    sy->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kBigEpi + 1) tmem_alloc_pair(&sy->tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sy->tmem, 0);
+  griddep_wait();
+  griddep_launch();
+  const int tchunks = (p.tokens + 2 * kF8M - 1) / (2 * kF8M);
+  const int ntiles = tchunks * ((p.rows + 2 * kF8M - 1) / (2 * kF8M));
+  const int tile0 = (int)blockIdx.x >> 1, tstep = (int)gridDim.x >> 1;
+
+  if (warp == kBigEpi) {  // ------------------------------- producer
+    const bool one = elect_one();
+    RingPos rp, sp;
+    int q = 0;
+    bool ok = true;
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+      const int nt = tile / tchunks, tt = tile - nt * tchunks;
+      const int t0 = tt * 2 * kF8M + (int)rank * kF8M, n0 = nt * 2 * kF8M + (int)rank * kF8M;
+      const uint32_t sbytes = (uint32_t)max(0L, min((long)kF8M, p.xs_pitch - t0)) * 4u;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = (q < kBigStages || f8_wait_warp(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort)) &&
+             (q < kF8Scales || f8_wait_warp(&sy->sempty[sp.s], sp.phase ^ 1u, p.status, abort));
+        if (!ok) break;
+        uint8_t* st = stages + rp.s * kBigStage;
+        // both CTAs' copies complete on the first one's barrier
+        const uint32_t bar = cluster_map(&sy->full[rp.s], 0);
+        if (one) {
+          if (rank == 0) mbar_expect_tx(&sy->full[rp.s], 2 * kBigStage);
+          tma_load_2d_pair(st, &maps.x, kb * kF8Block, t0, bar);
+          tma_load_3d_pair(st + kF8M * kF8Block, &maps.w0, kb * kF8Block, n0, 0, bar);
+          mbar_expect_tx(&sy->sfull[sp.s], sbytes);
+          if (sbytes)
+            tma_load_1d(s_scale + sp.s * kF8M, p.xs + (long)kb * p.xs_pitch + t0, sbytes,
+                        &sy->sfull[sp.s]);
+        }
+        ++q;
+        rp.next(kBigStages);
+        sp.next(kF8Scales);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kBigEpi + 1) {  // -------------------------- MMA
+    const bool one = elect_one();
+    if (rank == 0) {
+      RingPos rp, ap;
+      int q = 0;
+      bool ok = true;
+      const uint64_t desc = sw128_desc(stages);
+      const uint32_t idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+      for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = (q < 2 || f8_wait_warp(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
+               f8_wait_warp(&sy->full[rp.s], rp.phase, p.status, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = desc + (uint32_t)rp.s * (kBigStage >> 4);
+          const uint64_t bd = ad + (kF8M * kF8Block >> 4);
+          if (one) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tc_mma_f8_pair(tmem + ap.s * 256, ad + 2 * j, bd + 2 * j, idesc, j != 0);
+            tc_commit_pair(&sy->empty[rp.s]);
+            tc_commit_pair(&sy->tfull[ap.s]);
+          }
+          __syncwarp();
+          ++q;
+          rp.next(kBigStages);
+          ap.next(2);
+        }
+      }
+      // every MMA issued has completed before shared and tensor memory go
+      if (one) tc_commit_pair(&sy->done);
+    }
+    mbar_wait(&sy->done, 0, nullptr);
+    __syncwarp();
+  } else {  // -------------------------------------------------- epilogue
+    const int quad = warp & 3, part = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(32 * quad) << 16;
+    uint32_t* so = s_out + warp * 32 * kBigPitch;
+    const bool words = p.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(p.out) % 4 == 0;
+    RingPos ap, sp;
+    bool ok = true;
+    for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+      const int nt = tile / tchunks, tt = tile - nt * tchunks;
+      const int t0 = tt * 2 * kF8M + (int)rank * kF8M + 32 * quad;  // this warp's first token
+      const int n0 = nt * 2 * kF8M + part * 64;                     // its first column
+      const float* ws = p.ws0 + (long)min(n0 / kF8M, p.rblocks - 1) * p.kblocks;
+      float2 acc[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = make_float2(0.0f, 0.0f);
+      float wl = 0.0f;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if ((kb & 31) == 0) wl = kb + lane < p.kblocks ? __ldg(ws + kb + lane) : 0.0f;
+        ok = f8_wait(&sy->sfull[sp.s], sp.phase, p.status, abort);
+        const float f = s_scale[sp.s * kF8M + 32 * quad + lane] * __shfl_sync(0xffffffffu, wl, kb & 31);
+        ok = ok && f8_wait(&sy->tfull[ap.s], ap.phase, p.status, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t from = tmem + lane_base + ap.s * 256 + part * 64;
+        const float2 f2 = make_float2(f, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // 16 columns
+          uint32_t d[16];
+          tmem_ld16_issue(from + 16 * i, d);
+          tmem_wait_ld16(d);
+          if (i == 3) {  // everything read: the buffer and the scales are free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive_cluster(cluster_map(&sy->tempty[ap.s], 0));
+              mbar_arrive(&sy->sempty[sp.s]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            acc[8 * i + j] =
+                __ffma2_rn(make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), f2,
+                           acc[8 * i + j]);
+        }
+        ap.next(2);
+        sp.next(kF8Scales);
+      }
+      if (!ok) break;
+      // to row-major through shared memory: 16 words of the warp's 32 rows at a
+      // time, stored two rows an instruction
+      const int r2 = lane >> 4, w = lane & 15;
+      if (p.out_bf16) {
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 32 columns, two a word
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const __nv_bfloat162 v = __float22bfloat162_rn(acc[16 * h + j]);
+            so[lane * kBigPitch + j] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          __syncwarp();
+          const int n = n0 + 32 * h + 2 * w;
+#pragma unroll 8
+          for (int i = 0; i < 32; i += 2) {
+            const uint32_t v = so[(i + r2) * kBigPitch + w];
+            if (t0 + i + r2 >= p.tokens) continue;
+            __nv_bfloat16* o = out + (long)(t0 + i + r2) * p.ldo + n;
+            if (words && n + 1 < p.rows) {
+              *reinterpret_cast<uint32_t*>(o) = v;
+            } else {
+              const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(&v);
+              if (n < p.rows) o[0] = b.x;
+              if (n + 1 < p.rows) o[1] = b.y;
+            }
+          }
+          __syncwarp();
+        }
+      } else {
+        float* out = static_cast<float*>(p.out);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {  // 16 columns
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            so[lane * kBigPitch + j] =
+                __float_as_uint(j & 1 ? acc[8 * h + j / 2].y : acc[8 * h + j / 2].x);
+          __syncwarp();
+          const int n = n0 + 16 * h + w;
+#pragma unroll 8
+          for (int i = 0; i < 32; i += 2) {
+            const uint32_t v = so[(i + r2) * kBigPitch + w];
+            if (t0 + i + r2 < p.tokens && n < p.rows)
+              out[(long)(t0 + i + r2) * p.ldo + n] = __uint_as_float(v);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  if (*abort) f8_linger();
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // neither CTA's shared or tensor memory is in use any more
+  if (warp == kBigEpi + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -908,6 +1233,9 @@ cudaError_t launch_f8_pass(int nt, const F8Maps& maps, const F8Pass& p, long til
   }
 }
 
+// More tokens than this take the pairs' tiles of 256.
+constexpr int kF8BigTokens = 128;
+
 int f8_chunk(long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 int f8_blocks(long n) { return (int)((n + kF8Block - 1) / kF8Block); }
@@ -953,7 +1281,8 @@ cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* 
                               bool out_bf16, void* out, long ldo, bool after_quant, int* status,
                               cudaStream_t st) {
   F8Maps maps;
-  const int nt = f8_chunk(tokens);
+  const bool big = tokens > kF8BigTokens;
+  const int nt = big ? kF8M : f8_chunk(tokens);
   maps.w0 = maps.w1 = w.map;
   if (!f8_rows_map(&maps.x, q, f8_pad16(w.cols), tokens, w.cols, nt)) return cudaErrorInvalidValue;
   F8Pass p{};
@@ -970,7 +1299,12 @@ cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* 
   p.out_bf16 = out_bf16;
   p.early = after_quant;
   p.status = status;
-  return launch_f8_pass<1, kF8Out>(nt, maps, p, (long)p.chunks * p.rblocks, st);
+  if (!big) return launch_f8_pass<1, kF8Out>(nt, maps, p, (long)p.chunks * p.rblocks, st);
+  const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(f8_big_kernel), kBigSmem);
+  if (e != cudaSuccess) return e;
+  const long pairs = (long)((tokens + 255) / 256) * ((w.rows + 255) / 256);
+  return launch_pdl(f8_big_kernel, dim3((unsigned)(2 * std::min<long>(pairs, sm_count() / 2))),
+                    dim3(kBigThreads), kBigSmem, st, maps, p);
 }
 
 F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k) {
