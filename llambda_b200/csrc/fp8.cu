@@ -58,6 +58,18 @@ __device__ __forceinline__ float block_scale(uint32_t amax) {
   return s < FLT_MIN ? FLT_MIN : s;
 }
 
+// v / s, correctly rounded, with r the correctly rounded 1 / s: with q0 = v * r,
+// q0 + r * (v - q0 * s) is it (Markstein, IBM J. Res. Dev. 34, 1990), as long as
+// nothing underflows, which holds for the blocks that scale_divides accepts.  A
+// quotient a bit off would turn over the ties that bf16 inputs make.
+__device__ __forceinline__ float quotient(float v, float s, float r) {
+  const float q0 = __fmul_rn(v, r);
+  return fmaf(r, fmaf(-q0, s, v), q0);
+}
+__device__ __forceinline__ bool scale_divides(float s, uint32_t amax) {
+  return amax == 0 || (s >= 0x1p-80f && s <= 0x1p100f);
+}
+
 // ------------------------------------------------------------ quantiser
 
 __device__ __forceinline__ void load4(const float* p, bool vec, int n, float* v) {
@@ -95,12 +107,6 @@ constexpr int kQuantBlocks = 4;  // blocks of one token per warp
 // q_pitch bytes (a multiple of 16, zeros past cols), scales the layout
 // [block][s_pitch] the products read with bulk copies; ungrouped, the scales
 // of rows [tokens, s_pitch) are zeroed.
-//
-// x / s has to be the correctly rounded quotient (a quotient a bit off turns
-// over the ties of bf16 inputs).  With r the correctly rounded 1 / s and q0 =
-// x * r, q0 + r * (x - q0 * s) is it (Markstein, IBM J. Res. Dev. 34, 1990),
-// three instructions a value, as long as nothing underflows; blocks whose
-// scale is outside [2^-80, 2^100] divide.
 //
 // Bound by memory; the four blocks' scales are computed side by side on the
 // lanes, one division and one reciprocal for all.
@@ -150,17 +156,14 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
   const float s_own = block_scale(am);
   const float r_own = __frcp_rn(s_own);
   const bool plain = __all_sync(0xffffffffu,
-                                !mine || am == 0 || (s_own >= 0x1p-80f && s_own <= 0x1p100f));
+                                !mine || scale_divides(s_own, am));
   uint32_t w[kQuantBlocks];
   if (plain) {
 #pragma unroll
     for (int i = 0; i < kQuantBlocks; ++i) {
       const float s = __shfl_sync(0xffffffffu, s_own, i), r = __shfl_sync(0xffffffffu, r_own, i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float q0 = __fmul_rn(v[i][j], r);
-        v[i][j] = fmaf(r, fmaf(-q0, s, v[i][j]), q0);
-      }
+      for (int j = 0; j < 4; ++j) v[i][j] = quotient(v[i][j], s, r);
       w[i] = e4m3_pair(v[i][0], v[i][1]) | e4m3_pair(v[i][2], v[i][3]) << 16;
     }
   } else {
@@ -193,12 +196,18 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
   if (!GROUPED) {
     store(t);
   } else {
-    for (int j = 0; j < rows.k; ++j) {
-      const int id = t * rows.k + j, e = __ldg(rows.sel + id);
-      if (e < 0 || e >= rows.E) continue;
-      const int o = __ldcg(rows.row_start + e) + __ldcg(rows.pos + id);
-      if (b0 == 0 && lane == 0) rows.entry[o] = id;
-      store(o);
+    for (int j0 = 0; j0 < rows.k; j0 += 32) {  // the entries' rows, one a lane
+      const int id = t * rows.k + j0 + lane;
+      int o = -1;
+      if (j0 + lane < rows.k) {
+        const int e = __ldg(rows.sel + id);
+        if (e >= 0 && e < rows.E) o = __ldcg(rows.row_start + e) + __ldcg(rows.pos + id);
+      }
+      if (b0 == 0 && o >= 0) rows.entry[o] = id;
+      for (int j = 0; j < min(32, rows.k - j0); ++j) {
+        const int oj = __shfl_sync(0xffffffffu, o, j);
+        if (oj >= 0) store(oj);
+      }
     }
   }
 }
@@ -364,7 +373,9 @@ __device__ __forceinline__ F8Tile f8_tile(const F8Pass& p, int tile) {
   return t;
 }
 
-__device__ __forceinline__ float silu(float g) { return __fdiv_rn(g, 1.0f + expf(-g)); }
+// (__fdividef is off by two steps at most; its result for a divisor above 2^126
+// is 0, which is also that of the exact quotient here)
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -548,7 +559,10 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     int parity = 0;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep, parity ^= 1) {
       const F8Tile t = f8_tile<NT>(p, tile);
-      const int mine = min(NC, t.count - half * NC);  // valid tokens of this thread, may be <= 0
+      // this thread's tokens: groups of 8 columns in turn with the other half's,
+      // so that both have their share of a tile that is not full
+      auto col = [&](int c) { return (2 * (c >> 3) + half) * 8 + (c & 7); };
+      auto in = [&](int c) { return col(c) < t.count; };
       const long ws_row = ((long)t.expert * p.rblocks + t.rb) * p.kblocks;
       float2 acc[MATS][NC / 2];
 #pragma unroll
@@ -561,13 +575,15 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
       if (MODE == kF8Partial) {
 #pragma unroll
         for (int i = 0; i < (NC + 31) / 32; ++i)
-          ent[i] = 32 * i + lane < mine ? __ldcg(p.entry + t.row0 + half * NC + 32 * i + lane) : 0;
+          ent[i] = 32 * i + lane < NC && in(32 * i + lane)
+                       ? __ldcg(p.entry + t.row0 + col(32 * i + lane))
+                       : 0;
       }
       for (int kb = kb0; kb < kb1; ++kb) {
         if (((kb - kb0) & 31) == 0) {
-          const bool in = kb + lane < kb1;
-          wl[0] = in ? __ldg(p.ws0 + ws_row + kb + lane) : 0.0f;
-          if (MATS == 2) wl[MATS - 1] = in ? __ldg(p.ws1 + ws_row + kb + lane) : 0.0f;
+          const bool more = kb + lane < kb1;
+          wl[0] = more ? __ldg(p.ws0 + ws_row + kb + lane) : 0.0f;
+          if (MATS == 2) wl[MATS - 1] = more ? __ldg(p.ws1 + ws_row + kb + lane) : 0.0f;
         }
         float sw[MATS];
 #pragma unroll
@@ -577,7 +593,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const float* sc = s_scale + sp.s * NT + half * NC;
+        const float* sc = s_scale + sp.s * NT;
         // columns loaded together, as many as the registers hold: the loads of a
         // second group wait for the first
         constexpr int CH = MATS == 2 && NT == 128 ? 8
@@ -585,21 +601,20 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
                                                   : (NC < 64 / MATS ? NC : 64 / MATS);
 #pragma unroll
         for (int c0 = 0; c0 < NC; c0 += CH) {
-          if (c0 < mine) {  // warp-uniform
+          if (in(c0)) {  // warp-uniform
             uint32_t d[MATS][CH];
 #pragma unroll
             for (int m = 0; m < MATS; ++m)
 #pragma unroll
               for (int j = 0; j < CH; j += 8)
-                tmem_ld8_issue(tmem + lane_base + ap.s * C::kAcc + m * NT + half * NC + c0 + j,
-                               d[m] + j);
+                tmem_ld8_issue(tmem + lane_base + ap.s * C::kAcc + m * NT + col(c0 + j), d[m] + j);
 #pragma unroll
             for (int m = 0; m < MATS; ++m)
 #pragma unroll
               for (int j = 0; j < CH; j += 8) tmem_wait_ld8(d[m] + j);
 #pragma unroll
             for (int j = 0; j < CH; j += 4) {
-              const float4 sx = *reinterpret_cast<const float4*>(sc + c0 + j);
+              const float4 sx = *reinterpret_cast<const float4*>(sc + col(c0 + j));
 #pragma unroll
               for (int m = 0; m < MATS; ++m) {
                 const float2 w = make_float2(sw[m], sw[m]);
@@ -627,26 +642,26 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         // every product of this CTA is in registers, so the stages are free; CTA
         // `rank` finishes the columns that are `rank` modulo split, adding the
         // others' sums to its own in the order of their ranks from its own on
-        float* red = reinterpret_cast<float*>(stages) + (half * NC) * kF8M + r;
+        float* red = reinterpret_cast<float*>(stages) + r;
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (c < mine && !own(c))
-              red[(m * NT + c) * kF8M] = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
+            if (in(c) && !own(c))
+              red[(m * NT + col(c)) * kF8M] = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
         cluster_sync();
         synced = true;
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (c < mine && own(c)) {  // warp-uniform
+            if (in(c) && own(c)) {  // warp-uniform
               float v[kF8MaxSplit];
 #pragma unroll
               for (int k = 1; k < kF8MaxSplit; ++k)
                 if (k < split)
                   v[k] = cluster_ld(
-                      cluster_map(red + (m * NT + c) * kF8M, (rank + k) & (split - 1)));
+                      cluster_map(red + (m * NT + col(c)) * kF8M, (rank + k) & (split - 1)));
               float y = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
 #pragma unroll
               for (int k = 1; k < kF8MaxSplit; ++k)
@@ -658,14 +673,13 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
             }
       }
       const int row = t.rb * kF8M + r;
-      const int tok0 = t.row0 + half * NC;
       if (MODE == kF8Out) {
         if (row < p.rows) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
-            if (c < mine && own(c)) {
+            if (in(c) && own(c)) {
               const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
-              const long o = (long)(tok0 + c) * p.ldo + row;
+              const long o = (long)(t.row0 + col(c)) * p.ldo + row;
               if (p.out_bf16)
                 static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(y);
               else
@@ -675,41 +689,57 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
       } else if (MODE == kF8Partial) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          if (c < mine && own(c)) {  // warp-uniform
+          if (in(c) && own(c)) {  // warp-uniform
             const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
             const long id = __shfl_sync(0xffffffffu, ent[c / 32], c & 31);
             if (row < p.rows) p.partial[id * p.ldp + row] = y;
           }
       } else {
-        // the 128 rows of this tile are one block of the next product's K:
-        // its scale per token is a maximum over the four warps of this half
-        uint32_t* am = s_amax + parity * 4 * NT + half * NC;
+        // the 128 rows of this tile are one block of the next product's K: its
+        // scale per token is a maximum over the four warps of this half, and
+        // lane c works out the scale and its reciprocal of column c (and c + 32)
+        uint32_t* am = s_amax + parity * 4 * NT;
         float h[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float u = c & 1 ? acc[MATS - 1][c / 2].y : acc[MATS - 1][c / 2].x;
-          const float g = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
-          if (MATS == 2) {
-            h[c] = silu(g) * u;
-          } else {
-            const float v = u < 0.0f ? 0.0f : u;  // a NaN stays
-            h[c] = v * v;
-          }
-          if (row >= p.rows) h[c] = 0.0f;
-          if (c < mine && own(c)) {
+        for (int c = 0; c < NC; ++c)
+          if (in(c) && own(c)) {
+            const float u = c & 1 ? acc[MATS - 1][c / 2].y : acc[MATS - 1][c / 2].x;
+            const float g = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
+            if (MATS == 2) {
+              h[c] = silu(g) * u;
+            } else {
+              const float v = u < 0.0f ? 0.0f : u;  // a NaN stays
+              h[c] = v * v;
+            }
+            if (row >= p.rows) h[c] = 0.0f;
             const uint32_t a =
                 __reduce_max_sync(0xffffffffu, __float_as_uint(h[c]) & 0x7fffffffu);
-            if (lane == 0) am[quad * NT + c] = a;
+            if (lane == 0) am[quad * NT + col(c)] = a;
+          }
+        named_bar_sync(1 + half, 128);
+        float hs[(NC + 31) / 32], hr[(NC + 31) / 32];
+        bool plain = true;
+#pragma unroll
+        for (int i = 0; i < (NC + 31) / 32; ++i) {
+          const int c = 32 * i + lane;
+          hs[i] = hr[i] = 0.0f;
+          if (c < NC && in(c) && own(c)) {
+            const uint32_t* a = am + col(c);
+            const uint32_t top = max(max(a[0], a[NT]), max(a[2 * NT], a[3 * NT]));
+            hs[i] = block_scale(top);
+            hr[i] = __frcp_rn(hs[i]);
+            plain = plain && scale_divides(hs[i], top);
+            if (quad == 0) p.hs[t.rb * p.hs_pitch + t.row0 + col(c)] = hs[i];
           }
         }
-        named_bar_sync(1 + half, 128);
+        plain = __all_sync(0xffffffffu, plain);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          if (c < mine && own(c)) {
-            const float s = block_scale(
-                max(max(am[c], am[NT + c]), max(am[2 * NT + c], am[3 * NT + c])));
-            p.hq[(long)(tok0 + c) * p.h_pitch + row] = (uint8_t)e4m3_byte(__fdiv_rn(h[c], s));
-            if (r == 0) p.hs[t.rb * p.hs_pitch + tok0 + c] = s;
+          if (in(c) && own(c)) {
+            const float sc = __shfl_sync(0xffffffffu, hs[c / 32], c & 31);
+            const float rc = __shfl_sync(0xffffffffu, hr[c / 32], c & 31);
+            const float v = plain ? quotient(h[c], sc, rc) : __fdiv_rn(h[c], sc);
+            p.hq[(long)(t.row0 + col(c)) * p.h_pitch + row] = (uint8_t)e4m3_byte(v);
           }
       }
     }
