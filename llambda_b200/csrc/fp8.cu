@@ -98,7 +98,57 @@ struct F8Rows {
   const int *sel, *pos, *row_start;  // null: row t
   int* entry;                        // receives the entry of each grouped row
   int k, E;
+  // few entries: the quantiser groups them itself (no pos, no row_start) and
+  // its first CTA writes what the plan would have, and zeroes `clear` counters
+  int n, nt, nclear;
+  int4* tiles;
+  int *nchunks, *clear;
 };
+
+enum QuantMode { kQuantRows, kQuantGrouped, kQuantSelf };
+constexpr int kSelfEntries = 256;  // one a thread
+
+// Groups n <= kSelfEntries entries by expert as f8_plan_kernel does, in every
+// CTA for itself: entry i counts the entries of its expert before it and in
+// all, then the rows and chunks of the experts before its own.  row[i]: its
+// grouped row, -1 if its expert is outside [0, E).
+__device__ __forceinline__ void self_group(const F8Rows& r, int* s_e, int* s_count, int* s_row,
+                                           int* s_chunks) {
+  const int i = threadIdx.x;
+  int e = i < r.n ? __ldg(r.sel + i) : -1;
+  if (e >= r.E) e = -1;
+  s_e[i] = e;
+  if (i == 0) *s_chunks = 0;
+  __syncthreads();
+  int pos = 0, cnt = 0;
+  for (int j = 0; j < r.n; ++j) {
+    const bool same = s_e[j] == e;
+    pos += same && j < i;
+    cnt += same;
+  }
+  const bool first = e >= 0 && pos == 0;
+  s_count[i] = first ? cnt : 0;
+  __syncthreads();
+  int base = 0, chunk = 0;
+  for (int j = 0; j < r.n; ++j) {
+    const int c = s_e[j] < e ? s_count[j] : 0;
+    base += (c + 3) & ~3;
+    chunk += (c + r.nt - 1) / r.nt;
+  }
+  s_row[i] = e >= 0 ? base + pos : -1;
+  if (blockIdx.x == 0) {
+    if (e >= 0) r.entry[base + pos] = i;
+    if (first) {
+      const int ch = (cnt + r.nt - 1) / r.nt;
+      for (int c = 0; c < ch; ++c)
+        r.tiles[chunk + c] = make_int4(base + c * r.nt, min(r.nt, cnt - c * r.nt), e, 0);
+      atomicMax(s_chunks, chunk + ch);
+    }
+    for (int c = i; c < r.nclear; c += blockDim.x) r.clear[c] = 0;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && i == 0) *r.nchunks = *s_chunks;
+}
 
 constexpr int kQuantBlocks = 4;  // blocks of one token per warp
 
@@ -110,7 +160,7 @@ constexpr int kQuantBlocks = 4;  // blocks of one token per warp
 //
 // Bound by memory; the four blocks' scales are computed side by side on the
 // lanes, one division and one reciprocal for all.
-template <typename T, bool GROUPED>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, long ldx,
                                                        int tokens, int cols, uint8_t* q,
                                                        int q_pitch, float* scales, int s_pitch,
@@ -122,18 +172,20 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
   const unsigned per = (blocks + kQuantBlocks - 1) / kQuantBlocks;
   const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int t = (int)(unit / per), b0 = (int)(unit - t * per) * kQuantBlocks;
-  if (t >= (GROUPED ? tokens : s_pitch)) return;
   const bool mine = lane < kQuantBlocks && b0 + lane < blocks;  // this lane's scale exists
   float* sp = scales + (long)(b0 + lane) * s_pitch;
-  if (t >= tokens) {
-    if (mine) sp[t] = 0.0f;
+  if (MODE != kQuantSelf && t >= tokens) {
+    if (MODE == kQuantRows && t < s_pitch && mine) sp[t] = 0.0f;
     return;
   }
   const int c0 = b0 * kF8Block + 4 * lane;
   const T* src = x + t * ldx + c0;
   const bool whole = (b0 + kQuantBlocks) * kF8Block <= cols;
   float v[kQuantBlocks][4];
-  if (vec && whole) {
+  if (MODE == kQuantSelf && t >= tokens) {
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+  } else if (vec && whole) {
 #pragma unroll
     for (int i = 0; i < kQuantBlocks; ++i) load4(src + i * kF8Block, true, 4, v[i]);
   } else {
@@ -143,6 +195,13 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
       v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
       if (c < cols) load4(src + i * kF8Block, vec && c + 4 <= cols, cols - c, v[i]);
     }
+  }
+  __shared__ int s_e[MODE == kQuantSelf ? kSelfEntries : 1],
+      s_count[MODE == kQuantSelf ? kSelfEntries : 1], s_row[MODE == kQuantSelf ? kSelfEntries : 1],
+      s_chunks;
+  if (MODE == kQuantSelf) {  // while the loads are on their way
+    self_group(rows, s_e, s_count, s_row, &s_chunks);
+    if (t >= tokens) return;
   }
   uint32_t am = 0;  // lane i: the largest magnitude of block i
 #pragma unroll
@@ -193,8 +252,13 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
     }
     if (mine) sp[o] = s_own;
   };
-  if (!GROUPED) {
+  if (MODE == kQuantRows) {
     store(t);
+  } else if (MODE == kQuantSelf) {
+    for (int j = 0; j < rows.k; ++j) {
+      const int o = s_row[t * rows.k + j];
+      if (o >= 0) store(o);
+    }
   } else {
     for (int j0 = 0; j0 < rows.k; j0 += 32) {  // the entries' rows, one a lane
       const int id = t * rows.k + j0 + lane;
@@ -236,6 +300,12 @@ struct F8Pass {
   float* partial;                // kF8Partial: rows of partial by entry
   long ldp;
   const int* entry;
+  // kF8Partial with few entries: the last of a row block's CTAs to arrive at
+  // its counter adds up the block's columns of out (null: f8_combine_kernel does)
+  int* counters;
+  const int* sel;
+  const float* weights;
+  int k, E;
   int split;                     // CTAs of a cluster share a tile's K (1: no cluster)
   int early;                     // the weights and tiles are not the previous kernel's output
   int* status;
@@ -246,7 +316,7 @@ struct F8Sync {
   uint64_t sfull[kF8Scales], sempty[kF8Scales];
   uint64_t tfull[kF8MaxBuf], tempty[kF8MaxBuf], done;
   uint32_t tmem;
-  int abort;
+  int abort, last;
 };
 
 // Small tiles are bound by the weights' bytes: two CTAs a multiprocessor, so
@@ -348,6 +418,27 @@ __device__ __forceinline__ void f8_linger() {
 __device__ __forceinline__ bool f8_wait_warp(uint64_t* bar, uint32_t parity, int* status,
                                              volatile int* abort) {
   return __all_sync(0xffffffffu, f8_wait(bar, parity, status, abort));
+}
+
+__device__ __forceinline__ void store_out(void* out, int bf16, long i, float v) {
+  if (bf16)
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else
+    static_cast<float*>(out)[i] = v;
+}
+
+// One column of token t's weighted sum over its entries, in rank order; entries
+// whose expert is outside [0, E) add nothing.  partial: that column of entry 0.
+__device__ __forceinline__ float combine_column(const float* partial, long ldp, const int* sel,
+                                                int E, const float* weights, int t, int k) {
+  float a = 0.0f;
+#pragma unroll 8
+  for (int j = 0; j < k; ++j) {
+    const int e = sel[t * k + j];
+    if (e >= 0 && e < E)
+      a = fmaf(weights[t * k + j], __ldcg(partial + (long)(t * k + j) * ldp), a);
+  }
+  return a;
 }
 
 struct F8Tile {
@@ -557,6 +648,10 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     RingPos ap, sp;
     bool ok = true;
     int parity = 0;
+    if (MODE == kF8Partial && NT == 16 && p.counters && ntiles == 0)  // no entry is anyone's
+      for (long i = (long)blockIdx.x * kF8EpiWarps * 32 + threadIdx.x; i < (long)p.tokens * p.rows;
+           i += (long)gridDim.x * kF8EpiWarps * 32)
+        store_out(p.out, p.out_bf16, i / p.rows * p.ldo + i % p.rows, 0.0f);
     for (int tile = tile0; tile < ntiles && ok; tile += tstep, parity ^= 1) {
       const F8Tile t = f8_tile<NT>(p, tile);
       // this thread's tokens: groups of 8 columns in turn with the other half's,
@@ -679,11 +774,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
           for (int c = 0; c < NC; ++c)
             if (in(c) && own(c)) {
               const float y = c & 1 ? acc[0][c / 2].y : acc[0][c / 2].x;
-              const long o = (long)(t.row0 + col(c)) * p.ldo + row;
-              if (p.out_bf16)
-                static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(y);
-              else
-                static_cast<float*>(p.out)[o] = y;
+              store_out(p.out, p.out_bf16, (long)(t.row0 + col(c)) * p.ldo + row, y);
             }
         }
       } else if (MODE == kF8Partial) {
@@ -694,6 +785,21 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
             const long id = __shfl_sync(0xffffffffu, ent[c / 32], c & 31);
             if (row < p.rows) p.partial[id * p.ldp + row] = y;
           }
+        if (NT == 16 && p.counters) {
+          __threadfence();
+          named_bar_sync(3, kF8EpiWarps * 32);
+          if (threadIdx.x == 0)
+            sy->last = atomicAdd(p.counters + t.rb, 1) == ntiles / p.rblocks * split - 1;
+          named_bar_sync(3, kF8EpiWarps * 32);
+          if (sy->last) {
+            __threadfence();
+            const int c = t.rb * kF8M + (threadIdx.x & (kF8M - 1));
+            if (c < p.rows)
+              for (int tok = threadIdx.x / kF8M; tok < p.tokens; tok += kF8EpiWarps * 32 / kF8M)
+                store_out(p.out, p.out_bf16, tok * p.ldo + c,
+                          combine_column(p.partial + c, p.ldp, p.sel, p.E, p.weights, tok, p.k));
+          }
+        }
       } else {
         // the 128 rows of this tile are one block of the next product's K: its
         // scale per token is a maximum over the four warps of this half, and
@@ -1126,34 +1232,30 @@ __global__ void __launch_bounds__(1024) f8_plan_kernel(const int* __restrict__ s
   if (tid == 1023) *nchunks = s_warp[1][31];
 }
 
-// out[t] = sum over ranks j, in order, of weight * partial row; entries whose
-// expert is outside [0, E) add nothing.  Four columns a thread.
+// out[t] = sum over ranks j, in order, of weight * partial row.  Four columns a
+// thread.
 __global__ void __launch_bounds__(256) f8_combine_kernel(const float* partial, long ldp,
                                                          const int* sel, int E,
                                                          const float* weights, int k, int cols,
-                                                         void* out, long ldo,
-                                                         int out_bf16) {
+                                                         void* out, long ldo, int out_bf16) {
   griddep_wait();
   griddep_launch();
   const long t = blockIdx.x;
   for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int j = 0; j < k; ++j) {
       const int e = sel[t * k + j];
-      if (e < 0 || e >= E) continue;
-      const float w = weights[t * k + j];
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(partial + (t * k + j) * ldp + c));
-      a[0] = fmaf(w, v.x, a[0]), a[1] = fmaf(w, v.y, a[1]);
-      a[2] = fmaf(w, v.z, a[2]), a[3] = fmaf(w, v.w, a[3]);
+      if (e >= 0 && e < E) {
+        const float w = weights[t * k + j];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(partial + (t * k + j) * ldp + c));
+        a[0] = fmaf(w, v.x, a[0]), a[1] = fmaf(w, v.y, a[1]);
+        a[2] = fmaf(w, v.z, a[2]), a[3] = fmaf(w, v.w, a[3]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (c + i < cols) {
-        if (out_bf16)
-          static_cast<__nv_bfloat16*>(out)[t * ldo + c + i] = __float2bfloat16_rn(a[i]);
-        else
-          static_cast<float*>(out)[t * ldo + c + i] = a[i];
-      }
+      if (c + i < cols) store_out(out, out_bf16, t * ldo + c + i, a[i]);
   }
 }
 
@@ -1276,8 +1378,11 @@ cudaError_t quant_t(const T* x, long ldx, int tokens, int cols, uint8_t* q, long
   const int vec = ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
   const long per = (f8_blocks(cols) + kQuantBlocks - 1) / kQuantBlocks;
   const long ctas = ((rows.sel ? (long)tokens : s_pitch) * per + 7) / 8;
+  const bool self = rows.sel && !rows.pos;
   if (ctas > 0x0fffffffL) return cudaErrorInvalidValue;
-  auto kern = rows.sel ? f8_quant_kernel<T, true> : f8_quant_kernel<T, false>;
+  auto kern = self       ? f8_quant_kernel<T, kQuantSelf>
+              : rows.sel ? f8_quant_kernel<T, kQuantGrouped>
+                         : f8_quant_kernel<T, kQuantRows>;
   return launch_pdl(kern, dim3((unsigned)ctas), dim3(256), 0, st, x, ldx, tokens, cols, q,
                     (int)q_pitch, scales, (int)s_pitch, rows, vec);
 }
@@ -1353,6 +1458,7 @@ F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k) {
   L.entry = take((size_t)L.rows * 4);
   L.tiles = take((size_t)L.max_chunks * 16);
   L.nchunks = take(4);
+  L.counters = take((size_t)f8_blocks(m.down.rows) * 4);
   L.xq = take((size_t)L.rows * f8_pad16(m.up.cols));
   L.xs = take((size_t)f8_blocks(m.up.cols) * L.rows * 4);
   L.hq = take((size_t)L.rows * L.hp);
@@ -1378,10 +1484,23 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   // chunks of an expert's tokens: half again the average, so most experts take one
   const int nt = f8_chunk((3 * n / std::min<long>(n, m.up.experts) + 1) / 2);
   const long chunks = n / nt + std::min<long>(n, m.up.experts);
-  cudaError_t e = launch_pdl(f8_plan_kernel, dim3(1), dim3(1024), 0, st, sel, (int)n, m.up.experts,
-                             nt, pos, row_start, tiles, nchunks);
-  if (e != cudaSuccess) return e;
-  const F8Rows rows{sel, pos, row_start, entry, k, m.up.experts};
+  // A call so small that the down product has one tile a CTA at most takes three
+  // launches instead of five: the quantiser groups the entries, and the down
+  // product's CTAs add them up (one token, 10 of 512 experts: 27 us against 31).
+  // With more tiles the fence after each, and the weights that the plan's own
+  // launch lets the gate and up product request ahead, cost more (32 tokens, 6
+  // of 128 experts of 2688 x 1856: 215 us against 157).
+  const bool few = n <= kSelfEntries && nt == 16 &&
+                   chunks * f8_blocks(m.down.rows) <= (long)sm_count() * F8Cfg<16, 1>::kCtas;
+  int* counters = few ? reinterpret_cast<int*>(base + L.counters) : nullptr;
+  cudaError_t e = cudaSuccess;
+  if (!few) {
+    e = launch_pdl(f8_plan_kernel, dim3(1), dim3(1024), 0, st, sel, (int)n, m.up.experts, nt, pos,
+                   row_start, tiles, nchunks);
+    if (e != cudaSuccess) return e;
+  }
+  const F8Rows rows{sel, few ? nullptr : pos, row_start, entry, k, m.up.experts, (int)n, nt,
+                    few ? f8_blocks(m.down.rows) : 0, tiles, nchunks, counters};
   e = quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
             reinterpret_cast<float*>(base + L.xs), L.rows, rows, st);
   if (e != cudaSuccess) return e;
@@ -1404,7 +1523,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   p.h_pitch = L.hp;
   p.hs = reinterpret_cast<float*>(base + L.hs);
   p.hs_pitch = L.rows;
-  p.early = 1;
+  p.early = !few;  // the quantiser writes the tiles when it groups the entries
   p.status = status;
   e = m.gate.data ? launch_f8_pass<2, kF8Act>(nt, maps, p, chunks * p.rblocks, st)
                   : launch_f8_pass<1, kF8Act>(nt, maps, p, chunks * p.rblocks, st);
@@ -1424,10 +1543,19 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   d.partial = partial;
   d.ldp = L.ldp;
   d.entry = entry;
+  d.counters = counters;
+  d.sel = sel;
+  d.weights = weights;
+  d.k = k;
+  d.E = m.up.experts;
+  d.tokens = tokens;
+  d.out = out;
+  d.ldo = ldo;
+  d.out_bf16 = out_bf16;
   d.early = 1;
   d.status = status;
   e = launch_f8_pass<1, kF8Partial>(nt, maps, d, chunks * d.rblocks, st);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || few) return e;
   const unsigned gy = (unsigned)std::max(1, std::min((m.down.rows + 1023) / 1024, 64));
   return launch_pdl(f8_combine_kernel, dim3((unsigned)tokens, gy), dim3(256), 0, st, partial,
                     L.ldp, sel, m.up.experts, weights, k, m.down.rows, out, ldo, (int)out_bf16);

@@ -316,7 +316,7 @@ struct F8Moe {
 // Workspace of one call of the routed experts.
 struct F8MoeLayout {
   long rows, max_chunks, hp, ldp;
-  size_t pos, row_start, entry, tiles, nchunks, xq, xs, hq, hs, partial, bytes;
+  size_t pos, row_start, entry, tiles, nchunks, counters, xq, xs, hq, hs, partial, bytes;
 };
 
 inline long f8_pad16(long n) { return (n + 15) & ~15L; }
