@@ -90,25 +90,6 @@ __device__ __forceinline__ float choice_error(const RouteParams& r, float c, flo
   return (r.softmax ? 8e-6f * smax : 1e-6f) + 2.5e-7f * fabsf(c);
 }
 
-// A lane's two largest keys of those whose bit in `out` is clear, with their
-// places; equal keys in order of place.
-template <int R, typename K>
-__device__ __forceinline__ void two_largest(const K (&key)[R], uint32_t out, K& a, int& ai, K& b,
-                                            int& bi) {
-  a = b = 0;
-  ai = bi = 0;
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const K v = out >> j & 1u ? K(0) : key[j];
-    if (v > a) {
-      b = a, bi = ai;
-      a = v, ai = j;
-    } else if (v > b) {
-      b = v, bi = j;
-    }
-  }
-}
-
 // The choice of one token by one warp: lane L holds experts L * R .. L * R +
 // R - 1, so equal keys go to the lowest lane that has one, and to its lowest j.
 // Rank i's expert goes to lane i (and that of rank top_k, if there is such a
@@ -117,14 +98,18 @@ __device__ __forceinline__ void two_largest(const K (&key)[R], uint32_t out, K& 
 // was (by_logit: the compared values are exact).
 //
 // Each round takes the warp's largest key, one reduction over the lanes' own
-// largest.  A lane keeps its two largest and looks for more only when both are
-// gone.  At 8191 tokens, 256 experts in 8 groups, top 8, the search through all
-// of a lane's keys in every round took 27 us.
+// largest.  A lane knows its two largest; the keys themselves are in shared
+// memory (`keys`, R + 1 a lane), where the whole warp looks for the place of the
+// one taken among its lane's, and for that lane's next two when both are gone.
+// At 8191 tokens, 256 experts in 8 groups, top 8: 27 us with the keys in
+// registers and each lane looking through its own in every round, 20 looking
+// only when both are gone, 18 so.
 template <int R, typename F>
 __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R], const float* bias,
-                                       bool by_logit, float m, F z, int lane, int& sel,
-                                       bool& tied) {
+                                       bool by_logit, float m, F z, int lane, void* shared,
+                                       int& sel, bool& tied) {
   using K = decltype(order_key(F(0)));
+  K* keys = static_cast<K*>(shared);
   const bool check = sizeof(F) == 4 && !by_logit;
   const float smax = r.softmax ? 1.0f / (float)z : 1.0f;
   K key[R];
@@ -136,7 +121,6 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R]
                             : order_key(choice(r, bias, l[j], m, z, e));
   }
   bool sure = true;
-  uint32_t out = 0;  // this lane's experts that are out
   if (r.top_groups < r.groups) {
     const int size = r.experts / r.groups, span = size / R;
     K g1 = 0, g2 = 0;  // lane g: group g's two largest
@@ -191,32 +175,46 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R]
     int g = lane * R / size, left = (g + 1) * size - lane * R;  // experts left in group g
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (!(kept >> (g & 31) & 1u)) out |= 1u << j;
+      if (!(kept >> (g & 31) & 1u)) key[j] = 0;
       if (--left == 0) ++g, left = size;
     }
   }
-  K a, b, mine = 0, next = 0;  // mine: rank `lane`'s key; next: that of rank top_k
-  int ai, bi;
-  two_largest<R>(key, out, a, ai, b, bi);
+  K a = 0, b = 0, mine = 0, next = 0;  // mine: rank `lane`'s key; next: that of rank top_k
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    b = max(b, min(a, key[j]));
+    a = max(a, key[j]);
+    keys[lane * (R + 1) + j] = key[j];
+  }
+  __syncwarp();
   for (int i = 0; i <= r.top_k; ++i) {
     if (i == r.top_k && !check) break;
     const K best = warp_max(a);
     if (best == 0) break;  // no expert left to compare with
     const int owner = __ffs(__ballot_sync(kFull, a == best)) - 1;
-    const int e = __shfl_sync(kFull, lane * R + ai, owner);
+    // lane j: the owner's key j
+    K v = lane < R ? keys[owner * (R + 1) + lane] : K(0);
+    const int at = __ffs(__ballot_sync(kFull, v == best)) - 1;
+    const int e = owner * R + at;
     if (i == r.top_k) {
       next = best;
       if (lane == r.top_k) sel = e;  // compared with rank top_k - 1 below
-    } else if (lane == i) {
-      sel = e, mine = best;
+      break;
     }
-    bool dry = false;
-    if (lane == owner) {
-      out |= 1u << ai;
-      a = b, ai = bi, b = 0;
-      dry = a == 0;
+    if (lane == i) sel = e, mine = best;
+    if (lane == at) {
+      keys[owner * (R + 1) + at] = 0;
+      v = 0;
     }
-    if (R > 2 && __any_sync(kFull, dry)) two_largest<R>(key, out, a, ai, b, bi);
+    const bool held = lane == owner;
+    if (held) a = b, b = 0;
+    if (R > 2 && __any_sync(kFull, held && a == 0)) {
+      const K first = warp_max(v);
+      const int one = __ffs(__ballot_sync(kFull, v == first)) - 1;
+      const K second = warp_max(lane == one ? K(0) : v);
+      if (held) a = first, b = second;
+    }
+    __syncwarp();
   }
   if (check) {
     K after = __shfl_down_sync(kFull, mine, 1);
@@ -271,9 +269,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     route_kernel(const RouteParams r, const T* __restrict__ logits, long ld,
                  const float* __restrict__ bias, int tokens, int* __restrict__ selected,
                  float* __restrict__ weights, int vec) {
+  __shared__ unsigned long long s_keys[kRouteWarps][32 * (R + 1)];
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
+  void* shared = s_keys[threadIdx.x >> 5];
   const long t = (long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
   if (t >= tokens) return;
   const T* row = logits + t * ld;
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
   }
   int sel = 0;
   bool tied = false;
-  bool sure = choose<R, float>(r, l, bias, by_logit, m, z, lane, sel, tied);
+  bool sure = choose<R, float>(r, l, bias, by_logit, m, z, lane, shared, sel, tied);
   if (__any_sync(kFull, tied)) {
     // equal logits and biases are a true tie, which the index has decided
     const float lv = logit_at(row, sel), bv = bias ? __ldg(bias + sel) : 0.0f;
@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) zd += __shfl_xor_sync(kFull, zd, o);
     }
-    choose<R, double>(r, l, bias, false, m, zd, lane, sel, tied);
+    __syncwarp();
+    choose<R, double>(r, l, bias, false, m, zd, lane, shared, sel, tied);
   }
   // lane i: the weight of rank i
   float s = 0.0f;
