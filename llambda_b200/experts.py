@@ -27,27 +27,35 @@ BLOCK = 128  # columns (and weight rows) per scale
 
 
 # A one-token call is a few microseconds of GPU time, so what a call does on the
-# host is kept short: torch is looked up once, the entry points are bound once,
-# and the current stream is read as a raw handle where torch offers that.
-_t = None
+# host is kept short: torch, its types, the library and the lookup of the current
+# stream are bound once, by the first call that needs them.
+_t = _lib = _raw_stream = None
+_FLOATS = _FP8 = _INT = _F32 = ()
 
 
 def _torch():
-    global _t
+    global _t, _raw_stream, _FLOATS, _FP8, _INT, _F32
     if _t is None:
         import torch
+        _FLOATS = (torch.float32, torch.bfloat16)
+        _FP8 = (torch.float8_e4m3fn, torch.uint8)
+        _INT, _F32 = (torch.int32,), (torch.float32,)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda index: torch.cuda.current_stream(index).cuda_stream)
         _t = torch
     return _t
 
 
-@functools.lru_cache(maxsize=None)
-def _entry(name: str):
-    return getattr(N.lib(), name)
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = N.lib()
+    return _lib
 
 
-def _call(name: str, *args) -> None:
-    if _entry(name)(*args) != 0:
-        raise N.LlambdaCudaError(N.last_error() or f"{name} failed")
+def _check(status: int) -> None:
+    if status != 0:
+        raise N.LlambdaCudaError(N.last_error() or "the call failed")
 
 
 def _blocks(n: int) -> int:
@@ -93,41 +101,27 @@ def _device_tensor(t, name: str, dtypes, shape, device=None, contiguous=False):
 
 def _matrix(t, name: str, cols=None, device=None):
     """Checks a float32 or bfloat16 operand [tokens][cols]; its (rows, columns, row stride)."""
+    if _t is None:
+        _torch()
     try:
-        shape = t.shape
-        rows, want = shape if cols is None else (shape[0], cols)
-    except (AttributeError, ValueError, IndexError, TypeError):
-        rows, want = None, cols
-    _device_tensor(t, name, _FLOATS or _floats(), (rows, want), device)
-    return rows, want, t.stride(0) if rows > 1 else want
-
-
-_FLOATS = ()
-
-
-def _floats():
-    global _FLOATS
-    torch = _torch()
-    _FLOATS = (torch.float32, torch.bfloat16)
-    return _FLOATS
+        rows, width = t.shape
+    except (AttributeError, ValueError, TypeError):
+        rows = width = None
+    if cols is None:
+        cols = width
+    _device_tensor(t, name, _FLOATS, (rows, cols), device)
+    return rows, cols, t.stride(0) if rows > 1 else cols
 
 
 def _tag(dtype) -> int:
     return N.TYPE_F32 if dtype is _FLOATS[0] else N.TYPE_BF16
 
 
-@functools.lru_cache(maxsize=None)
-def _raw_stream():
-    torch = _torch()
-    return getattr(torch._C, "_cuda_getCurrentRawStream",
-                   lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 def _on(stream, device, allocate):
     """(raw handle of the call's stream, allocate()'s result with that stream
     current, so that what the call allocates belongs to it)."""
     if stream is None:
-        return _raw_stream()(device.index), allocate()
+        return _raw_stream(device.index), allocate()
     torch = _torch()
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
@@ -181,14 +175,14 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
     T, E, ld = _matrix(logits, "logits")
     dev = logits.device
     if bias is not None:
-        _device_tensor(bias, "bias", (_t.float32,), (E,), dev)
+        _device_tensor(bias, "bias", _F32, (E,), dev)
     desc = _route_desc(E, top_k, score, groups, top_groups, group_top, renormalise, weight_scale)
     raw, (selected, weights) = _on(stream, dev, lambda: (
         _t.empty((T, top_k), dtype=_t.int32, device=dev),
         _t.empty((T, top_k), dtype=_t.float32, device=dev)))
-    _call("llambda_cuda_route_device", desc, _tag(logits.dtype), logits.data_ptr(), ld,
+    _check((_lib or _library()).llambda_cuda_route_device(desc, _tag(logits.dtype), logits.data_ptr(), ld,
           bias.data_ptr() if bias is not None else None, T, selected.data_ptr(),
-          weights.data_ptr(), raw)
+          weights.data_ptr(), raw))
     return selected, weights
 
 
@@ -203,9 +197,9 @@ def _route_host(logits, bias, desc):
             raise ValueError(f"bias must have shape ({E},)")
     T = logits.shape[0]
     selected, weights = np.empty((T, k), np.int32), np.empty((T, k), np.float32)
-    _call("llambda_cuda_route", desc, logits.ctypes.data,
+    _check((_lib or _library()).llambda_cuda_route(desc, logits.ctypes.data,
           bias.ctypes.data if bias is not None else None, T, selected.ctypes.data,
-          weights.ctypes.data)
+          weights.ctypes.data))
     return selected, weights
 
 
@@ -223,8 +217,8 @@ def fp8_quantize(x, *, stream=None):
     raw, (q, scales) = _on(stream, dev, lambda: (
         _t.empty((T, _pad(cols, 16)), dtype=_t.float8_e4m3fn, device=dev),
         _t.empty((_blocks(cols), _pad(T, 4)), dtype=_t.float32, device=dev)))
-    _call("llambda_cuda_fp8_quantize_device", _tag(x.dtype), x.data_ptr(), ldx, T, cols,
-          q.data_ptr(), scales.data_ptr(), raw)
+    _check((_lib or _library()).llambda_cuda_fp8_quantize_device(_tag(x.dtype), x.data_ptr(), ldx, T, cols,
+          q.data_ptr(), scales.data_ptr(), raw))
     return q, scales
 
 
@@ -301,7 +295,7 @@ class Fp8ProjectionSession(_Fp8Session):
     def _create(cls, w, s, data, scales, on_device, device, keep):
         h = C.c_void_p()
         t = _fp8_tensor(w.shape, data, scales)
-        _call("llambda_cuda_fp8_session_create", C.byref(t), on_device, C.byref(h))
+        _check((_lib or _library()).llambda_cuda_fp8_session_create(C.byref(t), on_device, C.byref(h)))
         return cls(h, w.shape[0], w.shape[1], device, keep)
 
     @classmethod
@@ -329,8 +323,8 @@ class Fp8ProjectionSession(_Fp8Session):
         if x.ndim != 2 or x.shape[1] != self.cols or not x.size:
             raise ValueError(f"x must be [tokens][{self.cols}]")
         out = np.empty((x.shape[0], self.rows), np.float32)
-        _call("llambda_cuda_fp8_session_run", self._handle(), x.ctypes.data, x.shape[0],
-                                                      out.ctypes.data)
+        _check((_lib or _library()).llambda_cuda_fp8_session_run(self._handle(), x.ctypes.data, x.shape[0],
+                                                      out.ctypes.data))
         return out[0] if one else out
 
     def run_device(self, x, out=None, *, out_dtype=None, stream=None):
@@ -339,19 +333,18 @@ class Fp8ProjectionSession(_Fp8Session):
         h = self._handle()
         T, _, ldx = _matrix(x, "x", self.cols, self.device)
         dev = x.device
-        nbytes = _entry("llambda_cuda_fp8_session_workspace")(h, T)
+        nbytes = (_lib or _library()).llambda_cuda_fp8_session_workspace(h, T)
         raw, ((out, ldo), work) = _on(stream, dev, lambda: (
             _out(out, T, self.rows, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev)))
-        _call("llambda_cuda_fp8_session_run_device", h, _tag(x.dtype), x.data_ptr(), ldx, T,
-              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr(), nbytes, raw)
+        _check((_lib or _library()).llambda_cuda_fp8_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T,
+              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr(), nbytes, raw))
         return out
 
     def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):
         """As run_device over what fp8_quantize returned for `tokens` rows of
         `cols` columns (several projections of one input quantise it once)."""
         torch = _torch()
-        _floats()
         h = self._handle()
         _device_tensor(q, "q", (torch.float8_e4m3fn, torch.uint8), (tokens, _pad(self.cols, 16)),
                        self.device, contiguous=True)
@@ -359,8 +352,8 @@ class Fp8ProjectionSession(_Fp8Session):
                        q.device, contiguous=True)
         raw, (out, ldo) = _on(stream, q.device, lambda: _out(
             out, tokens, self.rows, out_dtype or torch.float32, q.device))
-        _call("llambda_cuda_fp8_session_run_quantized", h, q.data_ptr(), scales.data_ptr(), tokens,
-              _tag(out.dtype), out.data_ptr(), ldo, raw)
+        _check((_lib or _library()).llambda_cuda_fp8_session_run_quantized(h, q.data_ptr(), scales.data_ptr(), tokens,
+              _tag(out.dtype), out.data_ptr(), ldo, raw))
         return out
 
 
@@ -383,8 +376,7 @@ class Fp8MoeSession(_Fp8Session):
         ts = [_fp8_tensor(p[0].shape, ptr(p[0]), ptr(p[1])) if p is not None
               else N.Fp8Tensor(0, 0, 0, None, None) for p in (gate, up, down)]
         h = C.c_void_p()
-        _call("llambda_cuda_fp8_moe_session_create",
-            C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h))
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_create(C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h)))
         E, _, H = up[0].shape
         return cls(h, E, H, down[0].shape[1], device, (up, down, gate) if on_device else None)
 
@@ -417,9 +409,8 @@ class Fp8MoeSession(_Fp8Session):
                 or weights.shape != selected.shape:
             raise ValueError("selected and weights must both be [tokens][k]")
         out = np.empty((x.shape[0], self.out_features), np.float32)
-        _call("llambda_cuda_fp8_moe_session_run",
-            self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
-            weights.ctypes.data, out.ctypes.data)
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run(self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
+            weights.ctypes.data, out.ctypes.data))
         return out
 
     def run_device(self, x, selected, weights, out=None, *, out_dtype=None, stream=None):
@@ -431,13 +422,13 @@ class Fp8MoeSession(_Fp8Session):
         T, _, ldx = _matrix(x, "x", self.hidden, self.device)
         dev = x.device
         k = selected.shape[1] if getattr(selected, "ndim", 0) == 2 else None
-        _device_tensor(selected, "selected", (_t.int32,), (T, k), dev, contiguous=True)
-        _device_tensor(weights, "weights", (_t.float32,), (T, k), dev, contiguous=True)
-        nbytes = _entry("llambda_cuda_fp8_moe_session_workspace")(h, T, k)
+        _device_tensor(selected, "selected", _INT, (T, k), dev, contiguous=True)
+        _device_tensor(weights, "weights", _F32, (T, k), dev, contiguous=True)
+        nbytes = (_lib or _library()).llambda_cuda_fp8_moe_session_workspace(h, T, k)
         raw, ((out, ldo), work) = _on(stream, dev, lambda: (
             _out(out, T, self.out_features, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev)))
-        _call("llambda_cuda_fp8_moe_session_run_device", h, _tag(x.dtype), x.data_ptr(), ldx, T, k,
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T, k,
               selected.data_ptr(), weights.data_ptr(), _tag(out.dtype), out.data_ptr(), ldo,
-              work.data_ptr(), nbytes, raw)
+              work.data_ptr(), nbytes, raw))
         return out
