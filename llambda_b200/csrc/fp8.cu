@@ -33,7 +33,8 @@ constexpr int kF8EpiWarps = 8;    // two warpgroups, half of the tokens each
 constexpr int kF8Threads = (kF8EpiWarps + 3) * 32;
 constexpr int kF8Scales = 8;      // ring of staged activation scales
 constexpr int kF8MaxBuf = 4;      // ring of accumulators in tensor memory
-constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K
+constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K,
+constexpr int kF8SplitBlocks = 3; // with at least this many blocks each
 
 enum F8Mode {
   kF8Out,      // y to out (fp32 or bf16)
@@ -353,7 +354,7 @@ struct F8Sync {
 // shared memory for one.
 template <int NT, int MATS>
 struct F8Cfg {
-  static constexpr int kCtas = NT <= 32 || (NT == 64 && MATS == 1) ? 2 : 1;
+  static constexpr int kCtas = NT == 64 && MATS == 2 ? 1 : 2;
   static constexpr uint32_t kBudget = (kCtas == 2 ? 104u : 200u) * 1024u;
   static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
   static constexpr uint32_t kStage = MATS * kA + NT * kF8Block;
@@ -720,9 +721,8 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         const float* sc = s_scale + sp.s * NT;
         // columns loaded together, as many as the registers hold: the loads of a
         // second group wait for the first
-        constexpr int CH = MATS == 2 && NT == 128 ? 8
-                           : C::kCtas == 2        ? (NC < 16 / MATS ? NC : 16 / MATS)
-                                                  : (NC < 64 / MATS ? NC : 64 / MATS);
+        constexpr int CH = C::kCtas == 2 ? (NC < 16 / MATS ? NC : 16 / MATS)
+                                         : (NC < 64 / MATS ? NC : 64 / MATS);
 #pragma unroll
         for (int c0 = 0; c0 < NC; c0 += CH) {
           if (in(c0)) {  // warp-uniform
@@ -900,9 +900,9 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
 // weight rows [128 r, 128 r + 128) of the tile, 32 KB a block of K; the pair's
 // MMA reads both and leaves 128 tokens x 256 columns of fp32 sums in each CTA's
 // tensor memory, twice, so that a block's MMAs run while the one before is
-// added up.  What bounds the unpaired 128 x 128 form is the way from L2: it
-// reads 32 KB for a quarter of the products (2048 tokens by 14336 x 4096:
-// 264 us; pairs __BIG__ us).
+// added up.  What bounds small tiles of many tokens is the way from L2: one of
+// 128 x 64 reads 24 KB a block for an eighth of a pair's products (2048 tokens by
+// 14336 x 8192: 453 us in small tiles, 244 in pairs).
 //
 // Here M is the tokens' side: a thread of the epilogue has one token and 64
 // columns of one weight block, so a block of K has one factor a thread and 32
@@ -1351,20 +1351,21 @@ cudaError_t f8_allow_smem(const void* kern, size_t bytes) {
   return e;
 }
 
-// tiles: an upper bound.  Where they leave CTAs idle, clusters share a tile's K
-// as long as the CTAs stay resident together and each has about two blocks
-// (one token by 14336 x 4096: 17.0 us unsplit, __SPLIT__ in two).
+// tiles: an upper bound.  Where they leave multiprocessors idle, clusters share
+// a tile's K as long as every CTA has one to itself and a few blocks of K.  One
+// token, cold: 512 rows of 8192 columns 22.5 us unsplit, 12.6 in eight; 4096 of
+// 4096 17.3, 14.5 in four; 2688 of 1856 12.5, 12.3 in four; 14336 of 4096 (112
+// tiles) 22.5 unsplit, and with 24 tokens 22.6 against 26.7 in two.
 template <int NT, int MATS, int MODE>
 cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_t s) {
   using C = F8Cfg<NT, MATS>;
   const long slots = (long)sm_count() * C::kCtas;
   p.split = 1;
-  if (NT <= 64)
-    while (p.split < kF8MaxSplit && tiles * p.split * 2 <= slots && p.split * 2 <= (p.kblocks + 1) / 2)
-      p.split *= 2;
-  auto kern = f8_gemm_kernel<NT, MATS, MODE, false>;
-  if constexpr (NT <= 64)
-    if (p.split > 1) kern = f8_gemm_kernel<NT, MATS, MODE, true>;
+  while (p.split < kF8MaxSplit && tiles * p.split * 2 <= sm_count() &&
+         p.split * 2 * kF8SplitBlocks <= p.kblocks)
+    p.split *= 2;
+  auto kern = p.split > 1 ? f8_gemm_kernel<NT, MATS, MODE, true>
+                          : f8_gemm_kernel<NT, MATS, MODE, false>;
   const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -1389,15 +1390,15 @@ cudaError_t launch_f8_pass(int nt, const F8Maps& maps, const F8Pass& p, long til
   switch (nt) {
     case 16: return launch_f8_gemm<16, MATS, MODE>(maps, p, tiles, s);
     case 32: return launch_f8_gemm<32, MATS, MODE>(maps, p, tiles, s);
-    case 64: return launch_f8_gemm<64, MATS, MODE>(maps, p, tiles, s);
-    default: return launch_f8_gemm<128, MATS, MODE>(maps, p, tiles, s);
+    default: return launch_f8_gemm<64, MATS, MODE>(maps, p, tiles, s);
   }
 }
 
-// More tokens than this take the pairs' tiles of 256.
-constexpr int kF8BigTokens = 128;
-
-int f8_chunk(long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows of x in a tile of the small kind: as few columns as hold the tokens, 64
+// at most.  (Columns of 128 leave the weights half as many trips from L2, but
+// one CTA a multiprocessor instead of two: 2048 tokens, 2 of 8 experts of 2048 x
+// 1856 with gate 240 us, in 64 159; 128 tokens by 2688 x 8192 41 us and 31.)
+int f8_chunk(long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 int f8_blocks(long n) { return (int)((n + kF8Block - 1) / kF8Block); }
 
@@ -1446,8 +1447,14 @@ cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* 
                               bool out_bf16, void* out, long ldo, bool after_quant, int* status,
                               cudaStream_t st) {
   F8Maps maps;
-  const bool big = tokens > kF8BigTokens;
-  const int nt = big ? kF8M : f8_chunk(tokens);
+  // Pairs where the small tiles would come in several rounds.  Small and pairs:
+  // 256 tokens by 4096 x 8192 (128 small tiles) 38 and 41 us, 512 by 1024 x 8192
+  // (64) 34 and 41, by 2688 x 8192 (168) 49 and 44, by 14336 x 8192 (896) 145
+  // and 80.
+  const int nt_small = f8_chunk(tokens);
+  const bool big = tokens > nt_small && (long)f8_blocks(w.rows) *
+                                                ((tokens + nt_small - 1) / nt_small) > sm_count();
+  const int nt = big ? kF8M : nt_small;
   maps.w0 = maps.w1 = w.map;
   if (!f8_rows_map(&maps.x, q, f8_pad16(w.cols), tokens, w.cols, nt)) return cudaErrorInvalidValue;
   F8Pass p{};

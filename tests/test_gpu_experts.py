@@ -188,6 +188,25 @@ def test_quantize(dtype, T, K):
     assert not q[:, K:].float().any() and not s[:, T:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_every_magnitude(dtype):
+    """Blocks from below the smallest scale to the largest number, and values that are exact
+    ties of the type at their scale: the quotient has to be the correctly rounded one."""
+    g = gen(6)
+    e = torch.arange(-149, 128, device="cuda", dtype=torch.float64)
+    x = torch.rand(e.numel(), 384, generator=g, device="cuda").double() * 2 - 1
+    x = (x * torch.exp2(e)[:, None]).clamp(-3e38, 3e38)
+    # a power of two times 448 as the block's largest: every quotient is exact, many are ties
+    ties = torch.randint(0, 449 * 16, (e.numel(), 128), generator=g, device="cuda").double() / 16
+    ties[:, 0] = 448
+    x[:, 128:256] = (ties * torch.exp2(e)[:, None]).clamp(-3e38, 3e38)
+    x = x.float().to(dtype)
+    q, s = LB.fp8_quantize(x)
+    rq, rs = quantize_reference(x)
+    assert torch.equal(s[:, :x.shape[0]].double(), rs.t())
+    assert torch.equal(q.double(), rq.flatten(1))
+
+
 def test_quantize_strides_and_special_values():
     g = gen(5)
     wide = randn(g, 40, 300)
@@ -244,7 +263,8 @@ def check(out, y, bound):
 
 SIZES = [(1, 1, 16), (1, 300, 400), (2, 128, 128), (5, 64, 112), (16, 130, 1040), (17, 257, 144),
          (33, 2688, 1856), (64, 128, 2064), (65, 96, 256), (129, 384, 384), (300, 200, 640),
-         (513, 1030, 272), (1, 4096, 4096), (31, 4096, 8192)]
+         (513, 1030, 272), (1, 4096, 4096), (31, 4096, 8192), (48, 200, 4112), (100, 128, 4096),
+         (127, 2700, 528), (300, 20000, 272), (257, 19000, 144), (1025, 5000, 400)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -401,7 +421,9 @@ def experts_reference(x, sel, wt, up, down, gate):
 @pytest.mark.parametrize("T,E,k,H,I,O", [
     (1, 1, 1, 16, 16, 16), (1, 8, 4, 256, 128, 256), (3, 5, 5, 144, 80, 100),
     (9, 16, 3, 128, 192, 128), (40, 4, 2, 160, 144, 160), (70, 2, 2, 64, 272, 65),
-    (200, 1, 1, 128, 128, 130), (1, 4, 2, 2688, 1856, 2688)])
+    (200, 1, 1, 128, 128, 130), (1, 4, 2, 2688, 1856, 2688), (60, 4, 2, 96, 144, 128),
+    (40, 2, 1, 1024, 640, 512), (60, 2, 1, 1040, 528, 528), (2, 64, 40, 64, 128, 64),
+    (10, 64, 40, 128, 64, 80), (300, 2, 1, 256, 256, 1000)])
 def test_experts(dtype, gated, T, E, k, H, I, O):
     g = gen(T * 7 + H)
     x = randn(g, T, H).to(dtype)
@@ -444,6 +466,85 @@ def test_experts_do_not_depend_on_the_batch():
     got = m.run_device(x, one, wt)
     for t in (0, 149):
         assert torch.equal(m.run_device(x[t:t + 1], one[t:t + 1], wt[t:t + 1])[0], got[t])
+
+
+def test_experts_keep_special_values_to_their_token():
+    g = gen(23)
+    E, k, H, I, T = 4, 2, 160, 144, 30
+    up, down, gate = matrices(g, E, I, H), matrices(g, E, H, I), matrices(g, E, I, H)
+    sel = torch.randint(0, E, (T, k), generator=g, device="cuda").int()
+    x, wt = randn(g, T, H), randn(g, T, k)
+    for gated in (gate, None):
+        m = LB.Fp8MoeSession.from_device(up=up, down=down, gate=gated)
+        want = m.run_device(x, sel, wt)
+        bad = x.clone()
+        bad[3, 5], bad[7, 100], bad[11] = float("nan"), float("inf"), 0.0
+        out = m.run_device(bad, sel, wt)
+        assert out[3].isnan().all() and out[7].isnan().any() and not out[11].any()
+        rest = [t for t in range(T) if t not in (3, 7, 11)]
+        assert torch.equal(out[rest], want[rest])
+
+
+def test_experts_without_any_entry_give_zeros():
+    g = gen(24)
+    up, down = matrices(g, 3, 64, 32), matrices(g, 3, 40, 64)
+    m = LB.Fp8MoeSession.from_device(up=up, down=down)
+    for T, k in ((1, 1), (5, 2), (300, 4)):
+        x, wt = randn(g, T, 32), randn(g, T, k)
+        sel = torch.full((T, k), -7, dtype=torch.int32, device="cuda")
+        big = torch.full((T + 2, 50), 9.0, device="cuda")
+        m.run_device(x, sel, wt, out=big[1:1 + T, 3:43])
+        assert not big[1:1 + T, 3:43].any()
+        big[1:1 + T, 3:43] = 9.0
+        assert bool((big == 9.0).all())
+        sel[T - 1, 0] = 2  # one entry only: the last token's
+        out = m.run_device(x, sel, wt)
+        y, bound = experts_reference(x, sel, wt, up, down, None)
+        check(out, y, bound)
+
+
+def test_experts_views_leave_the_rest_alone():
+    g = gen(25)
+    up, down = matrices(g, 6, 128, 96), matrices(g, 6, 112, 128)
+    m = LB.Fp8MoeSession.from_device(up=up, down=down)
+    wide = randn(g, 400, 200)
+    for T in (1, 30, 390):
+        x = wide[3:3 + T, 7:103]
+        sel = torch.randint(0, 6, (T, 2), generator=g, device="cuda").int()
+        wt = randn(g, T, 2)
+        want = m.run_device(x.contiguous(), sel, wt)
+        big = torch.full((T + 5, 301), 4.0, device="cuda")
+        m.run_device(x, sel, wt, out=big[2:2 + T, 5:117])
+        assert torch.equal(big[2:2 + T, 5:117], want)
+        big[2:2 + T, 5:117] = 4.0
+        assert bool((big == 4.0).all())
+
+
+def test_offsets_past_32_bits():
+    """Rows of x and of out that start more than 2^31 elements in."""
+    g = gen(26)
+    N, K, T = 65536, 128, 40000
+    w, s = matrices(g, N, K)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    x = randn(g, T, K).to(torch.bfloat16)
+    out = p.run_device(x)
+    assert out.numel() > 2 ** 31
+    rows = torch.tensor([0, 32767, 32768, 39999], device="cuda")
+    y, bound = product_reference(*quantize_reference(x[rows]), w, s)
+    check(out[rows], y, bound)
+    del out
+    wide = torch.empty(9000, 262144, dtype=torch.bfloat16, device="cuda")
+    assert wide.numel() > 2 ** 31
+    wide[:, 70:70 + K] = x[:9000]
+    view = wide[:, 70:70 + K]
+    assert torch.equal(p.run_device(view[8900:]), p.run_device(x[8900:9000].contiguous()))
+    q, sc = LB.fp8_quantize(view)
+    q2, sc2 = LB.fp8_quantize(x[:9000].contiguous())
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(sc, sc2)
+    wide[:, 70:70 + K] = randn(g, 9000, K).to(torch.bfloat16)
+    sel, wt = LB.route_experts(view, 4)
+    sel2, wt2 = LB.route_experts(view.contiguous(), 4)
+    assert torch.equal(sel, sel2) and torch.equal(wt, wt2)
 
 
 def test_experts_refusals():
