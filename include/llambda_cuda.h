@@ -462,8 +462,8 @@ LLAMBDA_CUDA_API int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tens
 LLAMBDA_CUDA_API void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session* session);
 
 /* Host buffers: out [tokens][ne1] = W . x[t], x [tokens][ne0] quantised as by
- * llambda_cuda_fp8_quantize_device; products of a block summed exactly enough
- * for fp32, blocks added in fp32. */
+ * llambda_cuda_fp8_quantize_device; exact products, the sums of a block and of
+ * the blocks in fp32. */
 LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* session, const float* x,
                                                   size_t tokens, float* out);
 

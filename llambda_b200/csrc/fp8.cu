@@ -336,6 +336,7 @@ struct F8Pass {
   const int* sel;
   const float* weights;
   int k, E;
+  int pairs;                     // CTA pairs of the device (large products)
   int split;                     // CTAs of a cluster share a tile's K (1: no cluster)
   int early;                     // the weights and tiles are not the previous kernel's output
   int* status;
@@ -994,6 +995,33 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
                : "memory");
 }
 
+// What a pair works on: a tile, or (h 0 or 1) the half of it whose weights are
+// rows 64 h .. 64 h + 63 of both CTAs'.  The tiles of a last round that would
+// leave half of the pairs idle are given out in halves (256 x 65536 x 2688, 256
+// tiles on 74 pairs: 59.2 us in whole ones, 57.5 so).
+struct BigTile {
+  int tt, nt, h;
+};
+struct BigTiles {
+  int tchunks, whole, units;
+  __host__ __device__ BigTiles(int tokens, int rows, int pairs) {
+    tchunks = (tokens + 2 * kF8M - 1) / (2 * kF8M);
+    const int tiles = tchunks * ((rows + 2 * kF8M - 1) / (2 * kF8M));
+    const int rest = tiles % pairs;
+    const bool halves = 2 * rest <= pairs;
+    whole = halves ? tiles - rest : tiles;
+    units = halves ? tiles + rest : tiles;
+  }
+  __device__ BigTile at(int u) const {
+    BigTile t;
+    const int i = u < whole ? u : whole + ((u - whole) >> 1);
+    t.h = u < whole ? -1 : (u - whole) & 1;
+    t.nt = i / tchunks;
+    t.tt = i - t.nt * tchunks;
+    return t;
+  }
+};
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
     f8_big_kernel(const __grid_constant__ F8Maps maps, const F8Pass p) {
   extern __shared__ uint8_t smem_raw[];
@@ -1029,9 +1057,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, sy->tmem, 0);
   griddep_wait();
   griddep_launch();
-  const int tchunks = (p.tokens + 2 * kF8M - 1) / (2 * kF8M);
-  const int ntiles = tchunks * ((p.rows + 2 * kF8M - 1) / (2 * kF8M));
   const int tile0 = (int)blockIdx.x >> 1, tstep = (int)gridDim.x >> 1;
+  const BigTiles tiles(p.tokens, p.rows, p.pairs);
+  const int ntiles = tiles.units;
 
   if (warp == kBigEpi) {  // ------------------------------- producer
     const bool one = elect_one();
@@ -1039,8 +1067,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
     int q = 0;
     bool ok = true;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-      const int nt = tile / tchunks, tt = tile - nt * tchunks;
-      const int t0 = tt * 2 * kF8M + (int)rank * kF8M, n0 = nt * 2 * kF8M + (int)rank * kF8M;
+      const BigTile u = tiles.at(tile);
+      const int t0 = u.tt * 2 * kF8M + (int)rank * kF8M, n0 = u.nt * 2 * kF8M + (int)rank * kF8M;
       const uint32_t sbytes = (uint32_t)max(0L, min((long)kF8M, p.xs_pitch - t0)) * 4u;
       for (int kb = 0; kb < p.kblocks; ++kb) {
         ok = (q < kBigStages || f8_wait_warp(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort)) &&
@@ -1071,15 +1099,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
       int q = 0;
       bool ok = true;
       const uint64_t desc = sw128_desc(stages);
-      const uint32_t idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
       for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
+        const BigTile u = tiles.at(tile);
+        const uint32_t idesc =
+            (1u << 4) | ((u.h < 0 ? 256u >> 3 : 128u >> 3) << 17) | ((256u >> 4) << 24);
+        const uint32_t boff = (kF8M * kF8Block >> 4) + (u.h > 0 ? 64 * kF8Block >> 4 : 0);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = (q < 2 || f8_wait_warp(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
                f8_wait_warp(&sy->full[rp.s], rp.phase, p.status, abort);
           if (!ok) break;
           tc_fence_after();
           const uint64_t ad = desc + (uint32_t)rp.s * (kBigStage >> 4);
-          const uint64_t bd = ad + (kF8M * kF8Block >> 4);
+          const uint64_t bd = ad + boff;
           if (one) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1106,9 +1137,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
     RingPos ap, sp;
     bool ok = true;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-      const int nt = tile / tchunks, tt = tile - nt * tchunks;
-      const int t0 = tt * 2 * kF8M + (int)rank * kF8M + 32 * quad;  // this warp's first token
-      const int n0 = nt * 2 * kF8M + part * 64;                     // its first column
+      const BigTile u = tiles.at(tile);
+      const int t0 = u.tt * 2 * kF8M + (int)rank * kF8M + 32 * quad;  // this warp's first token
+      // its first column; of a half, the first two parts have 64 columns each
+      const int n0 = u.nt * 2 * kF8M + (u.h < 0 ? part * 64 : (part & 1) * kF8M + u.h * 64);
+      const bool idle = u.h >= 0 && part >= 2;
       const float* ws = p.ws0 + (long)min(n0 / kF8M, p.rblocks - 1) * p.kblocks;
       float2 acc[32];
 #pragma unroll
@@ -1124,6 +1157,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
         tc_fence_after();
         const uint32_t from = tmem + lane_base + ap.s * 256 + part * 64;
         const float2 f2 = make_float2(f, f);
+        if (idle) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_cluster(cluster_map(&sy->tempty[ap.s], 0));
+            mbar_arrive(&sy->sempty[sp.s]);
+          }
+          ap.next(2);
+          sp.next(kF8Scales);
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // 16 columns
           uint32_t d[16];
@@ -1147,6 +1191,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
         sp.next(kF8Scales);
       }
       if (!ok) break;
+      if (idle) continue;
       // to row-major through shared memory: 16 words of the warp's 32 rows at a
       // time, stored two rows an instruction
       const int r2 = lane >> 4, w = lane & 15;
@@ -1337,6 +1382,8 @@ bool f8_rows_map(CUtensorMap* map, const void* q, long pitch, long rows, int col
   return f8_encode(map, q, 2, dims, strides, nt);
 }
 
+constexpr long kF8MaxTiles = 1L << 30;  // tiles are counted in 32 bits
+
 // Raises a kernel's shared-memory limit, once per kernel and device.
 cudaError_t f8_allow_smem(const void* kern, size_t bytes) {
   static std::mutex mu;
@@ -1360,6 +1407,7 @@ template <int NT, int MATS, int MODE>
 cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_t s) {
   using C = F8Cfg<NT, MATS>;
   const long slots = (long)sm_count() * C::kCtas;
+  if (tiles > kF8MaxTiles) return cudaErrorInvalidValue;
   p.split = 1;
   while (p.split < kF8MaxSplit && tiles * p.split * 2 <= sm_count() &&
          p.split * 2 * kF8SplitBlocks <= p.kblocks)
@@ -1474,8 +1522,11 @@ cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* 
   if (!big) return launch_f8_pass<1, kF8Out>(nt, maps, p, (long)p.chunks * p.rblocks, st);
   const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(f8_big_kernel), kBigSmem);
   if (e != cudaSuccess) return e;
-  const long pairs = (long)((tokens + 255) / 256) * ((w.rows + 255) / 256);
-  return launch_pdl(f8_big_kernel, dim3((unsigned)(2 * std::min<long>(pairs, sm_count() / 2))),
+  if ((long)((tokens + 255) / 256) * ((w.rows + 255) / 256) > kF8MaxTiles)
+    return cudaErrorInvalidValue;
+  p.pairs = sm_count() / 2;
+  const int units = BigTiles(tokens, w.rows, p.pairs).units;
+  return launch_pdl(f8_big_kernel, dim3((unsigned)(2 * std::min(units, p.pairs))),
                     dim3(kBigThreads), kBigSmem, st, maps, p);
 }
 
