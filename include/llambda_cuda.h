@@ -467,7 +467,8 @@ LLAMBDA_CUDA_API void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session*
 LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* session, const float* x,
                                                   size_t tokens, float* out);
 
-/* Bytes of device workspace that a device call over `tokens` rows needs. */
+/* Bytes of device workspace that a device call over `tokens` rows needs; 0
+ * (then it may be NULL) for few rows, which the product quantises itself. */
 LLAMBDA_CUDA_API size_t llambda_cuda_fp8_session_workspace(const llambda_cuda_fp8_session* session,
                                                            size_t tokens);
 

@@ -1485,7 +1485,7 @@ struct F8Owner {
 };
 
 void require_workspace(const void* p, size_t have, size_t need, int device) {
-  if (have < need)
+  if (!p || have < need)
     throw Failure("The workspace has " + std::to_string(have) + " bytes; this call needs " +
                   std::to_string(need) + ".");
   require_on(p, device, "workspace");
@@ -1626,12 +1626,18 @@ int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor, int o
 void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session* session) { destroy_owner(session); }
 
 size_t llambda_cuda_fp8_session_workspace(const llambda_cuda_fp8_session* s, size_t tokens) {
-  return s && tokens ? f8_quant_bytes(s->w.cols, tokens, nullptr) : 0;
+  if (!s || !tokens || (tokens <= 16 && lb::f8_step_applies(s->w, (int)tokens))) return 0;
+  return f8_quant_bytes(s->w.cols, tokens, nullptr);
 }
 
 static void f8_project_call(llambda_cuda_fp8_session* s, bool x_bf16, const void* x, int64_t ldx,
                             int T, bool out_bf16, void* out, int64_t ldo, void* work,
                             cudaStream_t st) {
+  if (lb::f8_step_applies(s->w, T)) {
+    cuda_check(lb::launch_f8_step(s->w, x_bf16, x, ldx, T, out_bf16, out, ldo, s->status, st),
+               "product launch");
+    return;
+  }
   size_t at = 0;
   f8_quant_bytes(s->w.cols, T, &at);
   uint8_t* q = static_cast<uint8_t*>(work);
@@ -1655,7 +1661,7 @@ int llambda_cuda_fp8_session_run(llambda_cuda_fp8_session* s, const float* x, si
     const size_t in = tokens * s->w.cols * 4, ob = tokens * s->w.rows * 4;
     float* din = static_cast<float*>(s->din.get(in));
     float* dout = static_cast<float*>(s->dout.get(ob));
-    void* work = s->dwork.get(f8_quant_bytes(s->w.cols, tokens, nullptr));
+    void* work = s->dwork.get(llambda_cuda_fp8_session_workspace(s, tokens));
     cuda_check(cudaMemcpyAsync(din, x, in, cudaMemcpyHostToDevice, s->stream), "input copy");
     f8_project_call(s, false, din, s->w.cols, T, false, dout, s->w.rows, work, s->stream);
     s->finish(out, dout, ob, "e4m3 product");
@@ -1668,8 +1674,8 @@ int llambda_cuda_fp8_session_run_device(llambda_cuda_fp8_session* s, int x_type,
                                         int out_type, void* device_out, int64_t ldo,
                                         void* workspace, size_t workspace_bytes,
                                         void* cuda_stream) {
-  if (!s || !device_x || !device_out || !workspace) {
-    set_error("Session, device input/output and a workspace are required.");
+  if (!s || !device_x || !device_out) {
+    set_error("Session and device input/output are required.");
     return -1;
   }
   return guarded([&] {
@@ -1677,8 +1683,8 @@ int llambda_cuda_fp8_session_run_device(llambda_cuda_fp8_session* s, int x_type,
     DeviceGuard g(s->device);
     require_operand(x_type, device_x, ldx, tokens, s->w.cols, s->device, "input");
     require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
-    require_workspace(workspace, workspace_bytes, f8_quant_bytes(s->w.cols, tokens, nullptr),
-                      s->device);
+    if (const size_t need = llambda_cuda_fp8_session_workspace(s, tokens))
+      require_workspace(workspace, workspace_bytes, need, s->device);
     f8_project_call(s, is_bf16(x_type, "input"), device_x, ldx, T, is_bf16(out_type, "output"),
                     device_out, ldo, workspace, static_cast<cudaStream_t>(cuda_stream));
     return 0;

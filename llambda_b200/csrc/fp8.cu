@@ -35,9 +35,12 @@ constexpr int kF8Scales = 8;      // ring of staged activation scales
 constexpr int kF8MaxBuf = 4;      // ring of accumulators in tensor memory
 constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K,
 constexpr int kF8SplitBlocks = 3; // with at least this many blocks each
+constexpr int kF8StepBlocks = 64; // blocks of K a CTA quantises for itself at most,
+constexpr int kF8StepUnits = 4;   // and (token, four blocks) pairs a warp of it
 
 enum F8Mode {
   kF8Out,      // y to out (fp32 or bf16)
+  kF8Step,     // the same for few tokens, which every CTA quantises for itself
   kF8Act,      // activation of gate and up, quantised: the down product's input
   kF8Partial,  // y to the row of its (token, rank) entry
 };
@@ -176,6 +179,72 @@ __device__ __forceinline__ void self_group(const F8Rows& r, int* s_e, int* s_cou
 
 constexpr int kQuantBlocks = 4;  // blocks of one token per warp
 
+// The values of blocks b0 .. b0 + 3 of a row of `cols` columns, zeros past them.
+template <typename T, typename Raw>
+__device__ __forceinline__ void load_blocks(const T* row, int cols, int b0, bool vec,
+                                            Raw (&raw)[kQuantBlocks]) {
+  const int c0 = b0 * kF8Block + 4 * (threadIdx.x & 31);
+  const T* src = row + c0;
+  if (vec && (b0 + kQuantBlocks) * kF8Block <= cols) {
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) raw[i] = load4(src + i * kF8Block, true, 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const int c = c0 + i * kF8Block;
+      raw[i] = zero4(row);
+      if (c < cols) raw[i] = load4(src + i * kF8Block, vec && c + 4 <= cols, cols - c);
+    }
+  }
+}
+
+// Four blocks of a token, four columns a lane and block: their e4m3 bytes, and
+// on lane i the scale of block i (mine: that lane's block exists).
+template <typename Raw>
+__device__ __forceinline__ void quant_blocks(const Raw (&raw)[kQuantBlocks], bool mine,
+                                             uint32_t (&w)[kQuantBlocks], float& s_own) {
+  const int lane = threadIdx.x & 31;
+  float2 v[kQuantBlocks][2];
+  float am = 0.0f;  // lane i: the largest magnitude of block i
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks; ++i) {
+    floats4(raw[i], v[i]);
+    const float m = warp_max_nan(
+        max_abs3(max_abs3(v[i][0].x, v[i][0].y, v[i][1].x), v[i][1].y, 0.0f));
+    if (lane == i) am = m;
+  }
+  // am / 448 as a quotient by the rounded reciprocal; where that or the
+  // values' own do not hold, the slow way
+  s_own = quotient(am, 448.0f, 1.0f / 448.0f);
+  const bool plain =
+      __all_sync(0xffffffffu, !mine || am == 0.0f || (am >= 0x1p-70f && am <= 0x1p100f));
+  if (am == 0.0f) s_own = FLT_MIN;
+  if (!plain) s_own = block_scale(__float_as_uint(am));
+  if (plain) {
+    const float r_own = __frcp_rn(s_own);
+#pragma unroll
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const float s = __shfl_sync(0xffffffffu, s_own, i), r = __shfl_sync(0xffffffffu, r_own, i);
+      const float2 s2 = make_float2(-s, -s), r2 = make_float2(r, r);
+      w[i] = e4m3_word(quotient2(v[i][0], s2, r2), quotient2(v[i][1], s2, r2));
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kQuantBlocks; ++i) {
+      const float s = __shfl_sync(0xffffffffu, s_own, i);
+      uint32_t wi = 0;
+#pragma unroll
+      for (int ii = 0; ii < kQuantBlocks; ++ii)
+        if (ii == i)
+          wi = e4m3_word(make_float2(__fdiv_rn(v[ii][0].x, s), __fdiv_rn(v[ii][0].y, s)),
+                         make_float2(__fdiv_rn(v[ii][1].x, s), __fdiv_rn(v[ii][1].y, s)));
+#pragma unroll
+      for (int ii = 0; ii < kQuantBlocks; ++ii)
+        if (ii == i) w[ii] = wi;
+    }
+  }
+}
+
 // One warp per token and kQuantBlocks blocks of 128 columns, four columns a
 // lane and block, every load issued before the first is used.  q has rows of
 // q_pitch bytes (a multiple of 16, zeros past cols), scales the layout
@@ -212,64 +281,15 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
     if (MODE == kQuantRows && t < s_pitch && mine) sp[t] = 0.0f;
     return;
   }
-  const T* src = x + t * ldx + c0;
   Raw raw[kQuantBlocks];
-  if (vec && whole && t < tokens) {
-#pragma unroll
-    for (int i = 0; i < kQuantBlocks; ++i) raw[i] = load4(src + i * kF8Block, true, 4);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kQuantBlocks; ++i) {
-      const int c = c0 + i * kF8Block;
-      raw[i] = zero4(x);
-      if (t < tokens && c < cols)
-        raw[i] = load4(src + i * kF8Block, vec && c + 4 <= cols, cols - c);
-    }
-  }
+  load_blocks(x + t * ldx, t < tokens ? cols : 0, b0, vec, raw);
   if (MODE == kQuantSelf) {  // while the loads are on their way
     self_group(rows, s_e, s_count, s_row, &s_chunks);
     if (t >= tokens) return;
   }
-  float2 v[kQuantBlocks][2];
-  float am = 0.0f;  // lane i: the largest magnitude of block i
-#pragma unroll
-  for (int i = 0; i < kQuantBlocks; ++i) {
-    floats4(raw[i], v[i]);
-    const float m = warp_max_nan(
-        max_abs3(max_abs3(v[i][0].x, v[i][0].y, v[i][1].x), v[i][1].y, 0.0f));
-    if (lane == i) am = m;
-  }
-  // am / 448 as a quotient by the rounded reciprocal; where that or the
-  // values' own do not hold, the slow way
-  float s_own = quotient(am, 448.0f, 1.0f / 448.0f);
-  const bool plain =
-      __all_sync(0xffffffffu, !mine || am == 0.0f || (am >= 0x1p-70f && am <= 0x1p100f));
-  if (am == 0.0f) s_own = FLT_MIN;
-  if (!plain) s_own = block_scale(__float_as_uint(am));
   uint32_t w[kQuantBlocks];
-  if (plain) {
-    const float r_own = __frcp_rn(s_own);
-#pragma unroll
-    for (int i = 0; i < kQuantBlocks; ++i) {
-      const float s = __shfl_sync(0xffffffffu, s_own, i), r = __shfl_sync(0xffffffffu, r_own, i);
-      const float2 s2 = make_float2(-s, -s), r2 = make_float2(r, r);
-      w[i] = e4m3_word(quotient2(v[i][0], s2, r2), quotient2(v[i][1], s2, r2));
-    }
-  } else {
-#pragma unroll 1
-    for (int i = 0; i < kQuantBlocks; ++i) {
-      const float s = __shfl_sync(0xffffffffu, s_own, i);
-      uint32_t wi = 0;
-#pragma unroll
-      for (int ii = 0; ii < kQuantBlocks; ++ii)
-        if (ii == i)
-          wi = e4m3_word(make_float2(__fdiv_rn(v[ii][0].x, s), __fdiv_rn(v[ii][0].y, s)),
-                         make_float2(__fdiv_rn(v[ii][1].x, s), __fdiv_rn(v[ii][1].y, s)));
-#pragma unroll
-      for (int ii = 0; ii < kQuantBlocks; ++ii)
-        if (ii == i) w[ii] = wi;
-    }
-  }
+  float s_own;
+  quant_blocks(raw, mine, w, s_own);
   auto store = [&](uint8_t* row, float* scale) {
     uint32_t* out = reinterpret_cast<uint32_t*>(row);
     if (whole) {
@@ -320,7 +340,10 @@ struct F8Pass {
   int tokens, chunks;            // dense: rows of x and their tiles of NT
   const int4* tiles;             // grouped: {first row, rows, expert, 0} of each chunk,
   const int* nchunks;            //   null when dense
-  void* out;                     // kF8Out
+  const void* x;                 // kF8Step: the rows themselves
+  long ldx;
+  int cols, x_bf16, x_vec;
+  void* out;                     // kF8Out, kF8Step
   long ldo;
   int out_bf16;
   uint8_t* hq;                   // kF8Act: quantised activations and their scales
@@ -345,7 +368,7 @@ struct F8Pass {
 struct F8Sync {
   uint64_t full[16], empty[16];
   uint64_t sfull[kF8Scales], sempty[kF8Scales];
-  uint64_t tfull[kF8MaxBuf], tempty[kF8MaxBuf], done;
+  uint64_t tfull[kF8MaxBuf], tempty[kF8MaxBuf], done, xfull;
   uint32_t tmem;
   int abort, last;
 };
@@ -353,17 +376,21 @@ struct F8Sync {
 // Small tiles are bound by the weights' bytes: two CTAs a multiprocessor, so
 // that one loads while the other finishes a tile.  Large ones take the whole
 // shared memory for one.
-template <int NT, int MATS>
+template <int NT, int MATS, int MODE>
 struct F8Cfg {
-  static constexpr int kCtas = NT == 64 && MATS == 2 ? 1 : 2;
-  static constexpr uint32_t kBudget = (kCtas == 2 ? 104u : 200u) * 1024u;
+  static constexpr bool kStep = MODE == kF8Step;
+  static constexpr int kCtas = kStep || (NT == 64 && MATS == 2) ? 1 : 2;
   static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
-  static constexpr uint32_t kStage = MATS * kA + NT * kF8Block;
+  static constexpr uint32_t kX = NT * kF8Block;          // and of one block of activations
+  static constexpr uint32_t kStage = MATS * kA + (kStep ? 0 : kX);
+  static constexpr uint32_t kBudget = kStep ? 5 * kStage : (kCtas == 2 ? 104u : 200u) * 1024u;
   static constexpr int kStages = (int)(kBudget / kStage);
   static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
   static constexpr int kBufs = 512 / kAcc / kCtas > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc / kCtas;
   static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kF8Scales * NT * 4 +
+  static constexpr int kScales = kStep ? kF8StepBlocks : kF8Scales;  // blocks of scales staged
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage +
+                                  (kStep ? kF8StepBlocks * kX : 0) + kScales * NT * 4 +
                                   2 * 4 * NT * 4 + sizeof(F8Sync);
 };
 
@@ -520,6 +547,40 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
   return v;
 }
 
+// kF8Step: blocks [kb0, kb1) of every token, by the eight epilogue warps, into
+// shared memory as a TMA copy with the 128-byte swizzle would lay them out (16
+// bytes' place within a row of 128 exclusive-or the row's number modulo 8).
+// Rows of no token keep what they hold: they reach no column that is stored.
+template <int NT, typename T>
+__device__ __forceinline__ void step_quantize(const F8Pass& p, const T* x, int kb0, int kb1,
+                                              uint8_t* s_x, float* s_scale) {
+  using Raw = decltype(load4(x, true, 4));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (kb1 - kb0 + kQuantBlocks - 1) / kQuantBlocks, units = p.tokens * per;
+  Raw raw[kF8StepUnits][kQuantBlocks];
+#pragma unroll
+  for (int i = 0; i < kF8StepUnits; ++i) {  // every load before the first is used
+    const int u = warp + i * kF8EpiWarps, t = u / per;
+    if (u < units)
+      load_blocks(x + t * p.ldx, p.cols, kb0 + (u - t * per) * kQuantBlocks, p.x_vec, raw[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kF8StepUnits; ++i) {
+    const int u = warp + i * kF8EpiWarps, t = u / per, b0 = (u - t * per) * kQuantBlocks;
+    if (u >= units) break;
+    const bool mine = lane < kQuantBlocks && kb0 + b0 + lane < kb1;
+    uint32_t w[kQuantBlocks];
+    float s;
+    quant_blocks(raw[i], mine, w, s);
+#pragma unroll
+    for (int j = 0; j < kQuantBlocks; ++j)
+      if (kb0 + b0 + j < kb1)
+        *reinterpret_cast<uint32_t*>(s_x + (b0 + j) * (NT * kF8Block) + t * kF8Block +
+                                     (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w[j];
+    if (mine) s_scale[(b0 + lane) * NT + t] = s;
+  }
+}
+
 // Persistent over tiles of 128 weight rows x NT rows of x (M is the weights'
 // side, so one token costs a tile of 16 columns, and an expert's few tokens no
 // more).  Warp 8 stages weights and activations by TMA, warp 10 the activations'
@@ -532,14 +593,15 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
 // each, then each adds the sums of its share of the columns from the others'
 // shared memory.
 template <int NT, int MATS, int MODE, bool SPLIT>
-__global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
+__global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     f8_gemm_kernel(const __grid_constant__ F8Maps maps, const F8Pass p) {
-  using C = F8Cfg<NT, MATS>;
+  using C = F8Cfg<NT, MATS, MODE>;
   constexpr int NC = NT / 2;  // tokens per epilogue thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  float* s_scale = reinterpret_cast<float*>(stages + (size_t)C::kStages * C::kStage);
-  uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + kF8Scales * NT);  // [parity][quadrant][NT]
+  uint8_t* s_x = stages + (size_t)C::kStages * C::kStage;  // kF8Step: [block][NT][128], swizzled
+  float* s_scale = reinterpret_cast<float*>(s_x + (C::kStep ? kF8StepBlocks * C::kX : 0));
+  uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + C::kScales * NT);  // [parity][quadrant][NT]
   F8Sync* sy = reinterpret_cast<F8Sync*>(s_amax + 2 * 4 * NT);
   volatile int* abort = &sy->abort;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -557,6 +619,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
       mbar_init(&sy->tempty[b], kF8EpiWarps);
     }
     mbar_init(&sy->done, 1);
+    mbar_init(&sy->xfull, kF8EpiWarps);
     sy->abort = 0;
     fence_mbar_init();
   }
@@ -606,8 +669,9 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         if (!ok) break;
         if (one) {
           if (q >= ahead) load_weights(rp.s, kb, t);
-          tma_load_2d(stages + (size_t)rp.s * C::kStage + MATS * C::kA, &maps.x, kb * kF8Block,
-                      t.row0, &sy->full[rp.s]);
+          if (!C::kStep)
+            tma_load_2d(stages + (size_t)rp.s * C::kStage + MATS * C::kA, &maps.x, kb * kF8Block,
+                        t.row0, &sy->full[rp.s]);
         }
         ++q;
         rp.next(C::kStages);
@@ -618,7 +682,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     const bool one = elect_one();
     RingPos rp;
     int q = 0;
-    bool ok = true;
+    bool ok = !C::kStep;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
       const F8Tile t = f8_tile<NT>(p, tile);
       // row0 and the pitch are multiples of 4; columns past the pitch keep
@@ -642,7 +706,8 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     RingPos rp, ap;
     int q = 0;
     bool ok = true;
-    const uint64_t desc = sw128_desc(stages);
+    const uint64_t desc = sw128_desc(stages), xdesc = sw128_desc(s_x);
+    if (C::kStep) ok = f8_wait_warp(&sy->xfull, 0, p.status, abort);
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
       const F8Tile t = f8_tile<NT>(p, tile);
       const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
@@ -652,7 +717,8 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         if (!ok) break;
         tc_fence_after();
         const uint64_t ad = desc + (uint32_t)rp.s * (C::kStage >> 4);
-        const uint64_t bd = ad + (MATS * C::kA >> 4);
+        const uint64_t bd = C::kStep ? xdesc + (uint32_t)(kb - kb0) * (C::kX >> 4)
+                                     : ad + (MATS * C::kA >> 4);
         const uint32_t d = tmem + ap.s * C::kAcc;
         if (one) {
 #pragma unroll
@@ -679,6 +745,16 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
     RingPos ap, sp;
     bool ok = true;
     int parity = 0;
+    if constexpr (C::kStep) {
+      if (p.x_bf16)
+        step_quantize<NT>(p, static_cast<const __nv_bfloat16*>(p.x), kb0, kb1, s_x, s_scale);
+      else
+        step_quantize<NT>(p, static_cast<const float*>(p.x), kb0, kb1, s_x, s_scale);
+      fence_proxy_async_smem();  // the MMAs read what these threads wrote
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sy->xfull);
+      named_bar_sync(3, kF8EpiWarps * 32);  // and all of them the scales
+    }
     if (MODE == kF8Partial && NT == 16 && p.counters && ntiles == 0)  // no entry is anyone's
       for (long i = (long)blockIdx.x * kF8EpiWarps * 32 + threadIdx.x; i < (long)p.tokens * p.rows;
            i += (long)gridDim.x * kF8EpiWarps * 32)
@@ -714,12 +790,12 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         float sw[MATS];
 #pragma unroll
         for (int m = 0; m < MATS; ++m) sw[m] = __shfl_sync(0xffffffffu, wl[m], (kb - kb0) & 31);
-        ok = f8_wait(&sy->sfull[sp.s], sp.phase, p.status, abort) &&
+        ok = (C::kStep || f8_wait(&sy->sfull[sp.s], sp.phase, p.status, abort)) &&
              f8_wait(&sy->tfull[ap.s], ap.phase, p.status, abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const float* sc = s_scale + sp.s * NT;
+        const float* sc = s_scale + (C::kStep ? kb - kb0 : sp.s) * NT;
         // columns loaded together, as many as the registers hold: the loads of a
         // second group wait for the first
         constexpr int CH = C::kCtas == 2 ? (NC < 16 / MATS ? NC : 16 / MATS)
@@ -757,7 +833,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&sy->tempty[ap.s]);
-          mbar_arrive(&sy->sempty[sp.s]);
+          if (!C::kStep) mbar_arrive(&sy->sempty[sp.s]);
         }
         ap.next(C::kBufs);
         sp.next(kF8Scales);
@@ -798,7 +874,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS>::kCtas))
             }
       }
       const int row = t.rb * kF8M + r;
-      if (MODE == kF8Out) {
+      if (MODE == kF8Out || MODE == kF8Step) {
         if (row < p.rows) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
@@ -1398,20 +1474,25 @@ cudaError_t f8_allow_smem(const void* kern, size_t bytes) {
   return e;
 }
 
-// tiles: an upper bound.  Where they leave multiprocessors idle, clusters share
-// a tile's K as long as every CTA has one to itself and a few blocks of K.  One
+// CTAs to a tile.  Where the tiles (an upper bound of them) leave multiprocessors
+// idle, clusters share a tile's K as long as every CTA has one to itself and a few blocks of K.  One
 // token, cold: 512 rows of 8192 columns 22.5 us unsplit, 12.6 in eight; 4096 of
 // 4096 17.3, 14.5 in four; 2688 of 1856 12.5, 12.3 in four; 14336 of 4096 (112
 // tiles) 22.5 unsplit, and with 24 tokens 22.6 against 26.7 in two.
+int f8_split(long tiles, int kblocks) {
+  int split = 1;
+  while (split < kF8MaxSplit && tiles * split * 2 <= sm_count() &&
+         split * 2 * kF8SplitBlocks <= kblocks)
+    split *= 2;
+  return split;
+}
+
 template <int NT, int MATS, int MODE>
 cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_t s) {
-  using C = F8Cfg<NT, MATS>;
+  using C = F8Cfg<NT, MATS, MODE>;
   const long slots = (long)sm_count() * C::kCtas;
   if (tiles > kF8MaxTiles) return cudaErrorInvalidValue;
-  p.split = 1;
-  while (p.split < kF8MaxSplit && tiles * p.split * 2 <= sm_count() &&
-         p.split * 2 * kF8SplitBlocks <= p.kblocks)
-    p.split *= 2;
+  p.split = f8_split(tiles, p.kblocks);
   auto kern = p.split > 1 ? f8_gemm_kernel<NT, MATS, MODE, true>
                           : f8_gemm_kernel<NT, MATS, MODE, false>;
   const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), C::kSmem);
@@ -1489,6 +1570,38 @@ cudaError_t f8_check_scales(const float* scales, size_t n, unsigned* bad, cudaSt
 
 cudaError_t f8_prepare(F8Matrix* w) {
   return f8_weight_map(&w->map, *w) ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+bool f8_step_applies(const F8Matrix& w, int tokens) {
+  if (tokens > 16) return false;
+  const int kb = f8_blocks(w.cols);
+  const int most = (kb + f8_split(f8_blocks(w.rows), kb) - 1) / f8_split(f8_blocks(w.rows), kb);
+  return most <= kF8StepBlocks &&
+         tokens * ((most + kQuantBlocks - 1) / kQuantBlocks) <= kF8StepUnits * kF8EpiWarps;
+}
+
+cudaError_t launch_f8_step(const F8Matrix& w, bool x_bf16, const void* x, long ldx, int tokens,
+                           bool out_bf16, void* out, long ldo, int* status, cudaStream_t st) {
+  F8Maps maps;
+  maps.x = maps.w0 = maps.w1 = w.map;
+  F8Pass p{};
+  p.rows = w.rows;
+  p.rblocks = f8_blocks(w.rows);
+  p.kblocks = f8_blocks(w.cols);
+  p.ws0 = w.scales;
+  p.tokens = tokens;
+  p.chunks = 1;
+  p.x = x;
+  p.ldx = ldx;
+  p.cols = w.cols;
+  p.x_bf16 = x_bf16;
+  p.x_vec = (tokens == 1 || ldx % 4 == 0) &&
+            reinterpret_cast<uintptr_t>(x) % (x_bf16 ? 8 : 16) == 0;
+  p.out = out;
+  p.ldo = ldo;
+  p.out_bf16 = out_bf16;
+  p.status = status;
+  return launch_f8_gemm<16, 1, kF8Step>(maps, p, p.rblocks, st);
 }
 
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
@@ -1579,7 +1692,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   // launch lets the gate and up product request ahead, cost more (32 tokens, 6
   // of 128 experts of 2688 x 1856: 215 us against 157).
   const bool few = n <= kSelfEntries && nt == 16 &&
-                   chunks * f8_blocks(m.down.rows) <= (long)sm_count() * F8Cfg<16, 1>::kCtas;
+                   chunks * f8_blocks(m.down.rows) <= (long)sm_count() * F8Cfg<16, 1, kF8Partial>::kCtas;
   int* counters = few ? reinterpret_cast<int*>(base + L.counters) : nullptr;
   cudaError_t e = cudaSuccess;
   if (!few) {

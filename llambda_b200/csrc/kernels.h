@@ -336,6 +336,11 @@ cudaError_t launch_f8_quant(bool bf16, const void* x, long ldx, int tokens, int 
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,
                               bool out_bf16, void* out, long ldo, bool after_quant, int* status,
                               cudaStream_t st);
+// The same straight from few rows of x, without a quantised copy, where
+// f8_step_applies.
+bool f8_step_applies(const F8Matrix& w, int tokens);
+cudaError_t launch_f8_step(const F8Matrix& w, bool x_bf16, const void* x, long ldx, int tokens,
+                           bool out_bf16, void* out, long ldo, int* status, cudaStream_t st);
 F8MoeLayout f8_moe_layout(const F8Moe& m, long tokens, int k);
 cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, int tokens, int k,
                           const int* sel, const float* weights, bool out_bf16, void* out, long ldo,

@@ -336,9 +336,9 @@ class Fp8ProjectionSession(_Fp8Session):
         nbytes = (_lib or _library()).llambda_cuda_fp8_session_workspace(h, T)
         raw, ((out, ldo), work) = _on(stream, dev, lambda: (
             _out(out, T, self.rows, out_dtype or x.dtype, dev),
-            _t.empty(nbytes, dtype=_t.uint8, device=dev)))
+            _t.empty(nbytes, dtype=_t.uint8, device=dev) if nbytes else None))
         _check((_lib or _library()).llambda_cuda_fp8_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T,
-              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr(), nbytes, raw))
+              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr() if nbytes else None, nbytes, raw))
         return out
 
     def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):

@@ -264,7 +264,9 @@ def check(out, y, bound):
 SIZES = [(1, 1, 16), (1, 300, 400), (2, 128, 128), (5, 64, 112), (16, 130, 1040), (17, 257, 144),
          (33, 2688, 1856), (64, 128, 2064), (65, 96, 256), (129, 384, 384), (300, 200, 640),
          (513, 1030, 272), (1, 4096, 4096), (31, 4096, 8192), (48, 200, 4112), (100, 128, 4096),
-         (127, 2700, 528), (300, 20000, 272), (257, 19000, 144), (1025, 5000, 400)]
+         (127, 2700, 528), (300, 20000, 272), (257, 19000, 144), (1025, 5000, 400),
+         (1, 20000, 8192), (4, 300, 4096), (3, 128, 8208), (2, 20000, 8208), (16, 640, 1024),
+         (7, 130, 16), (1, 1000, 16400)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -356,23 +358,33 @@ def test_product_refusals():
         p.run_quantized(q, sc[:, :3], 3)
     # C calls: a workspace that is too small, host memory, a short row stride
     from llambda_b200 import _native as N
-    L, out = N.lib(), torch.empty(3, 64, device="cuda")
+    x = randn(g, 40, 64)
+    L, out = N.lib(), torch.empty(40, 64, device="cuda")
     work = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
-    args = [p._h, 0, x.data_ptr(), 64, 3, 0, out.data_ptr(), 64, work.data_ptr(), work.numel(), None]
+    assert 0 < L.llambda_cuda_fp8_session_workspace(p._h, 40) <= work.numel()
+    args = [p._h, 0, x.data_ptr(), 64, 40, 0, out.data_ptr(), 64, work.data_ptr(), work.numel(),
+            None]
 
     def call(i, v):
         return L.llambda_cuda_fp8_session_run_device(*(args[:i] + [v] + args[i + 1:]))
 
     assert call(9, 8) == -1 and "workspace" in N.last_error()
+    assert call(8, None) == -1 and "workspace" in N.last_error()
     assert call(8, work.data_ptr() + 16) == -1 and "256-byte" in N.last_error()
     assert call(3, 63) == -1 and "row stride" in N.last_error()
     assert call(1, 1) == -1 and "element type" in N.last_error()
     assert call(4, 0) == -1 and "token count" in N.last_error()
-    host = np.zeros((3, 64), np.float32)
+    host = np.zeros((40, 64), np.float32)
     assert call(2, host.ctypes.data) == -1 and "device memory" in N.last_error()
     assert call(3, 64) == 0
     torch.cuda.synchronize()
     assert torch.equal(out, p.run_device(x))
+    # a few rows need none
+    assert L.llambda_cuda_fp8_session_workspace(p._h, 1) == 0
+    args[4:5], args[8:10] = [1], [None, 0]
+    assert call(3, 64) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out[:1], p.run_device(x[:1]))
 
 
 # ------------------------------------------------------------------ routed experts
@@ -448,7 +460,8 @@ def test_experts(dtype, gated, T, E, k, H, I, O):
 
 
 def test_experts_do_not_depend_on_the_batch():
-    """A token's result has the same bits alone, in a batch, and beside skipped entries."""
+    """A token's result has the same bits alone, in a batch, and beside skipped entries (at
+    widths too small for CTAs to share them out, which another number of tiles may change)."""
     g = gen(21)
     E, k, H, I, T = 12, 3, 192, 160, 150
     up, down, gate = matrices(g, E, I, H), matrices(g, E, H, I), matrices(g, E, I, H)
