@@ -375,7 +375,7 @@ struct F8Sync {
 
 // Small tiles are bound by the weights' bytes: two CTAs a multiprocessor, so
 // that one loads while the other finishes a tile.  Large ones take the whole
-// shared memory for one.
+// shared memory for one, as does kF8Step with every block of its tokens.
 template <int NT, int MATS, int MODE>
 struct F8Cfg {
   static constexpr bool kStep = MODE == kF8Step;
@@ -522,8 +522,8 @@ __device__ __forceinline__ F8Tile f8_tile(const F8Pass& p, int tile) {
   return t;
 }
 
-// (__fdividef is off by two steps at most; its result for a divisor above 2^126
-// is 0, which is also that of the exact quotient here)
+// (__fdividef is off by two steps at most; for a divisor above 2^126 it gives 0,
+// where the exact quotient is below 2^-119)
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
