@@ -35,13 +35,14 @@ constexpr int kF8Scales = 8;      // ring of staged activation scales
 constexpr int kF8MaxBuf = 4;      // ring of accumulators in tensor memory
 constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K,
 constexpr int kF8SplitBlocks = 3; // with at least this many blocks each
-constexpr int kF8StepBlocks = 64; // blocks of K a CTA quantises for itself at most,
-constexpr int kF8StepUnits = 4;   // and (token, four blocks) pairs a warp of it
+constexpr int kF8StepUnits = 4;   // (row, four blocks) pairs of a warp that quantises, at a time
+constexpr int kF8StepEntries = 256;  // entries that a CTA groups for itself
 
 enum F8Mode {
   kF8Out,      // y to out (fp32 or bf16)
   kF8Step,     // the same for few tokens, which every CTA quantises for itself
   kF8Act,      // activation of gate and up, quantised: the down product's input
+  kF8StepAct,  // the same for few entries, which every CTA groups and quantises for itself
   kF8Partial,  // y to the row of its (token, rank) entry
 };
 
@@ -125,57 +126,7 @@ struct F8Rows {
   const int *sel, *pos, *row_start;  // null: row t
   int* entry;                        // receives the entry of each grouped row
   int k, E;
-  // few entries: the quantiser groups them itself (no pos, no row_start) and
-  // its first CTA writes what the plan would have, and zeroes `clear` counters
-  int n, nt, nclear;
-  int4* tiles;
-  int *nchunks, *clear;
 };
-
-enum QuantMode { kQuantRows, kQuantGrouped, kQuantSelf };
-constexpr int kSelfEntries = 256;  // one a thread
-
-// Groups n <= kSelfEntries entries by expert as f8_plan_kernel does, in every
-// CTA for itself: entry i counts the entries of its expert before it and in
-// all, then the rows and chunks of the experts before its own.  row[i]: its
-// grouped row, -1 if its expert is outside [0, E).
-__device__ __forceinline__ void self_group(const F8Rows& r, int* s_e, int* s_count, int* s_row,
-                                           int* s_chunks) {
-  const int i = threadIdx.x;
-  int e = i < r.n ? __ldg(r.sel + i) : -1;
-  if (e >= r.E) e = -1;
-  s_e[i] = e;
-  if (i == 0) *s_chunks = 0;
-  __syncthreads();
-  int pos = 0, cnt = 0;
-  for (int j = 0; j < r.n; ++j) {
-    const bool same = s_e[j] == e;
-    pos += same && j < i;
-    cnt += same;
-  }
-  const bool first = e >= 0 && pos == 0;
-  s_count[i] = first ? cnt : 0;
-  __syncthreads();
-  int base = 0, chunk = 0;
-  for (int j = 0; j < r.n; ++j) {
-    const int c = s_e[j] < e ? s_count[j] : 0;
-    base += (c + 3) & ~3;
-    chunk += (c + r.nt - 1) / r.nt;
-  }
-  s_row[i] = e >= 0 ? base + pos : -1;
-  if (blockIdx.x == 0) {
-    if (e >= 0) r.entry[base + pos] = i;
-    if (first) {
-      const int ch = (cnt + r.nt - 1) / r.nt;
-      for (int c = 0; c < ch; ++c)
-        r.tiles[chunk + c] = make_int4(base + c * r.nt, min(r.nt, cnt - c * r.nt), e, 0);
-      atomicMax(s_chunks, chunk + ch);
-    }
-    for (int c = i; c < r.nclear; c += blockDim.x) r.clear[c] = 0;
-  }
-  __syncthreads();
-  if (blockIdx.x == 0 && i == 0) *r.nchunks = *s_chunks;
-}
 
 constexpr int kQuantBlocks = 4;  // blocks of one token per warp
 
@@ -256,15 +207,12 @@ __device__ __forceinline__ void quant_blocks(const Raw (&raw)[kQuantBlocks], boo
 // at a time.  8192 x 4096 bf16: 47 us with a division a value, 25 with
 // quotients by the reciprocal one at a time, 21 now; warps that stay and
 // request the next token's values ahead took 27.
-template <typename T, int MODE>
+template <typename T, bool GROUPED>
 __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, long ldx,
                                                        int tokens, int cols, uint8_t* q,
                                                        int q_pitch, float* scales, int s_pitch,
                                                        F8Rows rows, int vec) {
   using Raw = decltype(load4(x, true, 4));
-  __shared__ int s_e[MODE == kQuantSelf ? kSelfEntries : 1],
-      s_count[MODE == kQuantSelf ? kSelfEntries : 1], s_row[MODE == kQuantSelf ? kSelfEntries : 1],
-      s_chunks;
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
@@ -277,16 +225,12 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
   const bool mine = lane < kQuantBlocks && b0 + lane < blocks;  // this lane's scale exists
   uint8_t* dst = q + c0;
   float* sp = scales + (long)(b0 + lane) * s_pitch;
-  if (MODE != kQuantSelf && t >= tokens) {
-    if (MODE == kQuantRows && t < s_pitch && mine) sp[t] = 0.0f;
+  if (t >= tokens) {
+    if (!GROUPED && t < s_pitch && mine) sp[t] = 0.0f;
     return;
   }
   Raw raw[kQuantBlocks];
-  load_blocks(x + t * ldx, t < tokens ? cols : 0, b0, vec, raw);
-  if (MODE == kQuantSelf) {  // while the loads are on their way
-    self_group(rows, s_e, s_count, s_row, &s_chunks);
-    if (t >= tokens) return;
-  }
+  load_blocks(x + t * ldx, cols, b0, vec, raw);
   uint32_t w[kQuantBlocks];
   float s_own;
   quant_blocks(raw, mine, w, s_own);
@@ -302,13 +246,8 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const T* __restrict__ x, 
     }
     if (mine) *scale = s_own;
   };
-  if (MODE == kQuantRows) {
+  if (!GROUPED) {
     store(dst + (long)t * q_pitch, sp + t);
-  } else if (MODE == kQuantSelf) {
-    for (int j = 0; j < rows.k; ++j) {
-      const int o = s_row[t * rows.k + j];
-      if (o >= 0) store(dst + (long)o * q_pitch, sp + o);
-    }
   } else {
     for (int j0 = 0; j0 < rows.k; j0 += 32) {  // the entries' rows, one a lane
       const int id = t * rows.k + j0 + lane;
@@ -340,9 +279,14 @@ struct F8Pass {
   int tokens, chunks;            // dense: rows of x and their tiles of NT
   const int4* tiles;             // grouped: {first row, rows, expert, 0} of each chunk,
   const int* nchunks;            //   null when dense
-  const void* x;                 // kF8Step: the rows themselves
+  const void* x;                 // kF8Step, kF8StepAct: the rows themselves
   long ldx;
   int cols, x_bf16, x_vec;
+  // kF8StepAct: what the first CTA writes for the down product: its tiles, the
+  // entry of each row, and zeroes in nclear counters
+  int4* tiles_out;
+  int *nchunks_out, *entry_out, *clear;
+  int n, nclear;
   void* out;                     // kF8Out, kF8Step
   long ldo;
   int out_bf16;
@@ -373,25 +317,36 @@ struct F8Sync {
   int abort, last;
 };
 
+// kF8StepAct: the grouping of up to kF8StepEntries entries by expert, as
+// f8_plan_kernel has it, and this CTA's tile of it.
+struct F8Group {
+  int e[kF8StepEntries], count[kF8StepEntries], row[kF8StepEntries];
+  int tok[16];  // token of each row of the tile
+  int chunks, row0, rows, expert;
+};
+
 // Small tiles are bound by the weights' bytes: two CTAs a multiprocessor, so
 // that one loads while the other finishes a tile.  Large ones take the whole
 // shared memory for one, as does kF8Step with every block of its tokens.
 template <int NT, int MATS, int MODE>
 struct F8Cfg {
-  static constexpr bool kStep = MODE == kF8Step;
+  static constexpr bool kStep = MODE == kF8Step || MODE == kF8StepAct;
   static constexpr int kCtas = kStep || (NT == 64 && MATS == 2) ? 1 : 2;
   static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
   static constexpr uint32_t kX = NT * kF8Block;          // and of one block of activations
   static constexpr uint32_t kStage = MATS * kA + (kStep ? 0 : kX);
-  static constexpr uint32_t kBudget = kStep ? 5 * kStage : (kCtas == 2 ? 104u : 200u) * 1024u;
+  static constexpr uint32_t kBudget =
+      kStep ? (MATS == 2 ? 4 : 5) * kStage : (kCtas == 2 ? 104u : 200u) * 1024u;
   static constexpr int kStages = (int)(kBudget / kStage);
+  static constexpr int kStepBlocks = MATS == 2 ? 40 : 64;  // blocks of K a CTA quantises, at most
   static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
   static constexpr int kBufs = 512 / kAcc / kCtas > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc / kCtas;
   static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
-  static constexpr int kScales = kStep ? kF8StepBlocks : kF8Scales;  // blocks of scales staged
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage +
-                                  (kStep ? kF8StepBlocks * kX : 0) + kScales * NT * 4 +
-                                  2 * 4 * NT * 4 + sizeof(F8Sync);
+  static constexpr int kScales = kStep ? kStepBlocks : kF8Scales;  // blocks of scales staged
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (kStep ? kStepBlocks * kX : 0) +
+                                  kScales * NT * 4 + 2 * 4 * NT * 4 + sizeof(F8Sync) +
+                                  (MODE == kF8StepAct ? sizeof(F8Group) : 0);
+  static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 // Instruction descriptor, kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), A and
@@ -547,37 +502,93 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
   return v;
 }
 
-// kF8Step: blocks [kb0, kb1) of every token, by the eight epilogue warps, into
-// shared memory as a TMA copy with the 128-byte swizzle would lay them out (16
-// bytes' place within a row of 128 exclusive-or the row's number modulo 8).
-// Rows of no token keep what they hold: they reach no column that is stored.
+// Groups the entries (token t, rank j; id t * k + j) by expert, in every CTA for
+// itself, as f8_plan_kernel does: entry i counts the entries of its expert
+// before it and in all, then the rows and chunks (of NT) of the experts before
+// its own.  Entries whose expert is outside [0, E) are in no group.  Leaves the
+// rows of chunk `mine` and their tokens in g (rows 0: there is no such chunk).
+template <int NT>
+__device__ __forceinline__ void step_group(const F8Pass& p, F8Group& g, int mine) {
+  const int i = threadIdx.x;
+  const bool on = i < kF8StepEntries;
+  int e = on && i < p.n ? __ldcg(p.sel + i) : -1;
+  if (e >= p.E) e = -1;
+  if (on) g.e[i] = e;
+  if (i == 0) g.chunks = g.row0 = g.rows = g.expert = 0;
+  __syncthreads();
+  int pos = 0, cnt = 0;
+  if (on)
+    for (int j = 0; j < p.n; ++j) {
+      const bool same = g.e[j] == e;
+      pos += same && j < i;
+      cnt += same;
+    }
+  const bool first = e >= 0 && pos == 0;
+  if (on) g.count[i] = first ? cnt : 0;
+  __syncthreads();
+  int base = 0, chunk = 0;
+  if (on) {
+    for (int j = 0; j < p.n; ++j) {
+      const int c = g.e[j] < e ? g.count[j] : 0;
+      base += (c + 3) & ~3;
+      chunk += (c + NT - 1) / NT;
+    }
+    g.row[i] = e >= 0 ? base + pos : -1;
+  }
+  const int ch = (cnt + NT - 1) / NT;
+  if (first) {
+    atomicMax(&g.chunks, chunk + ch);
+    const int c = mine - chunk;
+    if (c >= 0 && c < ch) g.row0 = base + c * NT, g.rows = min(NT, cnt - c * NT), g.expert = e;
+  }
+  __syncthreads();
+  if (on && g.row[i] >= g.row0 && g.row[i] < g.row0 + g.rows) g.tok[g.row[i] - g.row0] = i / p.k;
+  if (blockIdx.x == 0) {
+    if (e >= 0) p.entry_out[base + pos] = i;
+    if (first)
+      for (int c = 0; c < ch; ++c)
+        p.tiles_out[chunk + c] = make_int4(base + c * NT, min(NT, cnt - c * NT), e, 0);
+    for (int c = i; c < p.nclear; c += blockDim.x) p.clear[c] = 0;
+    if (i == 0) *p.nchunks_out = g.chunks;
+  }
+  __syncthreads();
+}
+
+// kF8Step, kF8StepAct: blocks [kb0, kb1) of `rows` rows (row r is token tok[r],
+// or r without tok), by the eight epilogue warps, into shared memory as a TMA
+// copy with the 128-byte swizzle would lay them out (16 bytes' place within a
+// row of 128 exclusive-or the row's number modulo 8).  Rows past the last keep
+// what they hold: they reach no column that is stored.
 template <int NT, typename T>
-__device__ __forceinline__ void step_quantize(const F8Pass& p, const T* x, int kb0, int kb1,
-                                              uint8_t* s_x, float* s_scale) {
+__device__ __forceinline__ void step_quantize(const F8Pass& p, const T* x, int rows, const int* tok,
+                                              int kb0, int kb1, uint8_t* s_x, float* s_scale) {
   using Raw = decltype(load4(x, true, 4));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (kb1 - kb0 + kQuantBlocks - 1) / kQuantBlocks, units = p.tokens * per;
-  Raw raw[kF8StepUnits][kQuantBlocks];
+  const int per = (kb1 - kb0 + kQuantBlocks - 1) / kQuantBlocks, units = rows * per;
+  for (int u0 = warp; u0 < units; u0 += kF8StepUnits * kF8EpiWarps) {
+    Raw raw[kF8StepUnits][kQuantBlocks];
 #pragma unroll
-  for (int i = 0; i < kF8StepUnits; ++i) {  // every load before the first is used
-    const int u = warp + i * kF8EpiWarps, t = u / per;
-    if (u < units)
-      load_blocks(x + t * p.ldx, p.cols, kb0 + (u - t * per) * kQuantBlocks, p.x_vec, raw[i]);
-  }
+    for (int i = 0; i < kF8StepUnits; ++i) {  // these units' loads before the first is used
+      const int u = u0 + i * kF8EpiWarps, r = u / per;
+      if (u < units)
+        load_blocks(x + (long)(tok ? tok[r] : r) * p.ldx, p.cols, kb0 + (u - r * per) * kQuantBlocks,
+                    p.x_vec, raw[i]);
+    }
 #pragma unroll
-  for (int i = 0; i < kF8StepUnits; ++i) {
-    const int u = warp + i * kF8EpiWarps, t = u / per, b0 = (u - t * per) * kQuantBlocks;
-    if (u >= units) break;
-    const bool mine = lane < kQuantBlocks && kb0 + b0 + lane < kb1;
-    uint32_t w[kQuantBlocks];
-    float s;
-    quant_blocks(raw[i], mine, w, s);
+    for (int i = 0; i < kF8StepUnits; ++i) {
+      const int u = u0 + i * kF8EpiWarps, r = u / per, b0 = (u - r * per) * kQuantBlocks;
+      if (u >= units) break;
+      const bool mine = lane < kQuantBlocks && kb0 + b0 + lane < kb1;
+      uint32_t w[kQuantBlocks];
+      float s;
+      quant_blocks(raw[i], mine, w, s);
 #pragma unroll
-    for (int j = 0; j < kQuantBlocks; ++j)
-      if (kb0 + b0 + j < kb1)
-        *reinterpret_cast<uint32_t*>(s_x + (b0 + j) * (NT * kF8Block) + t * kF8Block +
-                                     (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w[j];
-    if (mine) s_scale[(b0 + lane) * NT + t] = s;
+      for (int j = 0; j < kQuantBlocks; ++j)
+        if (kb0 + b0 + j < kb1)
+          *reinterpret_cast<uint32_t*>(s_x + (b0 + j) * (NT * kF8Block) + r * kF8Block +
+                                       (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = w[j];
+      if (mine) s_scale[(b0 + lane) * NT + r] = s;
+    }
   }
 }
 
@@ -600,9 +611,10 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* s_x = stages + (size_t)C::kStages * C::kStage;  // kF8Step: [block][NT][128], swizzled
-  float* s_scale = reinterpret_cast<float*>(s_x + (C::kStep ? kF8StepBlocks * C::kX : 0));
+  float* s_scale = reinterpret_cast<float*>(s_x + (C::kStep ? C::kStepBlocks * C::kX : 0));
   uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + C::kScales * NT);  // [parity][quadrant][NT]
   F8Sync* sy = reinterpret_cast<F8Sync*>(s_amax + 2 * 4 * NT);
+  F8Group* sg = reinterpret_cast<F8Group*>(sy + 1);  // kF8StepAct
   volatile int* abort = &sy->abort;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -633,10 +645,17 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     griddep_wait();
     griddep_launch();
   }
-  const int ntiles = (p.tiles ? __ldcg(p.nchunks) : p.chunks) * p.rblocks;
   const uint32_t rank = SPLIT ? cluster_rank() : 0;
   const int split = SPLIT ? p.split : 1;
   const int tile0 = (int)blockIdx.x / split, tstep = (int)gridDim.x / split;
+  if constexpr (MODE == kF8StepAct) step_group<NT>(p, *sg, tile0 / p.rblocks);
+  const int ntiles = (MODE == kF8StepAct ? sg->chunks : p.tiles ? __ldcg(p.nchunks) : p.chunks) *
+                     p.rblocks;
+  // (kF8StepAct: one tile a CTA at most)
+  auto tile_at = [&](int tile) {
+    return MODE == kF8StepAct ? F8Tile{sg->row0, sg->rows, sg->expert, tile % p.rblocks}
+                              : f8_tile<NT>(p, tile);
+  };
   const int kb0 = (int)rank * p.kblocks / split, kb1 = ((int)rank + 1) * p.kblocks / split;
   bool synced = false;  // split: this warp has met the others of the cluster
 
@@ -654,7 +673,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     };
     if (early) {  // the first tile's weights while the previous kernel still runs
       if (tile0 < ntiles) {
-        const F8Tile t = f8_tile<NT>(p, tile0);
+        const F8Tile t = tile_at(tile0);
         for (; ahead < C::kStages && kb0 + ahead < kb1; ++ahead)
           if (one) load_weights(ahead, kb0 + ahead, t);
       }
@@ -663,7 +682,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     }
     bool ok = true;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-      const F8Tile t = f8_tile<NT>(p, tile);
+      const F8Tile t = tile_at(tile);
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = q < C::kStages || f8_wait_warp(&sy->empty[rp.s], rp.phase ^ 1u, p.status, abort);
         if (!ok) break;
@@ -684,7 +703,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     int q = 0;
     bool ok = !C::kStep;
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-      const F8Tile t = f8_tile<NT>(p, tile);
+      const F8Tile t = tile_at(tile);
       // row0 and the pitch are multiples of 4; columns past the pitch keep
       // what an earlier tile left and belong to no valid row
       const uint32_t bytes = (uint32_t)min((long)NT, p.xs_pitch - t.row0) * 4u;
@@ -709,7 +728,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     const uint64_t desc = sw128_desc(stages), xdesc = sw128_desc(s_x);
     if (C::kStep) ok = f8_wait_warp(&sy->xfull, 0, p.status, abort);
     for (int tile = tile0; tile < ntiles && ok; tile += tstep) {
-      const F8Tile t = f8_tile<NT>(p, tile);
+      const F8Tile t = tile_at(tile);
       const uint32_t idesc = f8_idesc((t.count + 15) & ~15);
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = (q < C::kBufs || f8_wait_warp(&sy->tempty[ap.s], ap.phase ^ 1u, p.status, abort)) &&
@@ -746,10 +765,13 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     bool ok = true;
     int parity = 0;
     if constexpr (C::kStep) {
+      const int rows = MODE == kF8StepAct ? sg->rows : p.tokens;
+      const int* tok = MODE == kF8StepAct ? sg->tok : nullptr;
       if (p.x_bf16)
-        step_quantize<NT>(p, static_cast<const __nv_bfloat16*>(p.x), kb0, kb1, s_x, s_scale);
+        step_quantize<NT>(p, static_cast<const __nv_bfloat16*>(p.x), rows, tok, kb0, kb1, s_x,
+                          s_scale);
       else
-        step_quantize<NT>(p, static_cast<const float*>(p.x), kb0, kb1, s_x, s_scale);
+        step_quantize<NT>(p, static_cast<const float*>(p.x), rows, tok, kb0, kb1, s_x, s_scale);
       fence_proxy_async_smem();  // the MMAs read what these threads wrote
       __syncwarp();
       if (lane == 0) mbar_arrive(&sy->xfull);
@@ -760,7 +782,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
            i += (long)gridDim.x * kF8EpiWarps * 32)
         store_out(p.out, p.out_bf16, i / p.rows * p.ldo + i % p.rows, 0.0f);
     for (int tile = tile0; tile < ntiles && ok; tile += tstep, parity ^= 1) {
-      const F8Tile t = f8_tile<NT>(p, tile);
+      const F8Tile t = tile_at(tile);
       // this thread's tokens: groups of 8 columns in turn with the other half's,
       // so that both have their share of a tile that is not full
       auto col = [&](int c) { return (2 * (c >> 3) + half) * 8 + (c & 7); };
@@ -1498,7 +1520,8 @@ cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_
   const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : std::min(tiles, slots)));
+  cfg.gridDim = dim3((unsigned)(p.split > 1 || MODE == kF8StepAct ? tiles * p.split
+                                                                  : std::min(tiles, slots)));
   cfg.blockDim = dim3(kF8Threads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
@@ -1537,12 +1560,9 @@ cudaError_t quant_t(const T* x, long ldx, int tokens, int cols, uint8_t* q, long
   const int vec = ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
   const long per = (f8_blocks(cols) + kQuantBlocks - 1) / kQuantBlocks;
   const long units = (rows.sel ? (long)tokens : s_pitch) * per;
-  const bool self = rows.sel && !rows.pos;
   if (units > 0x3fffffffL) return cudaErrorInvalidValue;
   const long ctas = (units + 7) / 8;
-  auto kern = self       ? f8_quant_kernel<T, kQuantSelf>
-              : rows.sel ? f8_quant_kernel<T, kQuantGrouped>
-                         : f8_quant_kernel<T, kQuantRows>;
+  auto kern = rows.sel ? f8_quant_kernel<T, true> : f8_quant_kernel<T, false>;
   return launch_pdl(kern, dim3((unsigned)ctas), dim3(256), 0, st, x, ldx, tokens, cols, q,
                     (int)q_pitch, scales, (int)s_pitch, rows, vec);
 }
@@ -1572,11 +1592,16 @@ cudaError_t f8_prepare(F8Matrix* w) {
   return f8_weight_map(&w->map, *w) ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Rows of x that four consecutive values can be loaded from at once.
+static bool f8_rows_vec(bool bf16, const void* x, long ldx, int tokens) {
+  return (tokens == 1 || ldx % 4 == 0) && reinterpret_cast<uintptr_t>(x) % (bf16 ? 8 : 16) == 0;
+}
+
 bool f8_step_applies(const F8Matrix& w, int tokens) {
   if (tokens > 16) return false;
   const int kb = f8_blocks(w.cols);
   const int most = (kb + f8_split(f8_blocks(w.rows), kb) - 1) / f8_split(f8_blocks(w.rows), kb);
-  return most <= kF8StepBlocks &&
+  return most <= F8Cfg<16, 1, kF8Step>::kStepBlocks &&
          tokens * ((most + kQuantBlocks - 1) / kQuantBlocks) <= kF8StepUnits * kF8EpiWarps;
 }
 
@@ -1595,8 +1620,7 @@ cudaError_t launch_f8_step(const F8Matrix& w, bool x_bf16, const void* x, long l
   p.ldx = ldx;
   p.cols = w.cols;
   p.x_bf16 = x_bf16;
-  p.x_vec = (tokens == 1 || ldx % 4 == 0) &&
-            reinterpret_cast<uintptr_t>(x) % (x_bf16 ? 8 : 16) == 0;
+  p.x_vec = f8_rows_vec(x_bf16, x, ldx, tokens);
   p.out = out;
   p.ldo = ldo;
   p.out_bf16 = out_bf16;
@@ -1685,26 +1709,32 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   // chunks of an expert's tokens: half again the average, so most experts take one
   const int nt = f8_chunk((3 * n / std::min<long>(n, m.up.experts) + 1) / 2);
   const long chunks = n / nt + std::min<long>(n, m.up.experts);
-  // A call so small that the down product has one tile a CTA at most takes three
-  // launches instead of five: the quantiser groups the entries, and the down
-  // product's CTAs add them up (one token, 10 of 512 experts: 27 us against 31).
-  // With more tiles the fence after each, and the weights that the plan's own
-  // launch lets the gate and up product request ahead, cost more (32 tokens, 6
-  // of 128 experts of 2688 x 1856: 215 us against 157).
-  const bool few = n <= kSelfEntries && nt == 16 &&
-                   chunks * f8_blocks(m.down.rows) <= (long)sm_count() * F8Cfg<16, 1, kF8Partial>::kCtas;
+  // A call so small that the down product has one tile a CTA at most takes two
+  // launches instead of five: every CTA of the gate and up product groups the
+  // entries and quantises its rows for itself, and the down product's CTAs add
+  // the entries up (one token, 10 of 512 experts: __FEW__).  With more tiles the
+  // fence after each, and the weights that the plan's own launch lets the gate
+  // and up product request ahead, cost more (32 tokens, 6 of 128 experts of 2688 x
+  // 1856: 215 us against 157).
+  const int kb_up = f8_blocks(m.up.cols), rb_up = f8_blocks(m.up.rows);
+  const int split_up = f8_split(chunks * rb_up, kb_up);
+  const bool few = n <= kF8StepEntries && nt == 16 &&
+                   (kb_up + split_up - 1) / split_up <=
+                       (m.gate.data ? F8Cfg<16, 2, kF8StepAct>::kStepBlocks
+                                    : F8Cfg<16, 1, kF8StepAct>::kStepBlocks) &&
+                   chunks * f8_blocks(m.down.rows) <=
+                       (long)sm_count() * F8Cfg<16, 1, kF8Partial>::kCtas;
   int* counters = few ? reinterpret_cast<int*>(base + L.counters) : nullptr;
   cudaError_t e = cudaSuccess;
   if (!few) {
     e = launch_pdl(f8_plan_kernel, dim3(1), dim3(1024), 0, st, sel, (int)n, m.up.experts, nt, pos,
                    row_start, tiles, nchunks);
     if (e != cudaSuccess) return e;
+    const F8Rows rows{sel, pos, row_start, entry, k, m.up.experts};
+    e = quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
+              reinterpret_cast<float*>(base + L.xs), L.rows, rows, st);
+    if (e != cudaSuccess) return e;
   }
-  const F8Rows rows{sel, few ? nullptr : pos, row_start, entry, k, m.up.experts, (int)n, nt,
-                    few ? f8_blocks(m.down.rows) : 0, tiles, nchunks, counters};
-  e = quant(x_bf16, x, ldx, tokens, m.up.cols, base + L.xq, f8_pad16(m.up.cols),
-            reinterpret_cast<float*>(base + L.xs), L.rows, rows, st);
-  if (e != cudaSuccess) return e;
   F8Maps maps;
   F8Pass p{};
   maps.w0 = m.gate.data ? m.gate.map : m.up.map;
@@ -1724,10 +1754,32 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   p.h_pitch = L.hp;
   p.hs = reinterpret_cast<float*>(base + L.hs);
   p.hs_pitch = L.rows;
-  p.early = !few;  // the quantiser writes the tiles when it groups the entries
+  p.early = 1;
   p.status = status;
-  e = m.gate.data ? launch_f8_pass<2, kF8Act>(nt, maps, p, chunks * p.rblocks, st)
-                  : launch_f8_pass<1, kF8Act>(nt, maps, p, chunks * p.rblocks, st);
+  if (few) {
+    p.early = 0;
+    p.tiles = nullptr;
+    p.x = x;
+    p.ldx = ldx;
+    p.cols = m.up.cols;
+    p.x_bf16 = x_bf16;
+    p.x_vec = f8_rows_vec(x_bf16, x, ldx, tokens);
+    p.sel = sel;
+    p.k = k;
+    p.E = m.up.experts;
+    p.n = (int)n;
+    p.tiles_out = tiles;
+    p.nchunks_out = nchunks;
+    p.entry_out = entry;
+    p.clear = counters;
+    p.nclear = f8_blocks(m.down.rows);
+    // one CTA (or cluster) a tile: a CTA quantises the rows of one
+    e = m.gate.data ? launch_f8_gemm<16, 2, kF8StepAct>(maps, p, chunks * p.rblocks, st)
+                    : launch_f8_gemm<16, 1, kF8StepAct>(maps, p, chunks * p.rblocks, st);
+  } else {
+    e = m.gate.data ? launch_f8_pass<2, kF8Act>(nt, maps, p, chunks * p.rblocks, st)
+                    : launch_f8_pass<1, kF8Act>(nt, maps, p, chunks * p.rblocks, st);
+  }
   if (e != cudaSuccess) return e;
   F8Pass d{};
   maps.w0 = maps.w1 = m.down.map;
@@ -1753,7 +1805,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   d.out = out;
   d.ldo = ldo;
   d.out_bf16 = out_bf16;
-  d.early = 1;
+  d.early = !few;  // else the kernel before writes the tiles
   d.status = status;
   e = launch_f8_pass<1, kF8Partial>(nt, maps, d, chunks * d.rblocks, st);
   if (e != cudaSuccess || few) return e;
