@@ -44,6 +44,8 @@ enum F8Mode {
   kF8Act,      // activation of gate and up, quantised: the down product's input
   kF8StepAct,  // the same for few entries, which every CTA groups and quantises for itself
   kF8Partial,  // y to the row of its (token, rank) entry
+  kF8StepPartial,  // the same for few entries, which every CTA groups for itself; the
+                   // last CTA of a row block adds up the block's columns of out
 };
 
 // e4m3 of v as a byte: round to nearest even, NaN stays NaN.
@@ -282,12 +284,11 @@ struct F8Pass {
   const void* x;                 // kF8Step, kF8StepAct: the rows themselves
   long ldx;
   int cols, x_bf16, x_vec;
-  // kF8StepAct: what the first CTA writes for the down product: its tiles, the
-  // entry of each row, and zeroes in nclear counters
-  int4* tiles_out;
-  int *nchunks_out, *entry_out, *clear;
+  // few entries: their number, and a counter for each row block of the down
+  // product (kF8StepAct zeroes the nclear counters)
   int n, nclear;
-  void* out;                     // kF8Out, kF8Step
+  int* counters;
+  void* out;                     // kF8Out, kF8Step, kF8StepPartial
   long ldo;
   int out_bf16;
   uint8_t* hq;                   // kF8Act: quantised activations and their scales
@@ -297,9 +298,6 @@ struct F8Pass {
   float* partial;                // kF8Partial: rows of partial by entry
   long ldp;
   const int* entry;
-  // kF8Partial with few entries: the last of a row block's CTAs to arrive at
-  // its counter adds up the block's columns of out (null: f8_combine_kernel does)
-  int* counters;
   const int* sel;
   const float* weights;
   int k, E;
@@ -317,11 +315,11 @@ struct F8Sync {
   int abort, last;
 };
 
-// kF8StepAct: the grouping of up to kF8StepEntries entries by expert, as
-// f8_plan_kernel has it, and this CTA's tile of it.
+// kF8StepAct, kF8StepPartial: the grouping of up to kF8StepEntries entries by
+// expert, as f8_plan_kernel has it, and this CTA's tile of it.
 struct F8Group {
   int e[kF8StepEntries], count[kF8StepEntries], row[kF8StepEntries];
-  int tok[16];  // token of each row of the tile
+  int ent[16], tok[16];  // entry and token of each row of the tile
   int chunks, row0, rows, expert;
 };
 
@@ -331,21 +329,25 @@ struct F8Group {
 template <int NT, int MATS, int MODE>
 struct F8Cfg {
   static constexpr bool kStep = MODE == kF8Step || MODE == kF8StepAct;
-  static constexpr int kCtas = kStep || (NT == 64 && MATS == 2) ? 1 : 2;
+  static constexpr bool kGroup = MODE == kF8StepAct || MODE == kF8StepPartial;
+  static constexpr bool kPartial = MODE == kF8Partial || MODE == kF8StepPartial;
+  static constexpr int kCtas = MODE == kF8Step || (NT == 64 && MATS == 2) ? 1 : 2;
   static constexpr uint32_t kA = kF8M * kF8Block;        // bytes of one weight tile
   static constexpr uint32_t kX = NT * kF8Block;          // and of one block of activations
   static constexpr uint32_t kStage = MATS * kA + (kStep ? 0 : kX);
   static constexpr uint32_t kBudget =
-      kStep ? (MATS == 2 ? 4 : 5) * kStage : (kCtas == 2 ? 104u : 200u) * 1024u;
+      MODE == kF8Step ? 5 * kStage : kStep ? 64u * 1024u : (kCtas == 2 ? 104u : 200u) * 1024u;
   static constexpr int kStages = (int)(kBudget / kStage);
-  static constexpr int kStepBlocks = MATS == 2 ? 40 : 64;  // blocks of K a CTA quantises, at most
+  // blocks of K a CTA quantises, at most: kF8StepAct leaves room for a CTA of the
+  // down product, which requests its weights while it waits
+  static constexpr int kStepBlocks = MODE == kF8Step ? 64 : 21;
   static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
   static constexpr int kBufs = 512 / kAcc / kCtas > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc / kCtas;
   static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
   static constexpr int kScales = kStep ? kStepBlocks : kF8Scales;  // blocks of scales staged
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (kStep ? kStepBlocks * kX : 0) +
                                   kScales * NT * 4 + 2 * 4 * NT * 4 + sizeof(F8Sync) +
-                                  (MODE == kF8StepAct ? sizeof(F8Group) : 0);
+                                  (kGroup ? sizeof(F8Group) : 0);
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -506,7 +508,8 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
 // itself, as f8_plan_kernel does: entry i counts the entries of its expert
 // before it and in all, then the rows and chunks (of NT) of the experts before
 // its own.  Entries whose expert is outside [0, E) are in no group.  Leaves the
-// rows of chunk `mine` and their tokens in g (rows 0: there is no such chunk).
+// rows of chunk `mine`, their entries and tokens in g (rows 0: there is no such
+// chunk).
 template <int NT>
 __device__ __forceinline__ void step_group(const F8Pass& p, F8Group& g, int mine) {
   const int i = threadIdx.x;
@@ -542,14 +545,9 @@ __device__ __forceinline__ void step_group(const F8Pass& p, F8Group& g, int mine
     if (c >= 0 && c < ch) g.row0 = base + c * NT, g.rows = min(NT, cnt - c * NT), g.expert = e;
   }
   __syncthreads();
-  if (on && g.row[i] >= g.row0 && g.row[i] < g.row0 + g.rows) g.tok[g.row[i] - g.row0] = i / p.k;
-  if (blockIdx.x == 0) {
-    if (e >= 0) p.entry_out[base + pos] = i;
-    if (first)
-      for (int c = 0; c < ch; ++c)
-        p.tiles_out[chunk + c] = make_int4(base + c * NT, min(NT, cnt - c * NT), e, 0);
-    for (int c = i; c < p.nclear; c += blockDim.x) p.clear[c] = 0;
-    if (i == 0) *p.nchunks_out = g.chunks;
+  if (on && g.row[i] >= g.row0 && g.row[i] < g.row0 + g.rows) {
+    g.ent[g.row[i] - g.row0] = i;
+    g.tok[g.row[i] - g.row0] = i / p.k;
   }
   __syncthreads();
 }
@@ -559,23 +557,23 @@ __device__ __forceinline__ void step_group(const F8Pass& p, F8Group& g, int mine
 // copy with the 128-byte swizzle would lay them out (16 bytes' place within a
 // row of 128 exclusive-or the row's number modulo 8).  Rows past the last keep
 // what they hold: they reach no column that is stored.
-template <int NT, typename T>
+template <int NT, int UNITS, typename T>
 __device__ __forceinline__ void step_quantize(const F8Pass& p, const T* x, int rows, const int* tok,
                                               int kb0, int kb1, uint8_t* s_x, float* s_scale) {
   using Raw = decltype(load4(x, true, 4));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (kb1 - kb0 + kQuantBlocks - 1) / kQuantBlocks, units = rows * per;
-  for (int u0 = warp; u0 < units; u0 += kF8StepUnits * kF8EpiWarps) {
-    Raw raw[kF8StepUnits][kQuantBlocks];
+  for (int u0 = warp; u0 < units; u0 += UNITS * kF8EpiWarps) {
+    Raw raw[UNITS][kQuantBlocks];
 #pragma unroll
-    for (int i = 0; i < kF8StepUnits; ++i) {  // these units' loads before the first is used
+    for (int i = 0; i < UNITS; ++i) {  // these units' loads before the first is used
       const int u = u0 + i * kF8EpiWarps, r = u / per;
       if (u < units)
         load_blocks(x + (long)(tok ? tok[r] : r) * p.ldx, p.cols, kb0 + (u - r * per) * kQuantBlocks,
                     p.x_vec, raw[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kF8StepUnits; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
       const int u = u0 + i * kF8EpiWarps, r = u / per, b0 = (u - r * per) * kQuantBlocks;
       if (u >= units) break;
       const bool mine = lane < kQuantBlocks && kb0 + b0 + lane < kb1;
@@ -614,7 +612,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
   float* s_scale = reinterpret_cast<float*>(s_x + (C::kStep ? C::kStepBlocks * C::kX : 0));
   uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_scale + C::kScales * NT);  // [parity][quadrant][NT]
   F8Sync* sy = reinterpret_cast<F8Sync*>(s_amax + 2 * 4 * NT);
-  F8Group* sg = reinterpret_cast<F8Group*>(sy + 1);  // kF8StepAct
+  F8Group* sg = reinterpret_cast<F8Group*>(sy + 1);
   volatile int* abort = &sy->abort;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -640,21 +638,27 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sy->tmem, 0);
+  const uint32_t rank = SPLIT ? cluster_rank() : 0;
+  const int split = SPLIT ? p.split : 1;
+  const int tile0 = (int)blockIdx.x / split, tstep = (int)gridDim.x / split;
+  // the entries are not the kernel before's output when that is kF8StepAct, which has read them
+  if constexpr (MODE == kF8StepPartial) step_group<NT>(p, *sg, tile0 / p.rblocks);
   const bool early = p.early && warp == kF8EpiWarps;
   if (!early) {
     griddep_wait();
     griddep_launch();
   }
-  const uint32_t rank = SPLIT ? cluster_rank() : 0;
-  const int split = SPLIT ? p.split : 1;
-  const int tile0 = (int)blockIdx.x / split, tstep = (int)gridDim.x / split;
-  if constexpr (MODE == kF8StepAct) step_group<NT>(p, *sg, tile0 / p.rblocks);
-  const int ntiles = (MODE == kF8StepAct ? sg->chunks : p.tiles ? __ldcg(p.nchunks) : p.chunks) *
-                     p.rblocks;
-  // (kF8StepAct: one tile a CTA at most)
+  if constexpr (MODE == kF8StepAct) {
+    step_group<NT>(p, *sg, tile0 / p.rblocks);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i < p.nclear; i += kF8Threads) p.counters[i] = 0;
+  }
+  const int ntiles =
+      (C::kGroup ? sg->chunks : p.tiles ? __ldcg(p.nchunks) : p.chunks) * p.rblocks;
+  // (kGroup: one tile a CTA at most)
   auto tile_at = [&](int tile) {
-    return MODE == kF8StepAct ? F8Tile{sg->row0, sg->rows, sg->expert, tile % p.rblocks}
-                              : f8_tile<NT>(p, tile);
+    return C::kGroup ? F8Tile{sg->row0, sg->rows, sg->expert, tile % p.rblocks}
+                     : f8_tile<NT>(p, tile);
   };
   const int kb0 = (int)rank * p.kblocks / split, kb1 = ((int)rank + 1) * p.kblocks / split;
   bool synced = false;  // split: this warp has met the others of the cluster
@@ -765,19 +769,22 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
     bool ok = true;
     int parity = 0;
     if constexpr (C::kStep) {
+      // (an expert of few entries has a row or two: one unit a warp mostly)
+      constexpr int kUnits = MODE == kF8StepAct ? 1 : kF8StepUnits;
       const int rows = MODE == kF8StepAct ? sg->rows : p.tokens;
       const int* tok = MODE == kF8StepAct ? sg->tok : nullptr;
       if (p.x_bf16)
-        step_quantize<NT>(p, static_cast<const __nv_bfloat16*>(p.x), rows, tok, kb0, kb1, s_x,
-                          s_scale);
+        step_quantize<NT, kUnits>(p, static_cast<const __nv_bfloat16*>(p.x), rows, tok, kb0, kb1,
+                                  s_x, s_scale);
       else
-        step_quantize<NT>(p, static_cast<const float*>(p.x), rows, tok, kb0, kb1, s_x, s_scale);
+        step_quantize<NT, kUnits>(p, static_cast<const float*>(p.x), rows, tok, kb0, kb1, s_x,
+                                  s_scale);
       fence_proxy_async_smem();  // the MMAs read what these threads wrote
       __syncwarp();
       if (lane == 0) mbar_arrive(&sy->xfull);
       named_bar_sync(3, kF8EpiWarps * 32);  // and all of them the scales
     }
-    if (MODE == kF8Partial && NT == 16 && p.counters && ntiles == 0)  // no entry is anyone's
+    if (MODE == kF8StepPartial && ntiles == 0)  // no entry is anyone's
       for (long i = (long)blockIdx.x * kF8EpiWarps * 32 + threadIdx.x; i < (long)p.tokens * p.rows;
            i += (long)gridDim.x * kF8EpiWarps * 32)
         store_out(p.out, p.out_bf16, i / p.rows * p.ldo + i % p.rows, 0.0f);
@@ -796,12 +803,12 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
       auto own = [&](int c) { return !SPLIT || (c & (p.split - 1)) == (int)rank; };
       float wl[MATS];  // weight scales of 32 blocks, one a lane
       int ent[(NC + 31) / 32];  // entries of this thread's tokens, 32 a register
-      if (MODE == kF8Partial) {
+      if (C::kPartial) {
 #pragma unroll
         for (int i = 0; i < (NC + 31) / 32; ++i)
-          ent[i] = 32 * i + lane < NC && in(32 * i + lane)
-                       ? __ldcg(p.entry + t.row0 + col(32 * i + lane))
-                       : 0;
+          ent[i] = 32 * i + lane >= NC || !in(32 * i + lane) ? 0
+                   : MODE == kF8StepPartial ? sg->ent[col(32 * i + lane)]
+                                            : __ldcg(p.entry + t.row0 + col(32 * i + lane));
       }
       for (int kb = kb0; kb < kb1; ++kb) {
         if (((kb - kb0) & 31) == 0) {
@@ -864,7 +871,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
       if (SPLIT) {
         // every product of this CTA is in registers, so the stages are free; CTA
         // `rank` finishes the columns that are `rank` modulo split, adding the
-        // others' sums to its own in the order of their ranks from its own on
+        // CTAs' sums in rank order whoever adds them
         float* red = reinterpret_cast<float*>(stages) + r;
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
@@ -879,16 +886,16 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
 #pragma unroll
           for (int c = 0; c < NC; ++c)
             if (in(c) && own(c)) {  // warp-uniform
+              const float here = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
               float v[kF8MaxSplit];
 #pragma unroll
-              for (int k = 1; k < kF8MaxSplit; ++k)
-                if (k < split)
-                  v[k] = cluster_ld(
-                      cluster_map(red + (m * NT + col(c)) * kF8M, (rank + k) & (split - 1)));
-              float y = c & 1 ? acc[m][c / 2].y : acc[m][c / 2].x;
+              for (int k = 0; k < kF8MaxSplit; ++k)
+                if (k < split && k != (int)rank)
+                  v[k] = cluster_ld(cluster_map(red + (m * NT + col(c)) * kF8M, k));
+              float y = 0.0f;
 #pragma unroll
-              for (int k = 1; k < kF8MaxSplit; ++k)
-                if (k < split) y += v[k];
+              for (int k = 0; k < kF8MaxSplit; ++k)
+                if (k < split) y += k == (int)rank ? here : v[k];
               if (c & 1)
                 acc[m][c / 2].y = y;
               else
@@ -905,7 +912,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
               store_out(p.out, p.out_bf16, (long)(t.row0 + col(c)) * p.ldo + row, y);
             }
         }
-      } else if (MODE == kF8Partial) {
+      } else if (C::kPartial) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           if (in(c) && own(c)) {  // warp-uniform
@@ -913,7 +920,7 @@ __global__ void __launch_bounds__(kF8Threads, (F8Cfg<NT, MATS, MODE>::kCtas))
             const long id = __shfl_sync(0xffffffffu, ent[c / 32], c & 31);
             if (row < p.rows) p.partial[id * p.ldp + row] = y;
           }
-        if (NT == 16 && p.counters) {
+        if (MODE == kF8StepPartial) {
           __threadfence();
           named_bar_sync(3, kF8EpiWarps * 32);
           if (threadIdx.x == 0)
@@ -1520,7 +1527,7 @@ cudaError_t launch_f8_gemm(const F8Maps& maps, F8Pass p, long tiles, cudaStream_
   const cudaError_t e = f8_allow_smem(reinterpret_cast<const void*>(kern), C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.split > 1 || MODE == kF8StepAct ? tiles * p.split
+  cfg.gridDim = dim3((unsigned)(p.split > 1 || C::kGroup ? tiles * p.split
                                                                   : std::min(tiles, slots)));
   cfg.blockDim = dim3(kF8Threads);
   cfg.dynamicSmemBytes = C::kSmem;
@@ -1712,7 +1719,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   // A call so small that the down product has one tile a CTA at most takes two
   // launches instead of five: every CTA of the gate and up product groups the
   // entries and quantises its rows for itself, and the down product's CTAs add
-  // the entries up (one token, 10 of 512 experts: __FEW__).  With more tiles the
+  // the entries up (one token, 10 of 512 experts: 18 us against 31).  With more tiles the
   // fence after each, and the weights that the plan's own launch lets the gate
   // and up product request ahead, cost more (32 tokens, 6 of 128 experts of 2688 x
   // 1856: 215 us against 157).
@@ -1723,7 +1730,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
                        (m.gate.data ? F8Cfg<16, 2, kF8StepAct>::kStepBlocks
                                     : F8Cfg<16, 1, kF8StepAct>::kStepBlocks) &&
                    chunks * f8_blocks(m.down.rows) <=
-                       (long)sm_count() * F8Cfg<16, 1, kF8Partial>::kCtas;
+                       (long)sm_count() * F8Cfg<16, 1, kF8StepPartial>::kCtas;
   int* counters = few ? reinterpret_cast<int*>(base + L.counters) : nullptr;
   cudaError_t e = cudaSuccess;
   if (!few) {
@@ -1768,10 +1775,7 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
     p.k = k;
     p.E = m.up.experts;
     p.n = (int)n;
-    p.tiles_out = tiles;
-    p.nchunks_out = nchunks;
-    p.entry_out = entry;
-    p.clear = counters;
+    p.counters = counters;
     p.nclear = f8_blocks(m.down.rows);
     // one CTA (or cluster) a tile: a CTA quantises the rows of one
     e = m.gate.data ? launch_f8_gemm<16, 2, kF8StepAct>(maps, p, chunks * p.rblocks, st)
@@ -1796,19 +1800,24 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   d.partial = partial;
   d.ldp = L.ldp;
   d.entry = entry;
-  d.counters = counters;
-  d.sel = sel;
-  d.weights = weights;
-  d.k = k;
-  d.E = m.up.experts;
-  d.tokens = tokens;
-  d.out = out;
-  d.ldo = ldo;
-  d.out_bf16 = out_bf16;
-  d.early = !few;  // else the kernel before writes the tiles
+  d.early = 1;
   d.status = status;
+  if (few) {
+    d.tiles = nullptr;
+    d.n = (int)n;
+    d.counters = counters;
+    d.sel = sel;
+    d.weights = weights;
+    d.k = k;
+    d.E = m.up.experts;
+    d.tokens = tokens;
+    d.out = out;
+    d.ldo = ldo;
+    d.out_bf16 = out_bf16;
+    return launch_f8_gemm<16, 1, kF8StepPartial>(maps, d, chunks * d.rblocks, st);
+  }
   e = launch_f8_pass<1, kF8Partial>(nt, maps, d, chunks * d.rblocks, st);
-  if (e != cudaSuccess || few) return e;
+  if (e != cudaSuccess) return e;
   const unsigned gy = (unsigned)std::max(1, std::min((m.down.rows + 1023) / 1024, 64));
   return launch_pdl(f8_combine_kernel, dim3((unsigned)tokens, gy), dim3(256), 0, st, partial,
                     L.ldp, sel, m.up.experts, weights, k, m.down.rows, out, ldo, (int)out_bf16);

@@ -304,6 +304,35 @@ def test_projection_from_host(N, K):
     assert np.array_equal(p.run(x[3].cpu().numpy()), p.run_device(x[3:4]).cpu().numpy()[0])
 
 
+@pytest.mark.parametrize("T,N,K", [(3, 128, 8192), (16, 300, 4096), (50, 128, 4112),
+                                   (300, 128, 2064), (600, 5000, 400)])
+def test_rows_do_not_depend_on_their_place(T, N, K):
+    """The same rows in another order give the same bits, long K shared by CTAs too."""
+    g = gen(T + K)
+    w, s = matrices(g, N, K)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    x = randn(g, T, K)
+    order = torch.randperm(T, generator=g, device="cuda")
+    assert torch.equal(p.run_device(x[order].contiguous()), p.run_device(x)[order])
+
+
+def test_experts_rows_do_not_depend_on_their_place():
+    g = gen(27)
+    E, k, H, I = 3, 2, 2048, 1552
+    up, down, gate = matrices(g, E, I, H), matrices(g, E, 400, I), matrices(g, E, I, H)
+    for gated in (gate, None):
+        m = LB.Fp8MoeSession.from_device(up=up, down=down, gate=gated)
+        for T in (2, 20, 140):
+            x, wt = randn(g, T, H), randn(g, T, k)
+            sel = torch.randint(0, E, (T, k), generator=g, device="cuda").int()
+            order = torch.randperm(T, generator=g, device="cuda")
+            want = m.run_device(x, sel, wt)
+            got = m.run_device(x[order].contiguous(), sel[order].contiguous(),
+                               wt[order].contiguous())
+            assert torch.equal(got, want[order])
+            assert torch.equal(m.run_device(x, sel, wt), want)
+
+
 def test_projection_views_leave_the_rest_alone():
     g = gen(11)
     w, s = matrices(g, 200, 160)
