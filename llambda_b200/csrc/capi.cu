@@ -1626,7 +1626,7 @@ int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor, int o
 void llambda_cuda_fp8_session_destroy(llambda_cuda_fp8_session* session) { destroy_owner(session); }
 
 size_t llambda_cuda_fp8_session_workspace(const llambda_cuda_fp8_session* s, size_t tokens) {
-  if (!s || !tokens || (tokens <= 16 && lb::f8_step_applies(s->w, (int)tokens))) return 0;
+  if (!s || !tokens || (tokens <= 32 && lb::f8_step_applies(s->w, (int)tokens))) return 0;
   return f8_quant_bytes(s->w.cols, tokens, nullptr);
 }
 

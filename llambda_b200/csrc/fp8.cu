@@ -37,6 +37,8 @@ constexpr int kF8MaxSplit = 8;    // CTAs of a cluster that share a tile's K,
 constexpr int kF8SplitBlocks = 3; // with at least this many blocks each
 constexpr int kF8StepUnits = 4;   // (row, four blocks) pairs of a warp that quantises, at a time
 constexpr int kF8StepEntries = 256;  // entries that a CTA groups for itself
+constexpr int kF8StepMost = 48;   // such pairs of a CTA, at most,
+constexpr int kF8StepTokens = 32; // and tokens (33 to 64 gained by the smallest matrices alone)
 
 enum F8Mode {
   kF8Out,      // y to out (fp32 or bf16)
@@ -340,7 +342,7 @@ struct F8Cfg {
   static constexpr int kStages = (int)(kBudget / kStage);
   // blocks of K a CTA quantises, at most: kF8StepAct leaves room for a CTA of the
   // down product, which requests its weights while it waits
-  static constexpr int kStepBlocks = MODE == kF8Step ? 64 : 21;
+  static constexpr int kStepBlocks = MODE == kF8Step ? 128 * 1024 / (int)kX : 21;
   static constexpr uint32_t kAcc = NT * MATS;            // tensor-memory columns of one buffer
   static constexpr int kBufs = 512 / kAcc / kCtas > kF8MaxBuf ? kF8MaxBuf : 512 / kAcc / kCtas;
   static constexpr uint32_t kCols = kBufs * kAcc < 32 ? 32 : kBufs * kAcc;
@@ -1604,12 +1606,17 @@ static bool f8_rows_vec(bool bf16, const void* x, long ldx, int tokens) {
   return (tokens == 1 || ldx % 4 == 0) && reinterpret_cast<uintptr_t>(x) % (bf16 ? 8 : 16) == 0;
 }
 
+// One launch and no workspace against two, for what every CTA does over again.
+// By 4096 x 4096 (8 blocks a CTA) 24 tokens, 48 pairs, take 12.0 us and 15.4 in
+// two launches; by 14336 x 4096 (32 blocks) 8 tokens, 64 pairs, 17.9 and 15.0.
 bool f8_step_applies(const F8Matrix& w, int tokens) {
-  if (tokens > 16) return false;
-  const int kb = f8_blocks(w.cols);
-  const int most = (kb + f8_split(f8_blocks(w.rows), kb) - 1) / f8_split(f8_blocks(w.rows), kb);
-  return most <= F8Cfg<16, 1, kF8Step>::kStepBlocks &&
-         tokens * ((most + kQuantBlocks - 1) / kQuantBlocks) <= kF8StepUnits * kF8EpiWarps;
+  const int nt = f8_chunk(tokens), kb = f8_blocks(w.cols);
+  if (tokens > kF8StepTokens) return false;
+  const int split = f8_split(f8_blocks(w.rows), kb), most = (kb + split - 1) / split;
+  const int room =
+      nt == 16 ? F8Cfg<16, 1, kF8Step>::kStepBlocks : F8Cfg<32, 1, kF8Step>::kStepBlocks;
+  return most <= room &&
+         tokens * ((most + kQuantBlocks - 1) / kQuantBlocks) <= kF8StepMost;
 }
 
 cudaError_t launch_f8_step(const F8Matrix& w, bool x_bf16, const void* x, long ldx, int tokens,
@@ -1632,7 +1639,8 @@ cudaError_t launch_f8_step(const F8Matrix& w, bool x_bf16, const void* x, long l
   p.ldo = ldo;
   p.out_bf16 = out_bf16;
   p.status = status;
-  return launch_f8_gemm<16, 1, kF8Step>(maps, p, p.rblocks, st);
+  return f8_chunk(tokens) == 16 ? launch_f8_gemm<16, 1, kF8Step>(maps, p, p.rblocks, st)
+                                : launch_f8_gemm<32, 1, kF8Step>(maps, p, p.rblocks, st);
 }
 
 cudaError_t launch_f8_project(const F8Matrix& w, const uint8_t* q, const float* scales, int tokens,

@@ -266,7 +266,8 @@ SIZES = [(1, 1, 16), (1, 300, 400), (2, 128, 128), (5, 64, 112), (16, 130, 1040)
          (513, 1030, 272), (1, 4096, 4096), (31, 4096, 8192), (48, 200, 4112), (100, 128, 4096),
          (127, 2700, 528), (300, 20000, 272), (257, 19000, 144), (1025, 5000, 400),
          (1, 20000, 8192), (4, 300, 4096), (3, 128, 8208), (2, 20000, 8208), (16, 640, 1024),
-         (7, 130, 16), (1, 1000, 16400)]
+         (7, 130, 16), (1, 1000, 16400),
+         (24, 4096, 4096), (32, 2688, 512), (17, 130, 1536), (31, 256, 144)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
