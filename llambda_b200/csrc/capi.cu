@@ -1371,6 +1371,30 @@ void require_operand(int type, const void* p, int64_t ld, size_t tokens, uint64_
     throw Failure(std::string(what) + ": the row stride is smaller than a row.");
 }
 
+struct Rows {  // rows of a call's operand: where, bytes between them and of one, how many
+  const void* p;
+  size_t pitch, width, count;
+};
+
+Rows rows_of(const void* p, int type, int64_t ld, size_t tokens, size_t cols) {
+  const size_t size = type == LLAMBDA_CUDA_TYPE_BF16 ? 2 : 4;
+  return {p, tokens > 1 ? (size_t)ld * size : cols * size, cols * size, tokens};
+}
+
+// An output must not share a byte with an input: some kernels still read the
+// one when others write the other.  (Column ranges of one buffer share none.)
+void require_apart(const Rows& out, const Rows& in, const char* what) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
+  if (a + (out.count - 1) * out.pitch + out.width <= b ||
+      b + (in.count - 1) * in.pitch + in.width <= a)
+    return;
+  if (out.pitch == in.pitch) {
+    const size_t d = a >= b ? (a - b) % in.pitch : (in.pitch - (b - a) % in.pitch) % in.pitch;
+    if (d >= in.width && d + out.width <= in.pitch) return;
+  }
+  throw Failure(std::string("The output overlaps the ") + what + ".");
+}
+
 lb::RouteParams route_params(const llambda_cuda_route_desc* d) {
   if (!d) throw Failure("A routing descriptor is required.");
   if (d->experts < 1 || d->experts > 1024) throw Failure("Expert count must be in 1..1024.");
@@ -1547,6 +1571,10 @@ int llambda_cuda_route_device(const llambda_cuda_route_desc* desc, int logits_ty
       require_on(device_bias, dev, "bias");
       require_align(device_bias, 4, "bias");
     }
+    const Rows in = rows_of(device_logits, logits_type, ld, tokens, r.experts);
+    const size_t eb = (size_t)r.top_k * 4;
+    require_apart({device_selected, eb, eb, tokens}, in, "logits");
+    require_apart({device_weights, eb, eb, tokens}, in, "logits");
     cuda_check(lb::launch_route(r, is_bf16(logits_type, "logits"), device_logits, ld, device_bias,
                                 T, device_selected, device_weights,
                                 static_cast<cudaStream_t>(cuda_stream)),
@@ -1591,6 +1619,10 @@ int llambda_cuda_fp8_quantize_device(int type, const void* device_x, int64_t ldx
     require_on(device_scales, dev, "scales");
     require_align(device_q, 16, "quantised output");
     require_align(device_scales, 16, "scales");
+    const Rows in = rows_of(device_x, type, ldx, tokens, cols);
+    const size_t qp = (cols + 15) / 16 * 16, sp = (tokens + 3) / 4 * 16;
+    require_apart({device_q, qp, qp, tokens}, in, "input");
+    require_apart({device_scales, sp, sp, (cols + 127) / 128}, in, "input");
     cuda_check(lb::launch_f8_quant(is_bf16(type, "input"), device_x, ldx, T, (int)cols,
                                    static_cast<uint8_t*>(device_q), device_scales,
                                    static_cast<cudaStream_t>(cuda_stream)),
@@ -1683,6 +1715,8 @@ int llambda_cuda_fp8_session_run_device(llambda_cuda_fp8_session* s, int x_type,
     DeviceGuard g(s->device);
     require_operand(x_type, device_x, ldx, tokens, s->w.cols, s->device, "input");
     require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
+    require_apart(rows_of(device_out, out_type, ldo, tokens, s->w.rows),
+                  rows_of(device_x, x_type, ldx, tokens, s->w.cols), "input");
     if (const size_t need = llambda_cuda_fp8_session_workspace(s, tokens))
       require_workspace(workspace, workspace_bytes, need, s->device);
     f8_project_call(s, is_bf16(x_type, "input"), device_x, ldx, T, is_bf16(out_type, "output"),
@@ -1706,6 +1740,11 @@ int llambda_cuda_fp8_session_run_quantized(llambda_cuda_fp8_session* s, const vo
     require_align(device_q, 16, "quantised input");
     require_align(device_scales, 16, "scales");
     require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
+    const Rows out = rows_of(device_out, out_type, ldo, tokens, s->w.rows);
+    const size_t kb = (s->w.cols + 127) / 128, qp = ((size_t)s->w.cols + 15) / 16 * 16;
+    require_apart(out, {device_q, qp, qp, tokens}, "quantised input");
+    const size_t sp = (tokens + 3) / 4 * 16;
+    require_apart(out, {device_scales, sp, sp, kb}, "scales");
     cuda_check(lb::launch_f8_project(s->w, static_cast<const uint8_t*>(device_q), device_scales, T,
                                      is_bf16(out_type, "output"), device_out, ldo, false, s->status,
                                      static_cast<cudaStream_t>(cuda_stream)),
@@ -1817,6 +1856,11 @@ int llambda_cuda_fp8_moe_session_run_device(llambda_cuda_fp8_moe_session* s, int
     require_on(device_weights, s->device, "weights");
     require_align(device_selected, 4, "selected");
     require_align(device_weights, 4, "weights");
+    const Rows out = rows_of(device_out, out_type, ldo, tokens, s->m.down.rows);
+    const size_t eb = (size_t)top_k * 4;
+    require_apart(out, rows_of(device_x, x_type, ldx, tokens, s->m.up.cols), "input");
+    require_apart(out, {device_selected, eb, eb, tokens}, "selection");
+    require_apart(out, {device_weights, eb, eb, tokens}, "weights");
     require_workspace(workspace, workspace_bytes,
                       lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes, s->device);
     cuda_check(lb::launch_f8_moe(s->m, is_bf16(x_type, "input"), device_x, ldx, (int)tokens, top_k,

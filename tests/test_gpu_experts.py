@@ -417,6 +417,37 @@ def test_product_refusals():
     assert torch.equal(out[:1], p.run_device(x[:1]))
 
 
+def test_an_output_over_an_input_is_refused():
+    g = gen(31)
+    w, s = matrices(g, 128, 128)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    up, down = matrices(g, 4, 256, 128), matrices(g, 4, 128, 256)
+    m = LB.Fp8MoeSession.from_device(up=up, down=down)
+    for T in (1, 3, 70):
+        buf = randn(g, T + 1, 272)
+        sel = torch.randint(0, 4, (T, 2), generator=g, device="cuda").int()
+        wt = randn(g, T, 2)
+        x = buf[:T, :128]
+        want, keep = p.run_device(x.clone()), x.clone()
+        # the same place, a shared column, a row further on, an unequal stride
+        bad = [x, buf[:T, 127:255], torch.as_strided(buf, (T, 128), (136, 1), 0)]
+        if T > 1:
+            bad.append(buf[1:T + 1, :128])
+        for out in bad:
+            with pytest.raises(LB.LlambdaCudaError, match="overlaps the input"):
+                p.run_device(x, out=out)
+            with pytest.raises(LB.LlambdaCudaError, match="overlaps the input"):
+                m.run_device(x, sel, wt, out=out)
+        assert torch.equal(x, keep)
+        # columns next to each other, on either side
+        assert torch.equal(p.run_device(x, out=buf[:T, 128:256]), want)
+        buf[:T, 144:272] = keep
+        assert torch.equal(p.run_device(buf[:T, 144:272], out=buf[:T, 16:144]), want)
+        big = torch.randn(T * 128, generator=g, device="cuda")
+        with pytest.raises(LB.LlambdaCudaError, match="overlaps the weights"):
+            m.run_device(keep, sel, big[:2 * T].view(T, 2), out=big.view(T, 128))
+
+
 # ------------------------------------------------------------------ routed experts
 
 
