@@ -486,8 +486,9 @@ LLAMBDA_CUDA_API int llambda_cuda_fp8_session_run_quantized(
     llambda_cuda_fp8_session* session, const void* device_q, const float* device_scales,
     size_t tokens, int out_type, void* device_out, int64_t ldo, void* cuda_stream);
 
-/* Status word of the session's device-side checks, cleared by reading (0 = ok;
- * 2 = a wait inside a kernel timed out); -1 on a CUDA error. */
+/* Waits for the device, then the status word of the session's device-side
+ * checks, cleared by reading (0 = ok; 2 = a wait inside a kernel timed out); -1
+ * on a CUDA error. */
 LLAMBDA_CUDA_API int llambda_cuda_fp8_session_status(llambda_cuda_fp8_session* session);
 
 typedef struct llambda_cuda_fp8_moe_session llambda_cuda_fp8_moe_session;

@@ -1492,7 +1492,7 @@ struct F8Owner {
     cuda_check(cudaMemcpy(&bad, status + 1, sizeof(int), cudaMemcpyDeviceToHost), "scale check");
     if (bad) throw Failure(std::to_string(bad) + " block scale(s) are not finite.");
   }
-  // Reads and clears the status word; the stream's work is waited for.
+  // Reads and clears the status word; the caller has waited for the calls.
   int take_status() {
     int v = 0;
     cuda_check(cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost), "status copy");
@@ -1760,6 +1760,7 @@ int llambda_cuda_fp8_session_status(llambda_cuda_fp8_session* s) {
   }
   return guarded([&] {
     DeviceGuard g(s->device);
+    cuda_check(cudaDeviceSynchronize(), "device work");  // calls on any stream
     return s->take_status();
   });
 }
@@ -1879,6 +1880,7 @@ int llambda_cuda_fp8_moe_session_status(llambda_cuda_fp8_moe_session* s) {
   }
   return guarded([&] {
     DeviceGuard g(s->device);
+    cuda_check(cudaDeviceSynchronize(), "device work");  // calls on any stream
     return s->take_status();
   });
 }

@@ -257,8 +257,8 @@ class _Fp8Session:
     _destroy = _status = ""
 
     def status(self) -> int:
-        """The device-side status word, cleared by reading: 0, or 2 after a wait
-        inside a kernel timed out."""
+        """Waits for the device; its status word, cleared by reading: 0, or 2
+        after a wait inside a kernel timed out."""
         rc = getattr(N.lib(), self._status)(self._h)
         if rc < 0:
             raise N.LlambdaCudaError(N.last_error())

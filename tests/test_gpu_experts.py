@@ -729,3 +729,16 @@ def test_two_streams_share_the_sessions():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+def test_the_status_waits_for_every_stream():
+    g = gen(34)
+    w, s = matrices(g, 4096, 4096)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    x = randn(g, 2048, 4096)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    for _ in range(50):
+        out = p.run_device(x, stream=st)
+    assert p.status() == 0 and st.query()
+    assert torch.equal(out, p.run_device(x))
