@@ -90,12 +90,19 @@ __device__ __forceinline__ float choice_error(const RouteParams& r, float c, flo
   return (r.softmax ? 8e-6f * smax : 1e-6f) + 2.5e-7f * fabsf(c);
 }
 
+__device__ __forceinline__ float logit_at(const float* p, long i) { return __ldg(p + i); }
+__device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
+  return __bfloat162float(p[i]);
+}
+
 // The choice of one token by one warp: lane L holds experts L * R .. L * R +
 // R - 1, so equal keys go to the lowest lane that has one, and to its lowest j.
-// Rank i's expert goes to lane i (and that of rank top_k, if there is such a
-// lane, to lane top_k).  F = float: returns false when the comparison of the
-// groups was too close, and sets tied on lane i when that of ranks i and i + 1
-// was (by_logit: the compared values are exact).
+// Rank i's expert goes to lane i.  F = float: returns false when the comparison
+// of the groups was too close, or that of the last rank with an expert that is
+// not chosen, and sets tied on lane i when that of ranks i and i + 1 was
+// (by_logit: the compared values are exact).  Equal logits and biases are a true
+// tie, which the index decides: experts of the last rank's are not compared with
+// it (`row`: the token's logits), but whoever comes after them is.
 //
 // Each round takes the warp's largest key, one reduction over the lanes' own
 // largest.  A lane knows its two largest; the keys themselves are in shared
@@ -104,9 +111,9 @@ __device__ __forceinline__ float choice_error(const RouteParams& r, float c, flo
 // At 8191 tokens, 256 experts in 8 groups, top 8: 27 us with the keys in
 // registers and each lane looking through its own in every round, 20 looking
 // only when both are gone, 18 so.
-template <int R, typename F>
-__device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R], const float* bias,
-                                       bool by_logit, float m, F z, int lane, void* shared,
+template <int R, typename F, typename T>
+__device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const float (&l)[R],
+                                       const float* bias, bool by_logit, float m, F z, int lane, void* shared,
                                        int& sel, bool& tied) {
   using K = decltype(order_key(F(0)));
   K* keys = static_cast<K*>(shared);
@@ -179,7 +186,7 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R]
       if (--left == 0) ++g, left = size;
     }
   }
-  K a = 0, b = 0, mine = 0, next = 0;  // mine: rank `lane`'s key; next: that of rank top_k
+  K a = 0, b = 0, mine = 0, next = 0;  // mine: rank `lane`'s key; next: the best not chosen
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     b = max(b, min(a, key[j]));
@@ -198,7 +205,6 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R]
     const int e = owner * R + at;
     if (i == r.top_k) {
       next = best;
-      if (lane == r.top_k) sel = e;  // compared with rank top_k - 1 below
       break;
     }
     if (lane == i) sel = e, mine = best;
@@ -217,17 +223,26 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const float (&l)[R]
     __syncwarp();
   }
   if (check) {
-    K after = __shfl_down_sync(kFull, mine, 1);
-    if (lane == r.top_k - 1) after = next;
-    const F c = key_value(mine), d = key_value(after);
-    tied = lane < r.top_k && after != 0 && c - d <= (F)choice_error(r, (float)c, smax);
+    const K after = __shfl_down_sync(kFull, mine, 1);
+    const F c = key_value(mine), lim = (F)choice_error(r, (float)c, smax);
+    tied = lane < r.top_k - 1 && c - key_value(after) <= lim;
+    const F last = __shfl_sync(kFull, c, r.top_k - 1);
+    const F least = __shfl_sync(kFull, lim, r.top_k - 1);
+    if (next != 0 && last - key_value(next) <= least) {
+      const int e0 = __shfl_sync(kFull, sel, r.top_k - 1);
+      const float l0 = logit_at(row, e0), b0 = bias ? __ldg(bias + e0) : 0.0f;
+      bool near = false;
+#pragma unroll 1
+      for (int j = 0; j < R; ++j) {  // the keys of experts that are out or chosen are 0
+        const K v = keys[lane * (R + 1) + j];
+        if (v == 0 || !(last - key_value(v) <= least)) continue;
+        const int e = lane * R + j;
+        near |= logit_at(row, e) != l0 || (bias && __ldg(bias + e) != b0);
+      }
+      if (__any_sync(kFull, near)) sure = false;
+    }
   }
   return sure;
-}
-
-__device__ __forceinline__ float logit_at(const float* p, long i) { return __ldg(p + i); }
-__device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
-  return __bfloat162float(p[i]);
 }
 
 // R consecutive logits, in the widest loads their size allows when the rows are aligned.
@@ -308,12 +323,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
   }
   int sel = 0;
   bool tied = false;
-  bool sure = choose<R, float>(r, l, bias, by_logit, m, z, lane, shared, sel, tied);
+  bool sure = choose<R, float>(r, row, l, bias, by_logit, m, z, lane, shared, sel, tied);
   if (__any_sync(kFull, tied)) {
-    // equal logits and biases are a true tie, which the index has decided
+    // a true tie the index has decided
     const float lv = logit_at(row, sel), bv = bias ? __ldg(bias + sel) : 0.0f;
     const float ln = __shfl_down_sync(kFull, lv, 1), bn = __shfl_down_sync(kFull, bv, 1);
-    sure = sure && !__any_sync(kFull, tied && (lane == 31 || lv != ln || bv != bn));
+    sure = sure && !__any_sync(kFull, tied && (lv != ln || bv != bn));
   }
   if (!sure) {
     double zd = 1.0;
@@ -328,7 +343,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
       for (int o = 16; o > 0; o >>= 1) zd += __shfl_xor_sync(kFull, zd, o);
     }
     __syncwarp();
-    choose<R, double>(r, l, bias, false, m, zd, lane, shared, sel, tied);
+    choose<R, double>(r, row, l, bias, false, m, zd, lane, shared, sel, tied);
   }
   // lane i: the weight of rank i
   float s = 0.0f;
