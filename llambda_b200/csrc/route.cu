@@ -80,7 +80,9 @@ __device__ __forceinline__ double choice(const RouteParams& r, const float* bias
   return bias ? s + (double)__ldg(bias + e) : s;
 }
 
-// Bound on the error of the difference of two fp32 choices.  Sigmoid: __expf
+// Bound on the error of the difference of two fp32 choices near c (half of it:
+// of one choice, and of its part in a sum; z's error is common to all choices
+// and changes no order).  Sigmoid: __expf
 // is off by (2 + 1.173 |l|) steps at most, which moves s by at most 0.63 steps
 // of 2^-23, the sum by half a step, __fdividef by two.  Softmax, relative to
 // the largest score smax = 1 / z: the exponentials and the division 5e-7 each,
@@ -113,8 +115,8 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
 // only when both are gone, 18 so.
 template <int R, typename F, typename T>
 __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const float (&l)[R],
-                                       const float* bias, bool by_logit, float m, F z, int lane, void* shared,
-                                       int& sel, bool& tied) {
+                                       const float* bias, bool by_logit, float m, F z, int lane,
+                                       void* shared, int& sel, bool& tied) {
   using K = decltype(order_key(F(0)));
   K* keys = static_cast<K*>(shared);
   const bool check = sizeof(F) == 4 && !by_logit;
@@ -172,12 +174,19 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const
     const bool is_group = lane < r.groups;
     const unsigned kept = __ballot_sync(kFull, is_group && rank < r.top_groups);
     if (check) {
-      // the best group left out against the worst one kept, sums of two (a NaN compares false)
-      const int wi = __ffs(__ballot_sync(kFull, is_group && rank == r.top_groups - 1)) - 1;
-      const int bo = __ffs(__ballot_sync(kFull, is_group && rank == r.top_groups)) - 1;
-      const F in = key_value((K)__shfl_sync(kFull, gkey, wi));
-      const F out = key_value((K)__shfl_sync(kFull, gkey, bo));
-      if (in - out <= F(2) * (F)choice_error(r, (float)in, smax)) sure = false;
+      // Every group left out against every one kept.  A sum is off by what its
+      // addends are, however small it is itself.  One with NaN, or with an expert
+      // that is masked, is exact.
+      const bool two = r.group_top == 2, keep = kept >> lane & 1u;
+      const F sum = key_value(gkey), v1 = key_value(g1), v2 = two ? key_value(g2) : F(0);
+      const bool exact = isnan(sum) || (isinf(sum) && sum < 0 && (isinf(v1) || isinf(v2)));
+      const F lim = isinf(sum) ? F(0)
+                               : F(0.5) * ((F)choice_error(r, (float)v1, smax) +
+                                           (two ? (F)choice_error(r, (float)v2, smax) : F(0))) +
+                                     F(1.2e-7) * fabs(sum);
+      const K most = warp_max(is_group && !keep && !exact ? order_key(sum + lim) : K(0));
+      const K least = warp_max(is_group && keep ? order_key(lim - sum) : K(0));
+      if (most != 0 && key_value(most) >= -key_value(least)) sure = false;
     }
     int g = lane * R / size, left = (g + 1) * size - lane * R;  // experts left in group g
 #pragma unroll

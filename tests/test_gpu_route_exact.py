@@ -90,3 +90,24 @@ def test_ties_beside_scores_closer_than_fp32_tells_apart(score, E, k, groups, to
         for dtype in (torch.float32, torch.bfloat16):
             check_choice(logits.to(dtype), k, score, bias, groups=groups, top_groups=top_groups,
                          group_top=group_top)
+
+
+@pytest.mark.parametrize("score,E,groups,top_groups,big,small", [
+    ("sigmoid", 4, 2, 1, 100.0, 2e-5), ("sigmoid", 24, 8, 3, 100.0, 2e-5),
+    ("sigmoid", 64, 32, 9, 1000.0, 2e-4), ("softmax", 256, 16, 5, 8.0, 1e-3),
+    ("softmax", 16, 8, 2, 50.0, 2e-5)])
+def test_sums_of_two_that_cancel(score, E, groups, top_groups, big, small):
+    """Biases of opposite sign in every group: a sum is small and its rounding is not."""
+    g = gen(E + groups)
+    T = 600 if E < 100 else 60
+    logits = small * randn(g, T, E)
+    size = E // groups
+    bias = torch.full((E,), -big, device="cuda")
+    bias[::size] = big
+    kw = dict(groups=groups, top_groups=top_groups, group_top=2)
+    check_choice(logits, 1, score, bias, **kw)
+    # groups whose sums are as large and whose addends are not
+    bias[:size] = 0.0
+    bias[0] = 1.0 / E if score == "softmax" else 0.0
+    check_choice(logits, 1, score, bias, **kw)
+    check_choice(logits, min(size * top_groups, 4), score, None, **kw)
