@@ -419,9 +419,12 @@ typedef struct {
  * score s of every expert, the choice c = s + bias (bias [experts] F32 or
  * NULL), and the top_k experts of largest c within the kept groups, in
  * decreasing order, equal ones by index; selected [tokens][top_k], weights
- * [tokens][top_k] = s of the chosen (renormalised, scaled).  The order is that
- * of exact scores.  An expert with a logit of -inf has score 0 and is chosen
- * last, one with NaN after it; weights whose sum is 0 stay 0. */
+ * [tokens][top_k] = s of the chosen (renormalised, scaled).  Choices and sums of
+ * two are compared in 64 bits; where that does not tell them apart (scores next
+ * to 1, a bias that swallows them) the larger logit comes first, so experts of
+ * one bias are always in the order of their logits.  An expert with a logit of
+ * -inf has score 0 and is chosen last, one with NaN after it; weights whose sum
+ * is 0 stay 0. */
 LLAMBDA_CUDA_API int llambda_cuda_route_device(const llambda_cuda_route_desc* desc,
                                                int logits_type, const void* device_logits,
                                                int64_t ld, const float* device_bias, size_t tokens,

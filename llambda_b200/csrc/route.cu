@@ -12,7 +12,12 @@
 // the choice (no bias, and no sums of two scores) the logits themselves are
 // compared.  Elsewhere c is computed in fp32 first, and a token for which some
 // comparison that decided was closer than the error of c is done again in fp64
-// (well under 1 in 10 tokens for logits of unit variance).
+// (well under 1 in 10 tokens for logits of unit variance).  Where that is too
+// close too (scores next to 1, or beside large biases), the part of a choice that
+// its double rounds off is kept beside it, and choices that are still equal go by
+// their logits.  That pass is rare and the slowest: in the place of the fp64 one
+// it took 8191 tokens with 256 experts in 8 groups from 17.4 to 24.9 us; behind
+// it, with the checks that lead to it, 18.1.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -64,8 +69,8 @@ __device__ __forceinline__ float score(const RouteParams& r, float l, float m, f
   return r.softmax ? expf(l - m) / z : 1.0f / (1.0f + expf(-l));
 }
 
-// What the choice goes by, in fp32 (fast exp and division, errors within
-// choice_error) and in fp64.
+// What the choice goes by, in fp32 (fast exp and division) and in fp64, errors
+// within choice_error.
 __device__ __forceinline__ float choice(const RouteParams& r, const float* bias, float l, float m,
                                         float z, int e) {
   if (l == -INFINITY) return l;
@@ -80,16 +85,19 @@ __device__ __forceinline__ double choice(const RouteParams& r, const float* bias
   return bias ? s + (double)__ldg(bias + e) : s;
 }
 
-// Bound on the error of the difference of two fp32 choices near c (half of it:
-// of one choice, and of its part in a sum; z's error is common to all choices
-// and changes no order).  Sigmoid: __expf
-// is off by (2 + 1.173 |l|) steps at most, which moves s by at most 0.63 steps
-// of 2^-23, the sum by half a step, __fdividef by two.  Softmax, relative to
-// the largest score smax = 1 / z: the exponentials and the division 5e-7 each,
-// z (its exponentials and 37 additions) 4e-6.  Then the rounding of the sums
-// with the bias.
+// Bound on the error of the difference of two choices near c (half of it: of one
+// choice, and of its part in a sum; z's error is common to all choices and changes
+// no order).  fp32, sigmoid: __expf is off by (2 + 1.173 |l|) steps at most, which
+// moves s by at most 0.63 steps of 2^-23, the sum by half a step, __fdividef by
+// two.  Softmax, relative to the largest score smax = 1 / z: the exponentials and
+// the division 5e-7 each, z (its exponentials and 37 additions) 4e-6.  Then the
+// rounding of the sums with the bias.
 __device__ __forceinline__ float choice_error(const RouteParams& r, float c, float smax) {
   return (r.softmax ? 8e-6f * smax : 1e-6f) + 2.5e-7f * fabsf(c);
+}
+// fp64: exp is off by a step, the sum and the division by half a step each.
+__device__ __forceinline__ double choice_error(const RouteParams& r, double c, double smax) {
+  return 2e-15 * smax + 5e-16 * fabs(c);
 }
 
 __device__ __forceinline__ float logit_at(const float* p, long i) { return __ldg(p + i); }
@@ -97,14 +105,103 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
   return __bfloat162float(p[i]);
 }
 
+// A choice in 64 bits as keys that compare in this order: the nearest double, the
+// rest of the sum that it rounds, the logit.  All 0: an expert that is out.
+struct Exact {
+  unsigned long long k;
+  uint32_t lo, l;
+};
+__device__ __forceinline__ bool operator>(const Exact& a, const Exact& b) {
+  return a.k != b.k ? a.k > b.k : a.lo != b.lo ? a.lo > b.lo : a.l > b.l;
+}
+__device__ __forceinline__ bool operator==(const Exact& a, const Exact& b) {
+  return a.k == b.k && a.lo == b.lo && a.l == b.l;
+}
+__device__ __forceinline__ void take_two(Exact& a, Exact& b, const Exact& v) {  // the two largest
+  if (v > a)
+    b = a, a = v;
+  else if (v > b)
+    b = v;
+}
+__device__ __forceinline__ Exact shfl(const Exact& v, int lane) {
+  return {__shfl_sync(kFull, v.k, lane), __shfl_sync(kFull, v.lo, lane),
+          __shfl_sync(kFull, v.l, lane)};
+}
+// The warp's largest, and the lowest lane that has it.
+__device__ __forceinline__ Exact warp_max(const Exact& v, int& owner) {
+  Exact r;
+  r.k = warp_max(v.k);
+  bool in = v.k == r.k;
+  r.lo = warp_max(in ? v.lo : 0u);
+  in = in && v.lo == r.lo;
+  r.l = warp_max(in ? v.l : 0u);
+  in = in && v.l == r.l;
+  owner = __ffs(__ballot_sync(kFull, in)) - 1;
+  return r;
+}
+// a + b + c with |c| small beside the sum, or a, b doubles of any size (their sum
+// and its error: Knuth, The Art of Computer Programming 2, 4.2.2), logit key l.
+__device__ __forceinline__ Exact exact_sum(double a, double b, double c, uint32_t l) {
+  const double s = a + b, t = s - a, e = ((a - (s - t)) + (b - t)) + c;
+  const double hi = s + e;
+  if (!isfinite(hi)) return {order_key(s + c), 0u, 0u};
+  return {order_key(hi), order_key((float)(e - (hi - s))), l};
+}
+__device__ __forceinline__ Exact exact_choice(const RouteParams& r, const float* bias, float l,
+                                              float m, double z, int e) {
+  if (l == -INFINITY) return {order_key((double)l), 0u, 0u};
+  const double b = bias ? (double)__ldg(bias + e) : 0.0;
+  if (r.softmax) return exact_sum(b, exp((double)l - (double)m) / z, 0.0, order_key(l));
+  // a positive logit's score as 1 less what is left
+  if (l > 0.0f) return exact_sum(1.0, b, -1.0 / (1.0 + exp((double)l)), order_key(l));
+  return exact_sum(b, 1.0 / (1.0 + exp(-(double)l)), 0.0, order_key(l));
+}
+
+// Whether the groups (one a lane) that are close to each other have a true tie: their
+// two largest choices (g1, g2; `keys`: all, R + 1 a lane) are of equal logits and
+// biases, that is all choices near the first are, and all near the second.  Not
+// inlined, as choose_exact is not: the registers they take would be the whole
+// kernel's (8192 tokens, 1024 experts: 83 -> 90 us).
+template <int R, typename T>
+__device__ __noinline__ bool groups_tie(RouteParams r, const T* row, const float* bias,
+                                        const unsigned long long* keys, unsigned long long g1,
+                                        unsigned long long g2, double smax, bool close) {
+  const int lane = threadIdx.x & 31;
+  const unsigned near = __ballot_sync(kFull, close);
+  const int any = __ffs(near) - 1;
+  if (any < 0) return false;
+  const unsigned long long k1 = __shfl_sync(kFull, g1, any), k2 = __shfl_sync(kFull, g2, any);
+  if (!__all_sync(kFull, !close || (g1 == k1 && g2 == k2))) return false;
+  const double t1 = key_value(k1), t2 = key_value(k2);
+  const double from1 = t1 - choice_error(r, t1, smax), from2 = t2 - choice_error(r, t2, smax);
+  const int size = r.experts / r.groups;
+  uint32_t low[4] = {~0u, ~0u, ~0u, ~0u}, high[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+  for (int j = 0; j < R; ++j) {
+    const int e = lane * R + j;
+    const double v = key_value(keys[lane * (R + 1) + j]);  // (not a number where there is none)
+    if (e >= r.experts || !(near >> (e / size) & 1u) || !(v >= from2)) continue;
+    const bool first = v >= from1;
+    const uint32_t kl = order_key(logit_at(row, e)), kb = bias ? order_key(__ldg(bias + e)) : 0u;
+    low[0] = min(low[0], first ? kl : ~0u), high[0] = max(high[0], first ? kl : 0u);
+    low[1] = min(low[1], first ? kb : ~0u), high[1] = max(high[1], first ? kb : 0u);
+    low[2] = min(low[2], first ? ~0u : kl), high[2] = max(high[2], first ? 0u : kl);
+    low[3] = min(low[3], first ? ~0u : kb), high[3] = max(high[3], first ? 0u : kb);
+  }
+  bool same = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    same = __reduce_min_sync(kFull, low[i]) >= warp_max(high[i]) && same;
+  return same;
+}
+
 // The choice of one token by one warp: lane L holds experts L * R .. L * R +
 // R - 1, so equal keys go to the lowest lane that has one, and to its lowest j.
-// Rank i's expert goes to lane i.  F = float: returns false when the comparison
-// of the groups was too close, or that of the last rank with an expert that is
-// not chosen, and sets tied on lane i when that of ranks i and i + 1 was
-// (by_logit: the compared values are exact).  Equal logits and biases are a true
-// tie, which the index decides: experts of the last rank's are not compared with
-// it (`row`: the token's logits), but whoever comes after them is.
+// Rank i's expert goes to lane i.  Returns false when some comparison that
+// decided was closer than the error of the choices (by_logit: there is none):
+// that of two groups, of two ranks, or of the last rank with an expert that is not
+// chosen.  Equal logits and biases (`row`: the token's logits) are a true tie, which
+// the index decides.
 //
 // Each round takes the warp's largest key, one reduction over the lanes' own
 // largest.  A lane knows its two largest; the keys themselves are in shared
@@ -116,11 +213,11 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
 template <int R, typename F, typename T>
 __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const float (&l)[R],
                                        const float* bias, bool by_logit, float m, F z, int lane,
-                                       void* shared, int& sel, bool& tied) {
+                                       void* shared, int& sel) {
   using K = decltype(order_key(F(0)));
   K* keys = static_cast<K*>(shared);
-  const bool check = sizeof(F) == 4 && !by_logit;
-  const float smax = r.softmax ? 1.0f / (float)z : 1.0f;
+  const bool check = !by_logit;
+  const F smax = r.softmax ? F(1) / z : F(1);
   K key[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
@@ -181,12 +278,21 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const
       const F sum = key_value(gkey), v1 = key_value(g1), v2 = two ? key_value(g2) : F(0);
       const bool exact = isnan(sum) || (isinf(sum) && sum < 0 && (isinf(v1) || isinf(v2)));
       const F lim = isinf(sum) ? F(0)
-                               : F(0.5) * ((F)choice_error(r, (float)v1, smax) +
-                                           (two ? (F)choice_error(r, (float)v2, smax) : F(0))) +
-                                     F(1.2e-7) * fabs(sum);
+                               : F(0.5) * (choice_error(r, v1, smax) +
+                                         (two ? choice_error(r, v2, smax) : F(0))) +
+                                     (sizeof(F) == 4 ? F(1.2e-7) : F(2.3e-16)) * fabs(sum);
       const K most = warp_max(is_group && !keep && !exact ? order_key(sum + lim) : K(0));
       const K least = warp_max(is_group && keep ? order_key(lim - sum) : K(0));
-      if (most != 0 && key_value(most) >= -key_value(least)) sure = false;
+      if (most != 0 && key_value(most) >= -key_value(least)) {
+        sure = false;
+        if constexpr (sizeof(F) == 8) {
+#pragma unroll
+          for (int j = 0; j < R; ++j) keys[lane * (R + 1) + j] = key[j];
+          sure = groups_tie<R>(r, row, bias, keys, g1, two ? g2 : g1, smax,
+                               is_group && (keep ? sum - lim <= key_value(most)
+                                                 : !exact && sum + lim >= -key_value(least)));
+        }
+      }
     }
     int g = lane * R / size, left = (g + 1) * size - lane * R;  // experts left in group g
 #pragma unroll
@@ -233,8 +339,13 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const
   }
   if (check) {
     const K after = __shfl_down_sync(kFull, mine, 1);
-    const F c = key_value(mine), lim = (F)choice_error(r, (float)c, smax);
-    tied = lane < r.top_k - 1 && c - key_value(after) <= lim;
+    const F c = key_value(mine), lim = choice_error(r, c, smax);
+    const bool tied = lane < r.top_k - 1 && c - key_value(after) <= lim;
+    if (__any_sync(kFull, tied)) {
+      const float lv = logit_at(row, sel), bv = bias ? __ldg(bias + sel) : 0.0f;
+      const float ln = __shfl_down_sync(kFull, lv, 1), bn = __shfl_down_sync(kFull, bv, 1);
+      if (__any_sync(kFull, tied && (lv != ln || bv != bn))) sure = false;
+    }
     const F last = __shfl_sync(kFull, c, r.top_k - 1);
     const F least = __shfl_sync(kFull, lim, r.top_k - 1);
     if (next != 0 && last - key_value(next) <= least) {
@@ -252,6 +363,91 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const
     }
   }
   return sure;
+}
+
+// The choice by Exact keys, in shared memory (32 R of 8 bytes, then of 4).
+template <int R, typename T>
+__device__ __noinline__ int choose_exact(RouteParams r, const T* row, const float* bias,
+                                         float m, double z, void* shared) {
+  const int lane = threadIdx.x & 31;
+  int sel = 0;
+  unsigned long long* ks = static_cast<unsigned long long*>(shared);
+  uint32_t* los = reinterpret_cast<uint32_t*>(ks + 32 * R);
+  auto at = [&](int owner, int j) {  // expert owner * R + j
+    const int i = j * 32 + owner;
+    Exact v{ks[i], los[i], 0u};
+    if (v.k > 1ull && isfinite(key_value(v.k))) v.l = order_key(logit_at(row, owner * R + j));
+    return v;
+  };
+  constexpr Exact kOut{0ull, 0u, 0u};
+  Exact a = kOut, b = kOut;
+#pragma unroll(R < 4 ? R : 4)
+  for (int j = 0; j < R; ++j) {
+    const int e = lane * R + j;
+    const Exact v =
+        e < r.experts ? exact_choice(r, bias, logit_at(row, e), m, z, e) : kOut;
+    ks[j * 32 + lane] = v.k, los[j * 32 + lane] = v.lo;
+    take_two(a, b, v);
+  }
+  if (r.top_groups < r.groups) {
+    const int size = r.experts / r.groups, span = size / R;
+    Exact g1 = kOut, g2 = kOut;  // lane g: group g's two largest
+    if (size % R == 0 && (span & (span - 1)) == 0) {
+      for (int o = 1; o < span; o <<= 1) {
+        const Exact a2 = shfl(a, lane ^ o), b2 = shfl(b, lane ^ o);
+        take_two(a, b, a2);
+        take_two(a, b, b2);
+      }
+      g1 = shfl(a, lane * span & 31), g2 = shfl(b, lane * span & 31);
+    } else {
+      for (int g = 0; g < r.groups; ++g) {
+        const int lo = max(g * size - lane * R, 0), hi = min((g + 1) * size - lane * R, R);
+        a = b = kOut;
+        for (int j = lo; j < hi; ++j) take_two(a, b, at(lane, j));
+        int owner, other;
+        const Exact first = warp_max(a, owner);
+        const Exact second = warp_max(lane == owner ? b : a, other);
+        if (lane == g) g1 = first, g2 = second;
+      }
+    }
+    Exact rank_by = g1;
+    if (r.group_top == 2) {
+      const double d1 = key_value(g1.k), d2 = key_value(g2.k);
+      rank_by = exact_sum(d1, d2, isfinite(d1) && isfinite(d2)
+                                      ? (double)key_value(g1.lo) + (double)key_value(g2.lo)
+                                      : 0.0, 0u);
+    }
+    if (lane >= r.groups) rank_by = kOut;
+    int rank = 0;
+    for (int g = 0; g < r.groups; ++g) {
+      const Exact v = shfl(rank_by, g);
+      rank += v > rank_by || (v == rank_by && g < lane);
+    }
+    const unsigned kept = __ballot_sync(kFull, lane < r.groups && rank < r.top_groups);
+    a = kOut;
+    for (int j = 0; j < R; ++j) {
+      if (lane * R + j >= r.experts) break;
+      if (!(kept >> ((lane * R + j) / size) & 1u)) {
+        ks[j * 32 + lane] = 0ull;
+      } else {
+        const Exact v = at(lane, j);
+        if (v > a) a = v;
+      }
+    }
+  }
+  __syncwarp();
+  for (int i = 0; i < r.top_k; ++i) {
+    int owner, one;
+    const Exact best = warp_max(a, owner);
+    Exact v = lane < R ? at(owner, lane) : kOut;  // lane j: the owner's j-th
+    const int j = __ffs(__ballot_sync(kFull, v == best && lane < R)) - 1;
+    if (lane == i) sel = owner * R + j;
+    if (lane == j) ks[j * 32 + owner] = 0ull, v = kOut;
+    const Exact next = warp_max(v, one);
+    if (lane == owner) a = next;
+    __syncwarp();
+  }
+  return sel;
 }
 
 // R consecutive logits, in the widest loads their size allows when the rows are aligned.
@@ -293,7 +489,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     route_kernel(const RouteParams r, const T* __restrict__ logits, long ld,
                  const float* __restrict__ bias, int tokens, int* __restrict__ selected,
                  float* __restrict__ weights, int vec) {
-  __shared__ unsigned long long s_keys[kRouteWarps][32 * (R + 1)];
+  __shared__ unsigned long long s_keys[kRouteWarps][R == 1 ? 64 : 48 * R];  // 12 bytes an expert
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
@@ -331,14 +527,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     }
   }
   int sel = 0;
-  bool tied = false;
-  bool sure = choose<R, float>(r, row, l, bias, by_logit, m, z, lane, shared, sel, tied);
-  if (__any_sync(kFull, tied)) {
-    // a true tie the index has decided
-    const float lv = logit_at(row, sel), bv = bias ? __ldg(bias + sel) : 0.0f;
-    const float ln = __shfl_down_sync(kFull, lv, 1), bn = __shfl_down_sync(kFull, bv, 1);
-    sure = sure && !__any_sync(kFull, tied && (lv != ln || bv != bn));
-  }
+  const bool sure = choose<R, float>(r, row, l, bias, by_logit, m, z, lane, shared, sel);
   if (!sure) {
     double zd = 1.0;
     if (r.softmax) {
@@ -352,7 +541,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
       for (int o = 16; o > 0; o >>= 1) zd += __shfl_xor_sync(kFull, zd, o);
     }
     __syncwarp();
-    choose<R, double>(r, row, l, bias, false, m, zd, lane, shared, sel, tied);
+    if (!choose<R, double>(r, row, l, bias, false, m, zd, lane, shared, sel)) {
+      __syncwarp();
+      sel = choose_exact<R>(r, row, bias, m, zd, shared);
+    }
   }
   // lane i: the weight of rank i
   float s = 0.0f;

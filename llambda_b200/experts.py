@@ -166,7 +166,8 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
     score + bias (float32 [experts]), within the `top_groups` best of `groups`
     equal groups, a group's rank being its largest choice (group_top 1) or the
     sum of its two largest (2).  Experts come in decreasing order, equal ones by
-    index; the order is that of exact scores.  Weights are the scores without
+    index; choices are compared in 64 bits, and by their logits where that does
+    not tell them apart.  Weights are the scores without
     bias, divided by their sum with `renormalise`, times `weight_scale`.  An
     expert with a logit of -inf has score 0 and is chosen last."""
     if not hasattr(logits, "data_ptr"):

@@ -1,6 +1,7 @@
 """The choice of experts where fp32, or 64 bits, cannot tell scores apart: against the
-definition in 60 decimal digits."""
+definition with scores of 60 decimal digits and exact sums."""
 import decimal
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -25,10 +26,11 @@ def randn(g, *shape):
 
 def route_reference(logits, k, score, bias=None, groups=1, top_groups=1, group_top=1, renorm=True,
                     scale=1.0):
-    """(selected, weights as Python floats), logits and biases finite."""
+    """(selected, weights as Python floats, gap between the sums of the last group kept and the
+    first one left out), logits and biases finite."""
     l = logits.double().cpu().tolist()
     b = bias.double().cpu().tolist() if bias is not None else [0.0] * logits.shape[1]
-    sel, wts = [], []
+    sel, wts, gaps = [], [], []
     with decimal.localcontext(CTX):
         for row in l:
             if score == "softmax":
@@ -36,24 +38,31 @@ def route_reference(logits, k, score, bias=None, groups=1, top_groups=1, group_t
                 s = [v / sum(p) for v in p]
             else:
                 s = [1 / (1 + (-D(v)).exp()) for v in row]
-            c = [v + D(w) for v, w in zip(s, b)]
+            # (sums rounded to 60 digits would break ties of other pairs with the same sum)
+            c = [Fraction(v) + Fraction(w) for v, w in zip(s, b)]
             size = len(row) // groups
             ranks = [sum(sorted(c[g * size:(g + 1) * size], reverse=True)[:group_top])
                      for g in range(groups)]
-            kept = sorted(range(groups), key=lambda g: (-ranks[g], g))[:top_groups]
+            order = sorted(range(groups), key=lambda g: (-ranks[g], g))
+            kept = order[:top_groups]
+            gaps.append(float(ranks[kept[-1]] - ranks[order[top_groups]])
+                        if group_top == 2 and top_groups < groups else 0.0)
             cand = [e for g in kept for e in range(g * size, (g + 1) * size)]
             chosen = sorted(cand, key=lambda e: (-c[e], e))[:k]
             total = sum(s[e] for e in chosen) if renorm else 1
             sel.append(chosen)
             wts.append([float(s[e] / total * D(scale)) for e in chosen])
-    return np.array(sel), np.array(wts)
+    return np.array(sel), np.array(wts), np.array(gaps)
 
 
-def check_choice(logits, k, score, bias=None, **kw):
+def check_choice(logits, k, score, bias=None, least=0.0, **kw):
+    """least: sums of two that are nearer to each other, and not equal, are not compared."""
     sel, _ = LB.route_experts(logits, k, score=score, bias=bias, **kw)
-    want, _ = route_reference(logits, k, score, bias, **kw)
+    want, _, gaps = route_reference(logits, k, score, bias, **kw)
     got = sel.cpu().numpy()
-    bad = np.nonzero((got != want).any(1))[0]
+    told = (gaps == 0) | (gaps >= least)
+    assert told.mean() >= 0.5
+    bad = np.nonzero(told & (got != want).any(1))[0]
     assert bad.size == 0, (bad.size, bad[:4], got[bad[:4]], want[bad[:4]])
 
 
@@ -111,3 +120,79 @@ def test_sums_of_two_that_cancel(score, E, groups, top_groups, big, small):
     bias[0] = 1.0 / E if score == "softmax" else 0.0
     check_choice(logits, 1, score, bias, **kw)
     check_choice(logits, min(size * top_groups, 4), score, None, **kw)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k,groups,top_groups", [(2, 1, 1, 1), (16, 4, 1, 1), (64, 8, 8, 3),
+                                                   (60, 5, 5, 2), (1024, 32, 1, 1)])
+@pytest.mark.parametrize("lo,hi", [(30.0, 60.0), (-60.0, -30.0), (-1e-8, 1e-8), (37.0, 38.0)])
+def test_equal_biases_choose_as_none_does(score, E, k, groups, top_groups, lo, hi):
+    """Logits whose scores 64 bits do not tell apart: the logits' order decides."""
+    g = gen(E + k)
+    logits = torch.rand(20, E, generator=g, device="cuda") * (hi - lo) + lo
+    logits[:, ::5] = logits[:, 1:2]  # and true ties
+    kw = dict(score=score, groups=groups, top_groups=top_groups)
+    for dtype in (torch.float32, torch.bfloat16):
+        l = logits.to(dtype)
+        want, w = LB.route_experts(l, k, **kw)
+        for b in (0.0, 0.3, -1.0, 1e6, -1e30):
+            sel, _ = LB.route_experts(l, k, bias=torch.full((E,), b, device="cuda"), **kw)
+            assert torch.equal(sel, want), b
+        if groups == 1:  # without groups the order is the logits' by definition
+            order = torch.sort(l.float(), dim=1, descending=True, stable=True).indices[:, :k]
+            assert torch.equal(want.long(), order)
+
+
+@pytest.mark.parametrize("E,k,groups,top_groups", [(8, 3, 1, 1), (32, 6, 4, 2), (96, 10, 1, 1),
+                                                   (24, 2, 3, 1)])
+def test_scores_near_one_with_small_biases(E, k, groups, top_groups):
+    g = gen(E * k)
+    logits = 38 + 22 * torch.rand(30, E, generator=g, device="cuda")
+    bias = 1e-20 * randn(g, E)
+    for top in (1, 2):
+        kw = dict(groups=groups, top_groups=top_groups, group_top=top)
+        check_choice(logits, k, "sigmoid", bias, **kw)
+        check_choice(logits, k, "sigmoid", bias - 1.0, **kw)
+        check_choice(logits, k, "sigmoid", torch.zeros_like(bias), **kw)
+    # scores on both sides of one half, and a few far from it
+    mixed = torch.where(torch.rand(30, E, generator=g, device="cuda") < 0.5, logits, -logits)
+    check_choice(mixed, k, "sigmoid", torch.zeros_like(bias), groups=groups, top_groups=top_groups)
+
+
+def test_masked_experts_and_unusual_biases_keep_their_order():
+    """-inf logits after all others, NaN last, whatever sends a token to the 64-bit choice."""
+    inf, nan = float("inf"), float("nan")
+    logits = torch.tensor([[40.0, 50.0, -inf, nan, 41.0, -inf, 50.0, 30.0]], device="cuda")
+    zero = torch.zeros(8, device="cuda")
+    sel, _ = LB.route_experts(logits, 8, score="sigmoid", bias=zero)
+    assert sel.tolist() == [[1, 6, 4, 0, 7, 2, 5, 3]]
+    bias = zero.clone()
+    bias[7], bias[0] = inf, -inf
+    sel, _ = LB.route_experts(logits, 8, score="sigmoid", bias=bias)
+    assert sel.tolist() == [[7, 1, 6, 4, 0, 2, 5, 3]]
+    # groups of two: one with a masked expert and one with NaN come last
+    sel, _ = LB.route_experts(logits, 4, score="sigmoid", bias=zero, groups=4, top_groups=2,
+                              group_top=2)
+    assert sel.tolist() == [[1, 6, 0, 7]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,top_groups", [(64, 8, 3), (24, 8, 2), (256, 8, 4), (96, 32, 7)])
+@pytest.mark.parametrize("levels", [[1.0, 1.5, 2.0, 2.5], [17.0, 17.5, 38.0, 40.0, 50.0],
+                                    [0.0, 1e-9, 2e-9, 1.0]])
+def test_groups_whose_sums_tie(score, E, groups, top_groups, levels):
+    """Groups with the same two largest logits, and some that only look so."""
+    g = gen(E + len(levels))
+    lv = torch.tensor(levels, device="cuda")
+    T = 40 if E < 200 else 12
+    logits = lv[torch.randint(0, len(levels), (T, E), generator=g, device="cuda")]
+    two = 0.25 * torch.randint(0, 2, (E,), generator=g, device="cuda")
+    # Four scores of 64 bits, each within 2^-52 (exp a step, two operations half a step each, of a
+    # value of at most 1), do not tell sums apart that differ by less than 2^-50 and are not
+    # equal.  Logits 0 and 2e-9 against twice 1e-9 (fp32's 2e-9 is twice its 1e-9) give such:
+    # 1 / (1 + exp(-l)) = 1/2 + l / 4 - l^3 / 48 + ..., sums 6e-27 / 48 = 1.25e-28 apart.
+    least = 2.0 ** -50 if levels[0] == 0.0 else 0.0
+    for bias in (None, torch.zeros(E, device="cuda"), two):
+        for top in (1, 2):
+            check_choice(logits, min(4, top_groups * (E // groups)), score, bias, least,
+                         groups=groups, top_groups=top_groups, group_top=top)
