@@ -423,8 +423,8 @@ typedef struct {
  * two are compared in 64 bits; where that does not tell them apart (scores next
  * to 1, a bias that swallows them) the larger logit comes first, so experts of
  * one bias are always in the order of their logits.  An expert with a logit of
- * -inf has score 0 and is chosen last, one with NaN after it; weights whose sum
- * is 0 stay 0. */
+ * -inf has score 0 and is chosen last, one with NaN after it; a token all of
+ * whose chosen experts have logits of -inf has weights of 0. */
 LLAMBDA_CUDA_API int llambda_cuda_route_device(const llambda_cuda_route_desc* desc,
                                                int logits_type, const void* device_logits,
                                                int64_t ld, const float* device_bias, size_t tokens,

@@ -450,6 +450,31 @@ __device__ __noinline__ int choose_exact(RouteParams r, const T* row, const floa
   return sel;
 }
 
+// Lane i: the weight of rank i, whose logit is l, in fp64 and relative to the
+// largest chosen score: for tokens some of whose chosen scores are next to what
+// fp32 can hold, or below it, although their shares are not.
+__device__ __noinline__ float faint_weight(RouteParams r, float l, float m, float z) {
+  const bool on = (threadIdx.x & 31) < r.top_k;
+  const double top = key_value(warp_max(on ? order_key(l) : 0u));
+  double s = 0.0;
+  if (on && l != -INFINITY) {
+    const double x = (double)l;
+    if (r.softmax)
+      s = r.renormalise ? exp(x - top) : exp(x - (double)m) / (double)z;
+    else if (l > 0.0f)
+      s = 1.0 / (1.0 + exp(-x));
+    else
+      s = exp(x - (r.renormalise ? fmin(top, 0.0) : 0.0)) / (1.0 + exp(x));
+  }
+  if (r.renormalise) {
+    double sum = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    s /= sum;
+  }
+  return (float)(s * (double)r.scale);
+}
+
 // R consecutive logits, in the widest loads their size allows when the rows are aligned.
 template <int R>
 __device__ __forceinline__ void load_logits(const float* p, float (&l)[R]) {
@@ -547,16 +572,22 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
     }
   }
   // lane i: the weight of rank i
-  float s = 0.0f;
-  if (lane < r.top_k) s = score(r, logit_at(row, sel), m, z);
+  float s = 0.0f, lv = 0.0f;
+  if (lane < r.top_k) {
+    lv = logit_at(row, sel);
+    s = score(r, lv, m, z);
+  }
   float w = s;
   if (r.renormalise) {
     const float sum = warp_sum(s);
     w = sum == 0.0f ? 0.0f : s / sum;
   }
+  w *= r.scale;
+  if (__any_sync(kFull, lane < r.top_k && s < 0x1p-100f && lv != -INFINITY))
+    w = faint_weight(r, lv, m, z);
   if (lane < r.top_k) {
     selected[t * r.top_k + lane] = sel;
-    weights[t * r.top_k + lane] = w * r.scale;
+    weights[t * r.top_k + lane] = w;
   }
 }
 

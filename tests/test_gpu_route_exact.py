@@ -196,3 +196,47 @@ def test_groups_whose_sums_tie(score, E, groups, top_groups, levels):
         for top in (1, 2):
             check_choice(logits, min(4, top_groups * (E // groups)), score, bias, least,
                          groups=groups, top_groups=top_groups, group_top=top)
+
+
+# the argument of exp is off by 70 * U32 at most (scores below 2^-100 are computed in 64 bits),
+# exp by two steps, the sum of exponentials by 37 adds, then the division, the sum of 32 weights, its
+# division, the scale; a weight below fp32's smallest normal number by half of its smallest step
+FAINT_RTOL, FAINT_ATOL = (70 + 4 + 37 + 1 + 32 + 1 + 1) * U32, 2.0 ** -150
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E,k", [(8, 3), (64, 8), (40, 32)])
+def test_weights_of_scores_below_what_fp32_holds(E, k, dtype, renorm):
+    g = gen(E + k)
+    noise = randn(g, 6, E)
+    far = torch.tensor([-70.0, -95.0, -104.0, -200.0, -3000.0, -88.0], device="cuda")[:, None]
+    logits = (noise + far).to(dtype)
+    mixed = logits.clone()
+    mixed[:, 1] = noise[:, 1].to(dtype)  # one ordinary score beside them
+    # softmax: the bias keeps the choice off the experts that are not far below the largest
+    keep_off = torch.zeros(E, device="cuda")
+    keep_off[0] = -10.0
+    below = logits.clone()
+    below[:, 0] = noise[:, 0].to(dtype)
+    for l, score, bias in ((logits, "sigmoid", None), (mixed, "sigmoid", None),
+                           (logits, "sigmoid", keep_off), (mixed, "softmax", None),
+                           (below, "softmax", keep_off)):
+        sel, w = LB.route_experts(l, k, score=score, bias=bias, renormalise=renorm,
+                                  weight_scale=2.5)
+        rs, rw, _ = route_reference(l, k, score, bias, renorm=renorm, scale=2.5)
+        assert np.array_equal(sel.cpu().numpy(), rs)
+        np.testing.assert_allclose(w.double().cpu().numpy(), rw, rtol=FAINT_RTOL, atol=FAINT_ATOL)
+
+
+def test_weights_of_the_farthest_logits():
+    for v in (-3e38, -1e30, -800.0):
+        logits = torch.full((3, 16), v, device="cuda")
+        logits[1, 5], logits[2] = -float("inf"), -float("inf")
+        logits[2, 3] = v
+        _, w = LB.route_experts(logits, 4, score="sigmoid")
+        assert w[:2].tolist() == [[0.25] * 4] * 2 and w[2].tolist() == [1.0, 0.0, 0.0, 0.0]
+        bias = torch.zeros(16, device="cuda")
+        bias[15], logits[:2, 15] = -5.0, 0.0
+        sel, w = LB.route_experts(logits, 4, score="softmax", bias=bias)
+        assert w[0].tolist() == [0.25] * 4 and 15 not in sel[0].tolist()
