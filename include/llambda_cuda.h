@@ -395,9 +395,11 @@ LLAMBDA_CUDA_API int llambda_cuda_moe_forward_static_scratch(const llambda_cuda_
  * session's device), enqueue on `cuda_stream` and return without waiting.
  * They allocate nothing, use no memory but what they are given, and may be
  * captured into a CUDA graph; two calls may overlap when their outputs and
- * workspaces are apart.  An output that shares a byte with an input is refused
- * (column ranges of one buffer with one row stride share none).  Element types are tags: LLAMBDA_CUDA_TYPE_F32 or
- * LLAMBDA_CUDA_TYPE_BF16.  Row strides are in elements. */
+ * workspaces are apart.  An output or workspace that shares a byte with an input,
+ * with a session's weights or scales, or with another output or the workspace is
+ * refused (column ranges of one buffer with one row stride share none).  Element
+ * types are tags: LLAMBDA_CUDA_TYPE_F32 or LLAMBDA_CUDA_TYPE_BF16.  Row strides
+ * are in elements. */
 #define LLAMBDA_CUDA_TYPE_BF16 30
 
 #define LLAMBDA_CUDA_SCORE_SOFTMAX 0

@@ -1381,9 +1381,11 @@ Rows rows_of(const void* p, int type, int64_t ld, size_t tokens, size_t cols) {
   return {p, tokens > 1 ? (size_t)ld * size : cols * size, cols * size, tokens};
 }
 
-// An output must not share a byte with an input: some kernels still read the
-// one when others write the other.  (Column ranges of one buffer share none.)
-void require_apart(const Rows& out, const Rows& in, const char* what) {
+// What a call writes must not share a byte with what it reads, or writes
+// elsewhere: some CTAs or kernels still read the one when others write the other.
+// (Column ranges of one buffer share none.)
+void require_apart(const Rows& out, const Rows& in, const char* what,
+                   const char* who = "output") {
   const uintptr_t a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
   if (a + (out.count - 1) * out.pitch + out.width <= b ||
       b + (in.count - 1) * in.pitch + in.width <= a)
@@ -1392,7 +1394,15 @@ void require_apart(const Rows& out, const Rows& in, const char* what) {
     const size_t d = a >= b ? (a - b) % in.pitch : (in.pitch - (b - a) % in.pitch) % in.pitch;
     if (d >= in.width && d + out.width <= in.pitch) return;
   }
-  throw Failure(std::string("The output overlaps the ") + what + ".");
+  throw Failure(std::string("The ") + who + " overlaps the " + what + ".");
+}
+
+void require_apart(const Rows& out, const lb::F8Matrix& w, const char* who = "output") {
+  if (!w.data) return;
+  const size_t data = (size_t)w.experts * w.rows * w.pitch;
+  const size_t scales = (size_t)w.experts * ((w.rows + 127) / 128) * ((w.cols + 127) / 128) * 4;
+  require_apart(out, {w.data, data, data, 1}, "session's weights", who);
+  require_apart(out, {w.scales, scales, scales, 1}, "session's scales", who);
 }
 
 lb::RouteParams route_params(const llambda_cuda_route_desc* d) {
@@ -1575,6 +1585,13 @@ int llambda_cuda_route_device(const llambda_cuda_route_desc* desc, int logits_ty
     const size_t eb = (size_t)r.top_k * 4;
     require_apart({device_selected, eb, eb, tokens}, in, "logits");
     require_apart({device_weights, eb, eb, tokens}, in, "logits");
+    if (device_bias) {
+      const Rows b{device_bias, (size_t)r.experts * 4, (size_t)r.experts * 4, 1};
+      require_apart({device_selected, eb, eb, tokens}, b, "bias");
+      require_apart({device_weights, eb, eb, tokens}, b, "bias");
+    }
+    require_apart({device_selected, eb, eb, tokens}, {device_weights, eb, eb, tokens},
+                  "output of weights");
     cuda_check(lb::launch_route(r, is_bf16(logits_type, "logits"), device_logits, ld, device_bias,
                                 T, device_selected, device_weights,
                                 static_cast<cudaStream_t>(cuda_stream)),
@@ -1623,6 +1640,8 @@ int llambda_cuda_fp8_quantize_device(int type, const void* device_x, int64_t ldx
     const size_t qp = (cols + 15) / 16 * 16, sp = (tokens + 3) / 4 * 16;
     require_apart({device_q, qp, qp, tokens}, in, "input");
     require_apart({device_scales, sp, sp, (cols + 127) / 128}, in, "input");
+    require_apart({device_q, qp, qp, tokens}, {device_scales, sp, sp, (cols + 127) / 128},
+                  "output of scales");
     cuda_check(lb::launch_f8_quant(is_bf16(type, "input"), device_x, ldx, T, (int)cols,
                                    static_cast<uint8_t*>(device_q), device_scales,
                                    static_cast<cudaStream_t>(cuda_stream)),
@@ -1715,10 +1734,17 @@ int llambda_cuda_fp8_session_run_device(llambda_cuda_fp8_session* s, int x_type,
     DeviceGuard g(s->device);
     require_operand(x_type, device_x, ldx, tokens, s->w.cols, s->device, "input");
     require_operand(out_type, device_out, ldo, tokens, s->w.rows, s->device, "output");
-    require_apart(rows_of(device_out, out_type, ldo, tokens, s->w.rows),
-                  rows_of(device_x, x_type, ldx, tokens, s->w.cols), "input");
-    if (const size_t need = llambda_cuda_fp8_session_workspace(s, tokens))
+    const Rows out = rows_of(device_out, out_type, ldo, tokens, s->w.rows);
+    const Rows in = rows_of(device_x, x_type, ldx, tokens, s->w.cols);
+    require_apart(out, in, "input");
+    require_apart(out, s->w);
+    if (const size_t need = llambda_cuda_fp8_session_workspace(s, tokens)) {
       require_workspace(workspace, workspace_bytes, need, s->device);
+      const Rows work{workspace, need, need, 1};
+      require_apart(work, in, "input", "workspace");
+      require_apart(work, out, "output", "workspace");
+      require_apart(work, s->w, "workspace");
+    }
     f8_project_call(s, is_bf16(x_type, "input"), device_x, ldx, T, is_bf16(out_type, "output"),
                     device_out, ldo, workspace, static_cast<cudaStream_t>(cuda_stream));
     return 0;
@@ -1745,6 +1771,7 @@ int llambda_cuda_fp8_session_run_quantized(llambda_cuda_fp8_session* s, const vo
     require_apart(out, {device_q, qp, qp, tokens}, "quantised input");
     const size_t sp = (tokens + 3) / 4 * 16;
     require_apart(out, {device_scales, sp, sp, kb}, "scales");
+    require_apart(out, s->w);
     cuda_check(lb::launch_f8_project(s->w, static_cast<const uint8_t*>(device_q), device_scales, T,
                                      is_bf16(out_type, "output"), device_out, ldo, false, s->status,
                                      static_cast<cudaStream_t>(cuda_stream)),
@@ -1859,11 +1886,21 @@ int llambda_cuda_fp8_moe_session_run_device(llambda_cuda_fp8_moe_session* s, int
     require_align(device_weights, 4, "weights");
     const Rows out = rows_of(device_out, out_type, ldo, tokens, s->m.down.rows);
     const size_t eb = (size_t)top_k * 4;
-    require_apart(out, rows_of(device_x, x_type, ldx, tokens, s->m.up.cols), "input");
-    require_apart(out, {device_selected, eb, eb, tokens}, "selection");
-    require_apart(out, {device_weights, eb, eb, tokens}, "weights");
-    require_workspace(workspace, workspace_bytes,
-                      lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes, s->device);
+    const size_t need = lb::f8_moe_layout(s->m, (long)tokens, top_k).bytes;
+    require_workspace(workspace, workspace_bytes, need, s->device);
+    const Rows in = rows_of(device_x, x_type, ldx, tokens, s->m.up.cols);
+    const Rows work{workspace, need, need, 1};
+    require_apart(work, out, "output", "workspace");
+    for (const bool is_out : {true, false}) {
+      const Rows& to = is_out ? out : work;
+      const char* who = is_out ? "output" : "workspace";
+      require_apart(to, in, "input", who);
+      require_apart(to, {device_selected, eb, eb, tokens}, "selection", who);
+      require_apart(to, {device_weights, eb, eb, tokens}, "weights", who);
+      require_apart(to, s->m.gate, who);
+      require_apart(to, s->m.up, who);
+      require_apart(to, s->m.down, who);
+    }
     cuda_check(lb::launch_f8_moe(s->m, is_bf16(x_type, "input"), device_x, ldx, (int)tokens, top_k,
                                  device_selected, device_weights, is_bf16(out_type, "output"),
                                  device_out, ldo, workspace, s->status,

@@ -11,7 +11,8 @@ ValueError, a failed call a LlambdaCudaError.
 Device calls run on `stream` (default: the current stream of the tensors'
 device); memory they return or need for working is allocated on that stream, so
 they may be captured into a CUDA graph and overlap on different streams.  An `out`
-that overlaps an input is refused (columns of one buffer do not overlap).  Torch
+that overlaps an input or a session's weights is refused (columns of one buffer
+do not overlap).  Torch
 is only plumbing here (allocation and streams).  The inputs are read, never
 differentiated: a tensor that requires grad is refused while autograd records.
 """

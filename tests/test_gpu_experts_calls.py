@@ -1,0 +1,160 @@
+"""Calls of the routing and 8-bit entry points that are refused, and how they deal with
+streams and memory."""
+import ctypes as C
+
+import pytest
+
+import llambda_b200 as LB
+from llambda_b200 import _native as N
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def matrices(g, *shape):
+    w = (randn(g, *shape) * 40).clamp(-448, 448).to(torch.float8_e4m3fn)
+    s = randn(g, *shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128)) * 0.01
+    return w, s
+
+
+def refused(rc, match):
+    assert rc == -1 and match in N.last_error(), (rc, N.last_error())
+
+
+def test_routing_refuses_outputs_that_overlap():
+    g = gen(1)
+    T, E, k = 40, 16, 4
+    logits, bias = randn(g, T, E), randn(g, E)
+    sel = torch.empty(T, k, dtype=torch.int32, device="cuda")
+    wts = torch.empty(T, k, device="cuda")
+    d = N.RouteDesc(E, k, 0, 1, 1, 1, 1, 1.0)
+
+    def call(s, w, b=bias.data_ptr()):
+        return N.lib().llambda_cuda_route_device(C.byref(d), 0, logits.data_ptr(), E, b, T, s, w,
+                                                 None)
+
+    s, w, nb = sel.data_ptr(), wts.data_ptr(), T * k * 4
+    buf = torch.zeros(2 * nb, dtype=torch.uint8, device="cuda")
+    at = buf.data_ptr()
+    refused(call(bias.data_ptr(), w), "overlaps the bias")
+    refused(call(s, bias.data_ptr()), "overlaps the bias")
+    refused(call(s, at, at + nb - 4), "overlaps the bias")
+    refused(call(at, w, at + nb - 4), "overlaps the bias")
+    refused(call(s, s), "overlaps the output of weights")
+    refused(call(at, at + nb - 4), "overlaps the output of weights")
+    refused(call(at + nb - 4, at), "overlaps the output of weights")
+    # next to each other
+    assert call(at, at + nb) == 0 and call(at + nb, at) == 0 and call(s, w) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(buf[:nb].view(torch.float32).view(T, k), wts)
+    assert torch.equal(buf[nb:].view(torch.int32).view(T, k), sel)
+
+
+def test_the_quantiser_refuses_outputs_that_overlap():
+    g = gen(2)
+    T, K = 24, 256
+    x = randn(g, T, K)
+    nq, ns = T * K, 2 * T * 4
+    buf = torch.zeros(nq + ns, dtype=torch.uint8, device="cuda")
+    at = buf.data_ptr()
+
+    def call(q, s):
+        return N.lib().llambda_cuda_fp8_quantize_device(0, x.data_ptr(), K, T, K, q, s, None)
+
+    refused(call(at, at), "overlaps the output of scales")
+    refused(call(at, at + nq - 16), "overlaps the output of scales")
+    refused(call(at + ns - 16, at), "overlaps the output of scales")
+    assert call(at, at + nq) == 0
+    torch.cuda.synchronize()
+    q, s = LB.fp8_quantize(x)
+    assert torch.equal(buf[:nq], q.view(torch.uint8).flatten())
+    assert torch.equal(buf[nq:].view(torch.float32), s.flatten())
+
+
+def test_products_refuse_outputs_and_workspaces_that_overlap():
+    g = gen(3)
+    H = 256
+    whole = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    w = whole[:H * H].view(torch.float8_e4m3fn).view(H, H)
+    src, s = matrices(g, H, H)
+    w.copy_(src)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    for T in (3, 100):  # without and with a workspace
+        x = randn(g, T, H)
+        want = p.run_device(x)
+        q, sc = LB.fp8_quantize(x)
+        n = T * H * 4
+        over_w = whole[:n].view(torch.float32).view(T, H)
+        with pytest.raises(LB.LlambdaCudaError, match="overlaps the session's weights"):
+            p.run_device(x, out=over_w)
+        with pytest.raises(LB.LlambdaCudaError, match="overlaps the session's weights"):
+            p.run_quantized(q, sc, T, out=over_w)
+        assert torch.equal(w.view(torch.uint8), src.view(torch.uint8))
+        # next to the weights
+        out = whole[H * H:H * H + n].view(torch.float32).view(T, H)
+        assert torch.equal(p.run_device(x, out=out), want)
+    # a session whose scales lie in a buffer
+    tail = torch.ones(1 + T * H, device="cuda")
+    p2 = LB.Fp8ProjectionSession.from_device(src[:128, :128].contiguous(), tail[:1].view(1, 1))
+    with pytest.raises(LB.LlambdaCudaError, match="overlaps the session's scales"):
+        p2.run_device(x[:, :128], out=tail[:T * 128].view(T, 128))
+    # workspaces, through the C call
+    L, T = N.lib(), 100
+    need = L.llambda_cuda_fp8_session_workspace(p._h, T)
+    assert need
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    room = torch.zeros(need + T * H * 4 + 256, dtype=torch.uint8, device="cuda")
+    out = torch.empty(T, H, device="cuda")
+
+    def call(px, po, pw):
+        return L.llambda_cuda_fp8_session_run_device(p._h, 0, px, H, T, 0, po, H, pw, need, None)
+
+    last = room.data_ptr() + (need - 1) // 256 * 256
+    refused(call(room.data_ptr(), out.data_ptr(), room.data_ptr()), "workspace overlaps the input")
+    refused(call(last, out.data_ptr(), room.data_ptr()), "workspace overlaps the input")
+    refused(call(x.data_ptr(), last, room.data_ptr()), "workspace overlaps the output")
+    refused(call(x.data_ptr(), out.data_ptr(), whole.data_ptr()), "workspace overlaps the session")
+    assert call(x.data_ptr(), out.data_ptr(), work.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_experts_refuse_outputs_and_workspaces_that_overlap(T):
+    g = gen(4)
+    E, k, H, I = 4, 2, 128, 256
+    up, down, gate = matrices(g, E, I, H), matrices(g, E, H, I), matrices(g, E, I, H)
+    m = LB.Fp8MoeSession.from_device(up=up, down=down, gate=gate)
+    x, wt = randn(g, T, H), randn(g, T, k)
+    sel = torch.randint(0, E, (T, k), generator=g, device="cuda").int()
+    want = m.run_device(x, sel, wt)
+    for name in ("up", "down", "gate"):
+        t = dict(up=up, down=down, gate=gate)[name]
+        out = t[0].view(torch.uint8).flatten()[:T * H * 4].view(torch.float32).view(T, H)
+        with pytest.raises(LB.LlambdaCudaError, match="overlaps the session's weights"):
+            m.run_device(x, sel, wt, out=out)
+    L = N.lib()
+    need = L.llambda_cuda_fp8_moe_session_workspace(m._h, T, k)
+    room = torch.zeros(need + T * H * 4 + 256, dtype=torch.uint8, device="cuda")
+    out = torch.empty(T, H, device="cuda")
+    names = ("input", "selection", "weights", "output")
+    ptrs = [x.data_ptr(), sel.data_ptr(), wt.data_ptr(), out.data_ptr()]
+
+    def call(a, work=room.data_ptr()):
+        return L.llambda_cuda_fp8_moe_session_run_device(m._h, 0, a[0], H, T, k, a[1], a[2], 0, a[3],
+                                                         H, work, need, None)
+
+    for i, name in enumerate(names):
+        for at in (room.data_ptr(), room.data_ptr() + (need - 1) // 256 * 256):
+            refused(call(ptrs[:i] + [at] + ptrs[i + 1:]), "workspace overlaps the " + name)
+    assert call(ptrs) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
