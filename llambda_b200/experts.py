@@ -10,7 +10,11 @@ ValueError, a failed call a LlambdaCudaError.
 
 Device calls run on `stream` (default: the current stream of the tensors'
 device); memory they return or need for working is allocated on that stream, so
-they may be captured into a CUDA graph and overlap on different streams.  An `out`
+they may be captured into a CUDA graph and overlap on different streams.  A call
+does not wait for other streams: whoever passes a `stream` orders it after what
+writes the inputs.  The inputs may be dropped right after the call when `stream`
+is a torch.cuda.Stream; with a raw handle or an ExternalStream they are kept until
+the stream is done with them.  An `out`
 that overlaps an input or a session's weights is refused (columns of one buffer
 do not overlap).  Torch
 is only plumbing here (allocation and streams).  The inputs are read, never
@@ -119,9 +123,11 @@ def _tag(dtype) -> int:
     return N.TYPE_F32 if dtype is _FLOATS[0] else N.TYPE_BF16
 
 
-def _on(stream, device, allocate):
+def _on(stream, device, operands, allocate):
     """(raw handle of the call's stream, allocate()'s result with that stream
-    current, so that what the call allocates belongs to it)."""
+    current, so that what the call allocates belongs to it).  The memory of
+    `operands` is not given out again before a `stream` is done with it; a raw
+    handle's owner may destroy its stream first, so there the caller keeps them."""
     if stream is None:
         return _raw_stream(device.index), allocate()
     torch = _torch()
@@ -129,6 +135,10 @@ def _on(stream, device, allocate):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     if stream.device != device:
         raise ValueError(f"the stream is on {stream.device}, not {device}")
+    if not isinstance(stream, torch.cuda.ExternalStream):
+        for t in operands:
+            if t is not None:
+                t.record_stream(stream)
     with torch.cuda.stream(stream):
         return stream.cuda_stream, allocate()
 
@@ -180,7 +190,7 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
     if bias is not None:
         _device_tensor(bias, "bias", _F32, (E,), dev)
     desc = _route_desc(E, top_k, score, groups, top_groups, group_top, renormalise, weight_scale)
-    raw, (selected, weights) = _on(stream, dev, lambda: (
+    raw, (selected, weights) = _on(stream, dev, (logits, bias), lambda: (
         _t.empty((T, top_k), dtype=_t.int32, device=dev),
         _t.empty((T, top_k), dtype=_t.float32, device=dev)))
     _check((_lib or _library()).llambda_cuda_route_device(desc, _tag(logits.dtype), logits.data_ptr(), ld,
@@ -217,7 +227,7 @@ def fp8_quantize(x, *, stream=None):
     the row's block, q = e4m3(x / scale), everything rounded to nearest."""
     T, cols, ldx = _matrix(x, "x")
     dev = x.device
-    raw, (q, scales) = _on(stream, dev, lambda: (
+    raw, (q, scales) = _on(stream, dev, (x,), lambda: (
         _t.empty((T, _pad(cols, 16)), dtype=_t.float8_e4m3fn, device=dev),
         _t.empty((_blocks(cols), _pad(T, 4)), dtype=_t.float32, device=dev)))
     _check((_lib or _library()).llambda_cuda_fp8_quantize_device(_tag(x.dtype), x.data_ptr(), ldx, T, cols,
@@ -337,7 +347,7 @@ class Fp8ProjectionSession(_Fp8Session):
         T, _, ldx = _matrix(x, "x", self.cols, self.device)
         dev = x.device
         nbytes = (_lib or _library()).llambda_cuda_fp8_session_workspace(h, T)
-        raw, ((out, ldo), work) = _on(stream, dev, lambda: (
+        raw, ((out, ldo), work) = _on(stream, dev, (x, out), lambda: (
             _out(out, T, self.rows, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev) if nbytes else None))
         _check((_lib or _library()).llambda_cuda_fp8_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T,
@@ -353,7 +363,7 @@ class Fp8ProjectionSession(_Fp8Session):
                        self.device, contiguous=True)
         _device_tensor(scales, "scales", (torch.float32,), (_blocks(self.cols), _pad(tokens, 4)),
                        q.device, contiguous=True)
-        raw, (out, ldo) = _on(stream, q.device, lambda: _out(
+        raw, (out, ldo) = _on(stream, q.device, (q, scales, out), lambda: _out(
             out, tokens, self.rows, out_dtype or torch.float32, q.device))
         _check((_lib or _library()).llambda_cuda_fp8_session_run_quantized(h, q.data_ptr(), scales.data_ptr(), tokens,
               _tag(out.dtype), out.data_ptr(), ldo, raw))
@@ -428,7 +438,7 @@ class Fp8MoeSession(_Fp8Session):
         _device_tensor(selected, "selected", _INT, (T, k), dev, contiguous=True)
         _device_tensor(weights, "weights", _F32, (T, k), dev, contiguous=True)
         nbytes = (_lib or _library()).llambda_cuda_fp8_moe_session_workspace(h, T, k)
-        raw, ((out, ldo), work) = _on(stream, dev, lambda: (
+        raw, ((out, ldo), work) = _on(stream, dev, (x, selected, weights, out), lambda: (
             _out(out, T, self.out_features, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev)))
         _check((_lib or _library()).llambda_cuda_fp8_moe_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T, k,

@@ -158,3 +158,42 @@ def test_experts_refuse_outputs_and_workspaces_that_overlap(T):
     assert call(ptrs) == 0
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_inputs_dropped_after_a_call_on_another_stream_keep_their_memory():
+    """The caller's allocator gives an input's memory out again only when the call's stream is
+    done with it."""
+    g = gen(5)
+    E, k, H = 8, 2, 1024
+    up, down = matrices(g, E, 256, H), matrices(g, E, H, 256)
+    m = LB.Fp8MoeSession.from_device(up=up, down=down)
+    p = LB.Fp8ProjectionSession.from_device(*matrices(g, 256, H))
+    T = 300
+    x = randn(g, T, H)
+    q, sc = LB.fp8_quantize(x)
+    sel = torch.randint(0, E, (T, k), generator=g, device="cuda").int()
+    wt, logits, bias = randn(g, T, k), randn(g, T, 600), randn(g, 600)
+    side = torch.cuda.Stream()
+
+    def busy(call, want, *inputs):
+        copies = [t.clone() for t in inputs]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        got = call(*copies)
+        places = {t.data_ptr() for t in copies}
+        del copies
+        again = [torch.empty_like(t) for t in inputs]  # (nothing is written to them)
+        assert not side.query(), "the side stream was done too soon to show anything"
+        assert not places & {t.data_ptr() for t in again}
+        torch.cuda.synchronize()
+        for a, b in zip(got if isinstance(got, tuple) else (got,),
+                        want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+    busy(lambda a: p.run_device(a, stream=side), p.run_device(x), x)
+    busy(lambda a, b: p.run_quantized(a, b, T, stream=side), p.run_quantized(q, sc, T), q, sc)
+    busy(lambda a: LB.fp8_quantize(a, stream=side), (q, sc), x)
+    busy(lambda a, b, c: m.run_device(a, b, c, stream=side), m.run_device(x, sel, wt), x, sel, wt)
+    busy(lambda a, b: LB.route_experts(a, k, bias=b, stream=side),
+         LB.route_experts(logits, k, bias=bias), logits, bias)
