@@ -461,7 +461,8 @@ typedef struct llambda_cuda_fp8_session llambda_cuda_fp8_session;
 
 /* One matrix (ne2 1) as a projection.  on_device 0: host memory, copied; 1:
  * device memory of the current device, borrowed until the session is
- * destroyed (data 16-byte aligned, ne0 a multiple of 16). */
+ * destroyed (data 16-byte aligned, ne0 a multiple of 16); the call waits for the
+ * device before it checks the scales. */
 LLAMBDA_CUDA_API int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor,
                                                      int on_device,
                                                      llambda_cuda_fp8_session** result);

@@ -1441,9 +1441,11 @@ struct F8Owner {
   std::vector<void*> owned;
   std::mutex mu;
   DevBuf din, dout, dwork, dsel, dw;
-  void open() {
+  void open(bool borrows) {
     device = current_device();
     require_b200(device);
+    // whatever stream writes the caller's tensors, the scales are checked when written
+    if (borrows) cuda_check(cudaDeviceSynchronize(), "device work");
     cuda_check(cudaMalloc(&status, 2 * sizeof(int)), "cudaMalloc");
     cuda_check(cudaMemset(status, 0, 2 * sizeof(int)), "memset");
   }
@@ -1662,7 +1664,7 @@ int llambda_cuda_fp8_session_create(const llambda_cuda_fp8_tensor* tensor, int o
     if (tensor->ne2 > 1) throw Failure("A projection has one matrix.");
     auto s = new llambda_cuda_fp8_session();
     try {
-      s->open();
+      s->open(on_device != 0);
       s->w = s->matrix(*tensor, on_device != 0, "projection tensor");
       s->checked();
     } catch (...) {
@@ -1811,7 +1813,7 @@ int llambda_cuda_fp8_moe_session_create(const llambda_cuda_fp8_tensor* gate,
       throw Failure("The down tensor does not fit the up tensor.");
     auto s = new llambda_cuda_fp8_moe_session();
     try {
-      s->open();
+      s->open(on_device != 0);
       if (gated) s->m.gate = s->matrix(*gate, on_device != 0, "gate tensor");
       s->m.up = s->matrix(*up, on_device != 0, "up tensor");
       s->m.down = s->matrix(*down, on_device != 0, "down tensor");

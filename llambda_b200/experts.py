@@ -321,11 +321,10 @@ class Fp8ProjectionSession(_Fp8Session):
     @classmethod
     def from_device(cls, weights, scales):
         """Borrows CUDA tensors (kept alive by the session): weights
-        float8_e4m3fn or uint8, cols a multiple of 16."""
+        float8_e4m3fn or uint8, cols a multiple of 16.  Waits for the device, so
+        whatever stream writes them, the scales are checked when written."""
         w, s = _device_weights((weights, scales), "projection", 2)
         with _torch().cuda.device(w.device):
-            # weights that a side stream is still writing are checked when written
-            _torch().cuda.current_stream().synchronize()
             return cls._create(w, s, w.data_ptr(), s.data_ptr(), 1, w.device, (w, s))
 
     def run(self, x: np.ndarray) -> np.ndarray:
@@ -403,13 +402,12 @@ class Fp8MoeSession(_Fp8Session):
     @classmethod
     def from_device(cls, up, down, gate=None):
         """Borrows CUDA tensors (kept alive by the session), H and I multiples
-        of 16."""
+        of 16, after waiting for the device."""
         up = _device_weights(up, "up", 3)
         dev = up[0].device
         down = _device_weights(down, "down", 3, dev)
         gate = _device_weights(gate, "gate", 3, dev) if gate is not None else None
         with _torch().cuda.device(dev):
-            _torch().cuda.current_stream().synchronize()
             return cls._create(up, down, gate, lambda t: t.data_ptr(), 1, dev)
 
     def run(self, x: np.ndarray, selected: np.ndarray, weights: np.ndarray) -> np.ndarray:

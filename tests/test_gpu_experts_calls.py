@@ -197,3 +197,27 @@ def test_inputs_dropped_after_a_call_on_another_stream_keep_their_memory():
     busy(lambda a, b, c: m.run_device(a, b, c, stream=side), m.run_device(x, sel, wt), x, sel, wt)
     busy(lambda a, b: LB.route_experts(a, k, bias=b, stream=side),
          LB.route_experts(logits, k, bias=bias), logits, bias)
+
+
+def test_a_session_waits_for_scales_that_another_stream_writes():
+    g = gen(6)
+    w, s = matrices(g, 64, 64)
+    up, down = matrices(g, 2, 64, 64), matrices(g, 2, 64, 64)
+    side = torch.cuda.Stream()
+
+    def late(t):
+        """t's values, not finite until the side stream has written them."""
+        to = torch.full_like(t, float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)
+            to.copy_(t)
+        return to
+
+    x = randn(g, 3, 64)
+    want = LB.Fp8ProjectionSession.from_device(w, s).run_device(x)
+    assert torch.equal(LB.Fp8ProjectionSession.from_device(w, late(s)).run_device(x), want)
+    sel, wt = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), randn(g, 3, 1)
+    want = LB.Fp8MoeSession.from_device(up=up, down=down).run_device(x, sel, wt)
+    got = LB.Fp8MoeSession.from_device(up=up, down=(down[0], late(down[1])))
+    assert torch.equal(got.run_device(x, sel, wt), want)
