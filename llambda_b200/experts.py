@@ -18,7 +18,8 @@ the stream is done with them.  An `out`
 that overlaps an input or a session's weights is refused (columns of one buffer
 do not overlap).  Torch
 is only plumbing here (allocation and streams).  The inputs are read, never
-differentiated: a tensor that requires grad is refused while autograd records.
+differentiated: a tensor that requires grad is refused while autograd records,
+and one with a tangent in forward mode.
 """
 from __future__ import annotations
 
@@ -35,14 +36,15 @@ BLOCK = 128  # columns (and weight rows) per scale
 # A one-token call is a few microseconds of GPU time, so what a call does on the
 # host is kept short: torch, its types, the library and the lookup of the current
 # stream are bound once, by the first call that needs them.
-_t = _lib = _raw_stream = None
+_t = _lib = _raw_stream = _forward = None
 _FLOATS = _FP8 = _INT = _F32 = ()
 
 
 def _torch():
-    global _t, _raw_stream, _FLOATS, _FP8, _INT, _F32
+    global _t, _raw_stream, _forward, _FLOATS, _FP8, _INT, _F32
     if _t is None:
         import torch
+        import torch.autograd.forward_ad as _forward
         _FLOATS = (torch.float32, torch.bfloat16)
         _FP8 = (torch.float8_e4m3fn, torch.uint8)
         _INT, _F32 = (torch.int32,), (torch.float32,)
@@ -78,7 +80,7 @@ def _device_tensor(t, name: str, dtypes, shape, device=None, contiguous=False):
     try:  # the usual case in few steps; what fails it is looked at below
         if (t.is_cuda and t.dtype in dtypes and t.shape == shape and t.is_contiguous()
                 and t.numel() and (device is None or t.device == device)
-                and not t.requires_grad):
+                and not t.requires_grad and _forward._current_level < 0):
             return t
     except AttributeError:
         pass
@@ -93,6 +95,8 @@ def _device_tensor(t, name: str, dtypes, shape, device=None, contiguous=False):
                          f"{tuple('any' if s is None else s for s in shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires grad; these operators have no backward pass")
+    if _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent; these operators have no derivative")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not {device}")
     if 0 in got:

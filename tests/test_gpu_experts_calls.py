@@ -221,3 +221,27 @@ def test_a_session_waits_for_scales_that_another_stream_writes():
     want = LB.Fp8MoeSession.from_device(up=up, down=down).run_device(x, sel, wt)
     got = LB.Fp8MoeSession.from_device(up=up, down=(down[0], late(down[1])))
     assert torch.equal(got.run_device(x, sel, wt), want)
+
+
+def test_tangents_of_forward_mode_are_refused():
+    import torch.autograd.forward_ad as fwd
+    g = gen(7)
+    w, s = matrices(g, 64, 64)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    m = LB.Fp8MoeSession.from_device(up=matrices(g, 2, 64, 64), down=matrices(g, 2, 64, 64))
+    x, sel, wt = randn(g, 3, 64), torch.zeros(3, 1, dtype=torch.int32, device="cuda"), randn(g, 3, 1)
+    want = p.run_device(x), m.run_device(x, sel, wt)
+    with fwd.dual_level():
+        d, dw = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(wt, torch.ones_like(wt))
+        for call in (lambda: LB.route_experts(d, 2), lambda: LB.fp8_quantize(d),
+                     lambda: p.run_device(d), lambda: m.run_device(d, sel, wt),
+                     lambda: m.run_device(x, sel, dw),
+                     lambda: LB.route_experts(x, 2, bias=fwd.make_dual(x[0], x[1]))):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        # without one
+        assert torch.equal(p.run_device(x), want[0])
+        assert torch.equal(m.run_device(x, sel, wt), want[1])
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(p.run_device, (x,), (torch.ones_like(x),))
+    assert torch.equal(p.run_device(x), want[0])
