@@ -10,19 +10,8 @@ from llambda_b200 import _native as N
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-
-def gen(seed):
-    return torch.Generator(device="cuda").manual_seed(seed)
-
-
-def randn(g, *shape):
-    return torch.randn(*shape, generator=g, device="cuda")
-
-
-def matrices(g, *shape):
-    w = (randn(g, *shape) * 40).clamp(-448, 448).to(torch.float8_e4m3fn)
-    s = randn(g, *shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128)) * 0.01
-    return w, s
+from test_gpu_experts import (U32, blocks_of, check, e4m3, gen, matrices,  # noqa: E402
+                              product_reference, quantize_reference, randn)
 
 
 def refused(rc, match):
@@ -245,3 +234,64 @@ def test_tangents_of_forward_mode_are_refused():
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(p.run_device, (x,), (torch.ones_like(x),))
     assert torch.equal(p.run_device(x), want[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width,at", [(5000 + 9, 4), (5003, 3), (5008, 8), (5002, 2), (5004, 1),
+                                      (5001, 0), (5000, 0)])
+def test_a_prompt_into_rows_of_any_stride_and_alignment(dtype, width, at):
+    """Pairs of CTAs store rows by bulk copies where they start on 16 bytes, by words or values
+    elsewhere; nothing beside them changes."""
+    g = gen(width + at)
+    T, N, K = 601, 5000, 272
+    w, s = matrices(g, N, K)
+    p = LB.Fp8ProjectionSession.from_device(w, s)
+    x = randn(g, T, K).to(dtype)
+    big = torch.full((T + 3, width), 7.0, dtype=dtype, device="cuda")
+    view = big[2:2 + T, at:at + N]
+    p.run_device(x, out=view)
+    check(view, *product_reference(*quantize_reference(x), w, s))
+    assert torch.equal(view, p.run_device(x))
+    view.fill_(7.0)
+    assert bool((big == 7.0).all())
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 8, 4096, 1536), (1, 16, 2, 7168, 256), (3, 8, 3, 4096, 1536),
+                                       (40, 8, 2, 7168, 2048), (300, 4, 2, 4096, 1536)])
+def test_experts_of_wide_layers(T, E, k, H, I, gated):
+    g = gen(H + I + T)
+    up, down, gate = matrices(g, E, I, H), matrices(g, E, H, I), matrices(g, E, I, H)
+    x, wt = randn(g, T, H), randn(g, T, k)
+    sel = torch.rand(T, E, generator=g, device="cuda").topk(k, dim=1).indices.int()
+    m = LB.Fp8MoeSession.from_device(up=up, down=down, gate=gate if gated else None)
+    out = m.run_device(x, sel, wt)
+    assert torch.equal(m.run_device(x, sel, wt), out) and m.status() == 0
+    q, sx = quantize_reference(x)
+    want = torch.zeros(T, H, dtype=torch.float64, device="cuda")
+    bound = torch.zeros_like(want)
+    for e in range(E):  # an expert's entries together
+        t, j = torch.nonzero(sel == e, as_tuple=True)
+        if not t.numel():
+            continue
+        u, du = product_reference(q[t], sx[t], up[0][e], up[1][e])
+        if gated:
+            v, dv = product_reference(q[t], sx[t], gate[0][e], gate[1][e])
+            a = v * torch.sigmoid(v)  # |silu'| <= 1.1; its own error 8 half steps
+            h, dh = a * u, (1.1 * dv + 8 * U32 * a.abs()) * (u.abs() + du) + a.abs() * du
+        else:
+            h, dh = torch.relu(u) ** 2, 2.0 * torch.relu(u) * du + du * du
+        p, dp = blocks_of(h), blocks_of(dh + 8 * U32 * h.abs())
+        s = (p.abs().amax(2) / 448).clamp(min=2.0 ** -126)
+        ds = dp.amax(2) / 448 / s + 2 * U32
+        v = p / s[:, :, None]
+        dv = dp / s[:, :, None] + v.abs() * (ds[:, :, None] + 2 * U32)
+        # a quotient within its error of a border of e4m3 may go to the other neighbour
+        hq, (lo, _), (hi, _) = e4m3(v)[0], e4m3(v - dv), e4m3(v + dv)
+        slack = torch.maximum((hq - lo).abs(), (hi - hq).abs()) + hq.abs() * ds[:, :, None]
+        y, dy = product_reference(hq, s, down[0][e], down[1][e])
+        mag, _ = product_reference(slack, s, down[0][e].float().abs(), down[1][e].abs())
+        w = wt[t, j][:, None].double()
+        want.index_add_(0, t, w * y)
+        bound.index_add_(0, t, w.abs() * (dy + mag + 4 * U32 * y.abs()))
+    check(out, want, bound * (1 + k * U32))
