@@ -63,24 +63,6 @@
   (session :pointer) (x :pointer) (tokens :size) (out :pointer)
   (selected :pointer) (weights :pointer))
 
-;; Other routers and e4m3 experts (host buffers; structs as in the header).
-(cffi:defcfun ("llambda_cuda_route" %cuda-route) :int
-  (desc :pointer) (logits :pointer) (bias :pointer) (tokens :size)
-  (selected :pointer) (weights :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_session_create" %cuda-fp8-session-create) :int
-  (tensor :pointer) (on-device :int) (result :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_session_destroy" %cuda-fp8-session-destroy) :void
-  (session :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_session_run" %cuda-fp8-session-run) :int
-  (session :pointer) (x :pointer) (tokens :size) (out :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_moe_session_create" %cuda-fp8-moe-session-create) :int
-  (gate :pointer) (up :pointer) (down :pointer) (on-device :int) (result :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_moe_session_destroy" %cuda-fp8-moe-session-destroy) :void
-  (session :pointer))
-(cffi:defcfun ("llambda_cuda_fp8_moe_session_run" %cuda-fp8-moe-session-run) :int
-  (session :pointer) (x :pointer) (tokens :size) (top-k :int)
-  (selected :pointer) (weights :pointer) (out :pointer))
-
 ;;; ------------------------------------------------------------------ errors
 
 (define-condition cuda-backend-error (simple-error) ())
