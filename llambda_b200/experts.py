@@ -5,8 +5,9 @@ than llambda's own two architectures and GGML blocks: `route_experts` turns
 router logits into experts and weights, `fp8_quantize` turns activations into
 e4m3 with a scale per row and 128 columns, `Fp8ProjectionSession` and
 `Fp8MoeSession` multiply them by e4m3 weights with a scale per 128 x 128 block.
-As everywhere in this package there is no CPU fallback: a refused argument is a
-ValueError, a failed call a LlambdaCudaError.
+As everywhere in this package there is no CPU fallback.  An argument whose type,
+shape, strides or device is wrong is a ValueError; what the library refuses
+(overlaps, sizes, routing options) and a call that fails are LlambdaCudaErrors.
 
 Device calls run on `stream` (default: the current stream of the tensors'
 device); memory they return or need for working is allocated on that stream, so
@@ -197,9 +198,10 @@ def route_experts(logits, top_k: int, *, score: str = "softmax", bias=None, grou
     raw, (selected, weights) = _on(stream, dev, (logits, bias), lambda: (
         _t.empty((T, top_k), dtype=_t.int32, device=dev),
         _t.empty((T, top_k), dtype=_t.float32, device=dev)))
-    _check((_lib or _library()).llambda_cuda_route_device(desc, _tag(logits.dtype), logits.data_ptr(), ld,
-          bias.data_ptr() if bias is not None else None, T, selected.data_ptr(),
-          weights.data_ptr(), raw))
+    _check((_lib or _library()).llambda_cuda_route_device(
+        desc, _tag(logits.dtype), logits.data_ptr(), ld,
+        bias.data_ptr() if bias is not None else None, T, selected.data_ptr(),
+        weights.data_ptr(), raw))
     return selected, weights
 
 
@@ -214,9 +216,9 @@ def _route_host(logits, bias, desc):
             raise ValueError(f"bias must have shape ({E},)")
     T = logits.shape[0]
     selected, weights = np.empty((T, k), np.int32), np.empty((T, k), np.float32)
-    _check((_lib or _library()).llambda_cuda_route(desc, logits.ctypes.data,
-          bias.ctypes.data if bias is not None else None, T, selected.ctypes.data,
-          weights.ctypes.data))
+    _check((_lib or _library()).llambda_cuda_route(
+        desc, logits.ctypes.data, bias.ctypes.data if bias is not None else None, T,
+        selected.ctypes.data, weights.ctypes.data))
     return selected, weights
 
 
@@ -234,8 +236,8 @@ def fp8_quantize(x, *, stream=None):
     raw, (q, scales) = _on(stream, dev, (x,), lambda: (
         _t.empty((T, _pad(cols, 16)), dtype=_t.float8_e4m3fn, device=dev),
         _t.empty((_blocks(cols), _pad(T, 4)), dtype=_t.float32, device=dev)))
-    _check((_lib or _library()).llambda_cuda_fp8_quantize_device(_tag(x.dtype), x.data_ptr(), ldx, T, cols,
-          q.data_ptr(), scales.data_ptr(), raw))
+    _check((_lib or _library()).llambda_cuda_fp8_quantize_device(
+        _tag(x.dtype), x.data_ptr(), ldx, T, cols, q.data_ptr(), scales.data_ptr(), raw))
     return q, scales
 
 
@@ -312,7 +314,8 @@ class Fp8ProjectionSession(_Fp8Session):
     def _create(cls, w, s, data, scales, on_device, device, keep):
         h = C.c_void_p()
         t = _fp8_tensor(w.shape, data, scales)
-        _check((_lib or _library()).llambda_cuda_fp8_session_create(C.byref(t), on_device, C.byref(h)))
+        _check((_lib or _library()).llambda_cuda_fp8_session_create(
+            C.byref(t), on_device, C.byref(h)))
         return cls(h, w.shape[0], w.shape[1], device, keep)
 
     @classmethod
@@ -339,8 +342,8 @@ class Fp8ProjectionSession(_Fp8Session):
         if x.ndim != 2 or x.shape[1] != self.cols or not x.size:
             raise ValueError(f"x must be [tokens][{self.cols}]")
         out = np.empty((x.shape[0], self.rows), np.float32)
-        _check((_lib or _library()).llambda_cuda_fp8_session_run(self._handle(), x.ctypes.data, x.shape[0],
-                                                      out.ctypes.data))
+        _check((_lib or _library()).llambda_cuda_fp8_session_run(
+            self._handle(), x.ctypes.data, x.shape[0], out.ctypes.data))
         return out[0] if one else out
 
     def run_device(self, x, out=None, *, out_dtype=None, stream=None):
@@ -353,8 +356,9 @@ class Fp8ProjectionSession(_Fp8Session):
         raw, ((out, ldo), work) = _on(stream, dev, (x, out), lambda: (
             _out(out, T, self.rows, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev) if nbytes else None))
-        _check((_lib or _library()).llambda_cuda_fp8_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T,
-              _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr() if nbytes else None, nbytes, raw))
+        _check((_lib or _library()).llambda_cuda_fp8_session_run_device(
+            h, _tag(x.dtype), x.data_ptr(), ldx, T, _tag(out.dtype), out.data_ptr(), ldo,
+            work.data_ptr() if nbytes else None, nbytes, raw))
         return out
 
     def run_quantized(self, q, scales, tokens: int, out=None, *, out_dtype=None, stream=None):
@@ -368,8 +372,8 @@ class Fp8ProjectionSession(_Fp8Session):
                        q.device, contiguous=True)
         raw, (out, ldo) = _on(stream, q.device, (q, scales, out), lambda: _out(
             out, tokens, self.rows, out_dtype or torch.float32, q.device))
-        _check((_lib or _library()).llambda_cuda_fp8_session_run_quantized(h, q.data_ptr(), scales.data_ptr(), tokens,
-              _tag(out.dtype), out.data_ptr(), ldo, raw))
+        _check((_lib or _library()).llambda_cuda_fp8_session_run_quantized(
+            h, q.data_ptr(), scales.data_ptr(), tokens, _tag(out.dtype), out.data_ptr(), ldo, raw))
         return out
 
 
@@ -392,7 +396,8 @@ class Fp8MoeSession(_Fp8Session):
         ts = [_fp8_tensor(p[0].shape, ptr(p[0]), ptr(p[1])) if p is not None
               else N.Fp8Tensor(0, 0, 0, None, None) for p in (gate, up, down)]
         h = C.c_void_p()
-        _check((_lib or _library()).llambda_cuda_fp8_moe_session_create(C.byref(ts[0]), C.byref(ts[1]), C.byref(ts[2]), on_device, C.byref(h)))
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_create(
+            *(C.byref(t) for t in ts), on_device, C.byref(h)))
         E, _, H = up[0].shape
         return cls(h, E, H, down[0].shape[1], device, (up, down, gate) if on_device else None)
 
@@ -424,7 +429,8 @@ class Fp8MoeSession(_Fp8Session):
                 or weights.shape != selected.shape:
             raise ValueError("selected and weights must both be [tokens][k]")
         out = np.empty((x.shape[0], self.out_features), np.float32)
-        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run(self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run(
+            self._handle(), x.ctypes.data, x.shape[0], selected.shape[1], selected.ctypes.data,
             weights.ctypes.data, out.ctypes.data))
         return out
 
@@ -443,7 +449,7 @@ class Fp8MoeSession(_Fp8Session):
         raw, ((out, ldo), work) = _on(stream, dev, (x, selected, weights, out), lambda: (
             _out(out, T, self.out_features, out_dtype or x.dtype, dev),
             _t.empty(nbytes, dtype=_t.uint8, device=dev)))
-        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run_device(h, _tag(x.dtype), x.data_ptr(), ldx, T, k,
-              selected.data_ptr(), weights.data_ptr(), _tag(out.dtype), out.data_ptr(), ldo,
-              work.data_ptr(), nbytes, raw))
+        _check((_lib or _library()).llambda_cuda_fp8_moe_session_run_device(
+            h, _tag(x.dtype), x.data_ptr(), ldx, T, k, selected.data_ptr(), weights.data_ptr(),
+            _tag(out.dtype), out.data_ptr(), ldo, work.data_ptr(), nbytes, raw))
         return out
