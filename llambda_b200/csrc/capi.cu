@@ -1552,11 +1552,10 @@ struct llambda_cuda_fp8_moe_session : F8Owner {
 
 namespace {
 
-void moe_call_sizes(const llambda_cuda_fp8_moe_session* s, size_t tokens, int top_k) {
+void moe_call_sizes(size_t tokens, int top_k) {
   token_count(tokens);
   if (top_k < 1 || top_k > 1024) throw Failure("top_k must be in 1..1024.");
   if (tokens * (size_t)top_k > (1u << 26)) throw Failure("Too many (token, expert) entries.");
-  (void)s;
 }
 
 }  // namespace
@@ -1845,7 +1844,7 @@ int llambda_cuda_fp8_moe_session_run(llambda_cuda_fp8_moe_session* s, const floa
     return -1;
   }
   return guarded([&] {
-    moe_call_sizes(s, tokens, top_k);
+    moe_call_sizes(tokens, top_k);
     std::lock_guard<std::mutex> lock(s->mu);
     DeviceGuard g(s->device);
     s->open_stream();
@@ -1878,7 +1877,7 @@ int llambda_cuda_fp8_moe_session_run_device(llambda_cuda_fp8_moe_session* s, int
     return -1;
   }
   return guarded([&] {
-    moe_call_sizes(s, tokens, top_k);
+    moe_call_sizes(tokens, top_k);
     DeviceGuard g(s->device);
     require_operand(x_type, device_x, ldx, tokens, s->m.up.cols, s->device, "input");
     require_operand(out_type, device_out, ldo, tokens, s->m.down.rows, s->device, "output");

@@ -1821,7 +1821,8 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   F8Pass p{};
   maps.w0 = m.gate.data ? m.gate.map : m.up.map;
   maps.w1 = m.up.map;
-  if (!f8_rows_map(&maps.x, base + L.xq, f8_pad16(m.up.cols), L.rows, m.up.cols, nt))
+  maps.x = maps.w1;  // not used by few entries' kernel
+  if (!few && !f8_rows_map(&maps.x, base + L.xq, f8_pad16(m.up.cols), L.rows, m.up.cols, nt))
     return cudaErrorInvalidValue;
   p.rows = m.up.rows;
   p.rblocks = f8_blocks(m.up.rows);
