@@ -106,10 +106,12 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, long i) {
 }
 
 // A choice in 64 bits as keys that compare in this order: the nearest double, the
-// rest of the sum that it rounds, the logit.  All 0: an expert that is out.
+// rest of the sum that it rounds (lo: as a float, so that sums of the same terms
+// in another order compare equal), the logit.  All 0: an expert that is out.
 struct Exact {
   unsigned long long k;
   uint32_t lo, l;
+  double rest;
 };
 __device__ __forceinline__ bool operator>(const Exact& a, const Exact& b) {
   return a.k != b.k ? a.k > b.k : a.lo != b.lo ? a.lo > b.lo : a.l > b.l;
@@ -125,7 +127,7 @@ __device__ __forceinline__ void take_two(Exact& a, Exact& b, const Exact& v) {  
 }
 __device__ __forceinline__ Exact shfl(const Exact& v, int lane) {
   return {__shfl_sync(kFull, v.k, lane), __shfl_sync(kFull, v.lo, lane),
-          __shfl_sync(kFull, v.l, lane)};
+          __shfl_sync(kFull, v.l, lane), __shfl_sync(kFull, v.rest, lane)};
 }
 // The warp's largest, and the lowest lane that has it.
 __device__ __forceinline__ Exact warp_max(const Exact& v, int& owner) {
@@ -137,6 +139,7 @@ __device__ __forceinline__ Exact warp_max(const Exact& v, int& owner) {
   r.l = warp_max(in ? v.l : 0u);
   in = in && v.l == r.l;
   owner = __ffs(__ballot_sync(kFull, in)) - 1;
+  r.rest = __shfl_sync(kFull, v.rest, owner);
   return r;
 }
 // a + b + c with |c| small beside the sum, or a, b doubles of any size (their sum
@@ -144,12 +147,13 @@ __device__ __forceinline__ Exact warp_max(const Exact& v, int& owner) {
 __device__ __forceinline__ Exact exact_sum(double a, double b, double c, uint32_t l) {
   const double s = a + b, t = s - a, e = ((a - (s - t)) + (b - t)) + c;
   const double hi = s + e;
-  if (!isfinite(hi)) return {order_key(s + c), 0u, 0u};
-  return {order_key(hi), order_key((float)(e - (hi - s))), l};
+  if (!isfinite(hi)) return {order_key(s + c), 0u, 0u, 0.0};
+  const double rest = e - (hi - s);
+  return {order_key(hi), order_key((float)rest), l, rest};
 }
 __device__ __forceinline__ Exact exact_choice(const RouteParams& r, const float* bias, float l,
                                               float m, double z, int e) {
-  if (l == -INFINITY) return {order_key((double)l), 0u, 0u};
+  if (l == -INFINITY) return {order_key((double)l), 0u, 0u, 0.0};
   const double b = bias ? (double)__ldg(bias + e) : 0.0;
   if (r.softmax) return exact_sum(b, exp((double)l - (double)m) / z, 0.0, order_key(l));
   // a positive logit's score as 1 less what is left
@@ -365,30 +369,24 @@ __device__ __forceinline__ bool choose(const RouteParams& r, const T* row, const
   return sure;
 }
 
-// The choice by Exact keys, in shared memory (32 R of 8 bytes, then of 4).
+// The choice by Exact keys; `shared` holds which experts are out (of lane i the bits of
+// its R), the keys are worked out anew where they are looked at.
 template <int R, typename T>
 __device__ __noinline__ int choose_exact(RouteParams r, const T* row, const float* bias,
                                          float m, double z, void* shared) {
   const int lane = threadIdx.x & 31;
   int sel = 0;
-  unsigned long long* ks = static_cast<unsigned long long*>(shared);
-  uint32_t* los = reinterpret_cast<uint32_t*>(ks + 32 * R);
+  uint32_t* out = static_cast<uint32_t*>(shared);
+  constexpr Exact kOut{0ull, 0u, 0u, 0.0};
   auto at = [&](int owner, int j) {  // expert owner * R + j
-    const int i = j * 32 + owner;
-    Exact v{ks[i], los[i], 0u};
-    if (v.k > 1ull && isfinite(key_value(v.k))) v.l = order_key(logit_at(row, owner * R + j));
-    return v;
+    const int e = owner * R + j;
+    if (e >= r.experts || (out[owner] >> j & 1u)) return kOut;
+    return exact_choice(r, bias, logit_at(row, e), m, z, e);
   };
-  constexpr Exact kOut{0ull, 0u, 0u};
+  out[lane] = 0u;
   Exact a = kOut, b = kOut;
 #pragma unroll(R < 4 ? R : 4)
-  for (int j = 0; j < R; ++j) {
-    const int e = lane * R + j;
-    const Exact v =
-        e < r.experts ? exact_choice(r, bias, logit_at(row, e), m, z, e) : kOut;
-    ks[j * 32 + lane] = v.k, los[j * 32 + lane] = v.lo;
-    take_two(a, b, v);
-  }
+  for (int j = 0; j < R; ++j) take_two(a, b, at(lane, j));
   if (r.top_groups < r.groups) {
     const int size = r.experts / r.groups, span = size / R;
     Exact g1 = kOut, g2 = kOut;  // lane g: group g's two largest
@@ -413,9 +411,7 @@ __device__ __noinline__ int choose_exact(RouteParams r, const T* row, const floa
     Exact rank_by = g1;
     if (r.group_top == 2) {
       const double d1 = key_value(g1.k), d2 = key_value(g2.k);
-      rank_by = exact_sum(d1, d2, isfinite(d1) && isfinite(d2)
-                                      ? (double)key_value(g1.lo) + (double)key_value(g2.lo)
-                                      : 0.0, 0u);
+      rank_by = exact_sum(d1, d2, g1.rest + g2.rest, 0u);
     }
     if (lane >= r.groups) rank_by = kOut;
     int rank = 0;
@@ -426,13 +422,9 @@ __device__ __noinline__ int choose_exact(RouteParams r, const T* row, const floa
     const unsigned kept = __ballot_sync(kFull, lane < r.groups && rank < r.top_groups);
     a = kOut;
     for (int j = 0; j < R; ++j) {
-      if (lane * R + j >= r.experts) break;
-      if (!(kept >> ((lane * R + j) / size) & 1u)) {
-        ks[j * 32 + lane] = 0ull;
-      } else {
-        const Exact v = at(lane, j);
-        if (v > a) a = v;
-      }
+      if (!(kept >> ((lane * R + j) / size & 31) & 1u)) out[lane] |= 1u << j;
+      const Exact v = at(lane, j);
+      if (v > a) a = v;
     }
   }
   __syncwarp();
@@ -442,7 +434,10 @@ __device__ __noinline__ int choose_exact(RouteParams r, const T* row, const floa
     Exact v = lane < R ? at(owner, lane) : kOut;  // lane j: the owner's j-th
     const int j = __ffs(__ballot_sync(kFull, v == best && lane < R)) - 1;
     if (lane == i) sel = owner * R + j;
-    if (lane == j) ks[j * 32 + owner] = 0ull, v = kOut;
+    if (lane == j) {
+      out[owner] |= 1u << j;
+      v = kOut;
+    }
     const Exact next = warp_max(v, one);
     if (lane == owner) a = next;
     __syncwarp();
@@ -508,13 +503,14 @@ __device__ __forceinline__ void load_logits(const __nv_bfloat16* p, float (&l)[R
   }
 }
 
-// One warp per token.  vec: every row starts on 16 bytes.
+// One warp per token.  vec: every row starts on 16 bytes.  The rare passes' registers are
+// bounded (R 8: 72 and 18.5 us for 8191 tokens, 64 and 18.2; R 32: 194 without a bound).
 template <typename T, int R>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, R <= 8 ? 8 : 4)
     route_kernel(const RouteParams r, const T* __restrict__ logits, long ld,
                  const float* __restrict__ bias, int tokens, int* __restrict__ selected,
                  float* __restrict__ weights, int vec) {
-  __shared__ unsigned long long s_keys[kRouteWarps][R == 1 ? 64 : 48 * R];  // 12 bytes an expert
+  __shared__ unsigned long long s_keys[kRouteWarps][32 * (R + 1)];
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;

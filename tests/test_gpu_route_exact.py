@@ -240,3 +240,17 @@ def test_weights_of_the_farthest_logits():
         bias[15], logits[:2, 15] = -5.0, 0.0
         sel, w = LB.route_experts(logits, 4, score="softmax", bias=bias)
         assert w[0].tolist() == [0.25] * 4 and 15 not in sel[0].tolist()
+
+
+@pytest.mark.parametrize("big", [1.0, 100.0, 1e6])
+def test_sums_of_the_same_terms_in_other_pairs_tie(big):
+    """(l + B) + (l' - B) and (l' + B) + (l - B): a true tie, whatever each choice rounds."""
+    g = gen(int(big))
+    T, E = 60, 64
+    for levels in ([18.0, 18.5, 19.0, 19.5], [40.0, 40.5, 45.0, 50.0], [-20.0, -3.0, 0.5, 2.0]):
+        lv = torch.tensor(levels, device="cuda")
+        logits = lv[torch.randint(0, 4, (T, E), generator=g, device="cuda")]
+        bias = big * (2.0 * torch.randint(0, 2, (E,), generator=g, device="cuda") - 1.0)
+        for groups, top_groups in ((32, 13), (16, 5)):
+            check_choice(logits, 8, "sigmoid", bias, groups=groups, top_groups=top_groups,
+                         group_top=2)
