@@ -1336,7 +1336,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1)
         // fifth stage of operands.  1024 x 8192 x 512 bf16 20.5 -> 18.6 us, 2048 x
         // 14336 x 4096 133 -> 129 (fp32 147 -> 141), 512 x 14336 x 8192 78.7 -> 79.4;
         // five stages and half the room 137.  Tensor copies, a warp's or by one
-        // warp for all, gained no more.
+        // warp for all, gained no more.  (Each pair of figures is of one run; the
+        // clock moves them by a few per cent between runs.)
         uint8_t* o = static_cast<uint8_t*>(p.out) + ((long)(t0 + lane) * p.ldo + n0) * size;
         const bool valid = t0 + lane < p.tokens;
         if (p.out_bf16) {
@@ -1797,7 +1798,8 @@ cudaError_t launch_f8_moe(const F8Moe& m, bool x_bf16, const void* x, long ldx, 
   // the entries up (one token, 10 of 512 experts: 18 us against 31).  With more tiles the
   // fence after each, and the weights that the plan's own launch lets the gate
   // and up product request ahead, cost more (32 tokens, 6 of 128 experts of 2688 x
-  // 1856: 215 us against 157).
+  // 1856: 215 us against 157).  Its CTAs hold kStepBlocks blocks of K: wider layers
+  // whose K is not shared (H above 2688) take five launches at one token too.
   const int kb_up = f8_blocks(m.up.cols), rb_up = f8_blocks(m.up.rows);
   const int split_up = f8_split(chunks * rb_up, kb_up);
   const bool few = n <= kF8StepEntries && nt == 16 &&
