@@ -295,3 +295,48 @@ def test_experts_of_wide_layers(T, E, k, H, I, gated):
         want.index_add_(0, t, w * y)
         bound.index_add_(0, t, w.abs() * (dy + mag + 4 * U32 * y.abs()))
     check(out, want, bound * (1 + k * U32))
+
+
+def test_a_captured_call_on_a_forked_stream():
+    """stream= inside a capture: inputs made and dropped in it, replayed on new values."""
+    g = gen(8)
+    E, k, H = 8, 2, 256
+    m = LB.Fp8MoeSession.from_device(up=matrices(g, E, 128, H), down=matrices(g, E, H, 128))
+    p = LB.Fp8ProjectionSession.from_device(*matrices(g, H, H))
+    bias = 0.1 * randn(g, E)
+    router = randn(g, H, E) / 16
+
+    def run(x, side):
+        here = torch.cuda.current_stream()
+        h = p.run_device(x)
+        logits, h2 = h @ router, h + 1.0
+        side.wait_stream(here)
+        sel, wt = LB.route_experts(logits, k, score="sigmoid", bias=bias, stream=side)
+        del logits
+        out = m.run_device(h, sel, wt, stream=side)
+        del h
+        q, s = LB.fp8_quantize(h2, stream=side)
+        del h2
+        junk = torch.full((4 * T, H), 9.0, device="cuda")  # beside them, in memory that is free
+        here.wait_stream(side)
+        del junk
+        return sel, wt, out, q, s
+
+    for T in (3, 130):
+        x = randn(g, T, H)
+        side = torch.cuda.Stream()
+        run(x, side)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = run(x, side)
+        for _ in range(3):
+            new = randn(g, T, H)
+            x.copy_(new)
+            gr.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in res]
+            want = run(new, side)
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
